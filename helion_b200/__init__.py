@@ -11,6 +11,7 @@ from .install import install, uninstall
 from .matmul_ops import matmul, matmul_vec
 from .norm_ops import residual_rmsnorm, rmsnorm, rmsnorm_backward
 from .optim_ops import adamw_step, clip_grad_norm, grad_sumsq
+from .rope_ops import qk_norm_rope, rope, rope_frequencies
 from .ops import linear_cross_entropy, linear_cross_entropy_backward
 
 __all__ = [
@@ -25,9 +26,12 @@ __all__ = [
     "linear_cross_entropy_backward",
     "matmul",
     "matmul_vec",
+    "qk_norm_rope",
     "residual_rmsnorm",
     "rmsnorm",
     "rmsnorm_backward",
+    "rope",
+    "rope_frequencies",
     "sample_head",
     "topk_head",
     "uninstall",

@@ -17,6 +17,14 @@ FLAG_FORCE_SIMT, FLAG_FORCE_TC, FLAG_DX_F32, FLAG_NO_DX, FLAG_NO_DW, FLAG_ONE_CT
 
 REDUCTIONS = {"none": REDUCTION_NONE, "mean": REDUCTION_MEAN, "sum": REDUCTION_SUM}
 
+class HeadRows(ctypes.Structure):
+    """``lce_head_rows`` of include/helion_lce.h."""
+
+    _fields_ = [("x", c_void_p), ("x_stride", c_int64 * 3), ("out", c_void_p), ("out_stride", c_int64 * 3),
+                ("grad", c_void_p), ("grad_stride", c_int64 * 3), ("weight", c_void_p), ("dweight", c_void_p),
+                ("heads", c_int64)]
+
+
 # name -> (restype, argtypes); mirrors include/helion_lce.h declaration by declaration
 SIGNATURES = {
     "lce_version": (c_int, []),
@@ -67,6 +75,14 @@ SIGNATURES = {
     "lce_rmsnorm_plan": (c_int, [c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "lce_rmsnorm_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                      c_int64, ctypes.c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "lce_rope": (c_int, [ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int,
+                         ctypes.c_float, c_int, c_int, c_void_p]),
+    "lce_qk_norm_rope_forward": (c_int, [ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
+                                         c_void_p, c_int64, c_int, ctypes.c_float, ctypes.c_float, c_int, c_void_p]),
+    "lce_qk_norm_rope_backward_workspace_bytes": (c_size_t, [c_int64]),
+    "lce_qk_norm_rope_backward": (c_int, [ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
+                                          c_void_p, c_int64, c_int, ctypes.c_float, ctypes.c_float, c_int, c_void_p, c_size_t,
+                                          c_void_p]),
     "lce_set_tuning": (None, [c_int, c_int, c_int]),
     "lce_debug_wait_test": (c_int, [ctypes.c_ulonglong, c_uint]),
     "lce_debug_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int,

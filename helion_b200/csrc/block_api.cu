@@ -1,0 +1,222 @@
+// extern "C" entry points of the operators of a decoder block around the head (declared in include/helion_lce.h):
+// rotary positions and the query / key norms. Argument checks, the choice of kernel form, and the launches.
+#include "api_common.cuh"
+#include "rope_kernels.cuh"
+
+namespace lce {
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// rotary positions, query / key norms
+// ---------------------------------------------------------------------------------------------
+struct HeadCall {
+    long long batch, seq, dim, half;
+    int interleaved, mode, dtype, sm_count;
+};
+
+// Whether every row, and every pair of vectors that rotate together, is made of whole aligned `vec`-element vectors.
+bool head_rows_vectors(const lce_head_rows& r, const HeadCall& c, long long vec, uintptr_t bytes) {
+    auto fits = [&](const void* p, const int64_t* stride) {
+        return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride[0] % vec == 0 && stride[1] % vec == 0 && stride[2] % vec == 0;
+    };
+    if (r.heads == 0) return true;
+    if (!fits(r.x, r.x_stride) || !fits(r.out, r.out_stride)) return false;
+    if (c.mode == kHeadNormBackward && !fits(r.grad, r.grad_stride)) return false;
+    return c.mode == kHeadRope || reinterpret_cast<uintptr_t>(r.weight) % bytes == 0;
+}
+
+int check_head_rows(const lce_head_rows* r, const HeadCall& c) {
+    if (!r || r->heads < 0) return LCE_ERR_ARG;
+    if (r->heads > 0x7fffffll / 32) return LCE_ERR_TOO_LARGE;
+    if (r->heads == 0 || c.batch == 0 || c.seq == 0) return LCE_OK;
+    if (!r->x || !r->out) return LCE_ERR_ARG;
+    if (c.mode != kHeadRope && !r->weight) return LCE_ERR_ARG;
+    if (c.mode == kHeadNormBackward && !r->grad) return LCE_ERR_ARG;
+    return LCE_OK;
+}
+
+// Deals `tokens` x `heads` rows to warps: whole tokens per warp (their angles are formed once) as long as that gives
+// every SM `kWarps` warps, pieces of a token otherwise. A step is `per_step` heads.
+template <class T>
+HeadRows<T> deal_heads(const lce_head_rows& r, const HeadCall& c, int per_step, int warps_per_cta, long long max_ctas) {
+    HeadRows<T> h;
+    h.x = static_cast<const T*>(r.x);
+    h.x_b = r.x_stride[0], h.x_s = r.x_stride[1], h.x_h = r.x_stride[2];
+    h.dy = static_cast<const T*>(r.grad);
+    h.dy_b = r.grad_stride[0], h.dy_s = r.grad_stride[1], h.dy_h = r.grad_stride[2];
+    h.out = static_cast<T*>(r.out);
+    h.o_b = r.out_stride[0], h.o_s = r.out_stride[1], h.o_h = r.out_stride[2];
+    h.weight = static_cast<const T*>(r.weight);
+    h.partial = nullptr;
+    h.heads = static_cast<int>(r.heads);
+    const long long tokens = c.batch * c.seq, total_steps = cdiv(r.heads, per_step);
+    if (tokens == 0 || total_steps == 0) {
+        h.chunks = h.steps = 1;
+        h.units = 0;
+        h.ctas = 0;
+        return h;
+    }
+    constexpr long long kWarps = 16;
+    long long steps = total_steps * tokens / (kWarps * c.sm_count);
+    steps = steps < 1 ? 1 : (steps > total_steps ? total_steps : steps);
+    h.steps = static_cast<int>(steps);
+    h.chunks = static_cast<int>(cdiv(total_steps, steps));
+    h.units = tokens * h.chunks;
+    const long long want = cdiv(h.units, warps_per_cta);
+    h.ctas = static_cast<int>(want < max_ctas ? want : max_ctas);
+    return h;
+}
+
+template <class T, bool INTERLEAVED, int MODE>
+int launch_heads(const HeadCall& c, const lce_head_rows& q, const lce_head_rows& k, RopePlan p, float* partial, cudaStream_t s) {
+    constexpr int VEC = RmsTile<T>::kVec;
+    const long long pair = INTERLEAVED ? 2 * c.half : c.half;  // what has to be whole vectors besides the rows
+    const long long np = c.half / VEC, nv = c.dim / VEC;
+    const int items = static_cast<int>(INTERLEAVED ? cdiv(nv, 2) : np + cdiv(nv - 2 * np, 2));
+    const bool vector = c.dim % VEC == 0 && pair % VEC == 0 && items <= 32 && head_rows_vectors(q, c, VEC, 16) &&
+                        head_rows_vectors(k, c, VEC, 16);
+    p.items = items;
+    p.lanes = 1;
+    while (p.lanes < items) p.lanes <<= 1;
+    p.pairs2 = c.dim % 2 == 0 && head_rows_vectors(q, c, 2, 2 * sizeof(T)) && head_rows_vectors(k, c, 2, 2 * sizeof(T));
+    const int per_step = vector ? 32 / p.lanes : 1;
+    const int warps = vector ? kHeadWarps : kRowFormWarps;
+    // The backward keeps sums over everything a warp walks, so its grid is what fits the GPU at once, shared between
+    // q and k by their numbers of heads; the others launch one warp per unit.
+    const long long all = q.heads + k.heads;
+    auto share = [&](long long heads) {
+        if (MODE != kHeadNormBackward) return 1ll << 20;
+        const long long fit = c.sm_count * (vector ? 2ll : 3ll);
+        const long long cap = (fit < kHeadMaxCtas ? fit : kHeadMaxCtas) * heads / (all > 0 ? all : 1);
+        return cap < 1 ? 1ll : cap;
+    };
+    HeadRows<T> hq = deal_heads<T>(q, c, per_step, warps, share(q.heads));
+    HeadRows<T> hk = deal_heads<T>(k, c, per_step, warps, share(k.heads));
+    if (MODE == kHeadNormBackward) {
+        if (q.dweight) hq.partial = partial;
+        if (k.dweight) hk.partial = partial + static_cast<long long>(hq.ctas) * c.dim;
+    }
+    if (hq.ctas + hk.ctas > 0) {
+        if (vector) {
+            const int smem = kHeadWarps * items * VEC * static_cast<int>(sizeof(float2));
+            heads_vector_kernel<T, INTERLEAVED, MODE><<<hq.ctas + hk.ctas, kHeadThreads, smem, s>>>(hq, hk, p);
+        } else {
+            const int smem = kRowFormWarps * row_form_floats(p.dim, p.half, MODE) * 4;
+            auto kern = heads_row_kernel<T, INTERLEAVED, MODE>;
+            if (smem > 48 * 1024 && cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)))
+                return LCE_ERR_CUDA;
+            kern<<<hq.ctas + hk.ctas, kRowFormWarps * 32, smem, s>>>(hq, hk, p);
+        }
+        LCE_COUNT_LAUNCH();
+        if (cuda_failed(cudaGetLastError())) return LCE_ERR_CUDA;
+    }
+    if (MODE == kHeadNormBackward && (q.dweight || k.dweight)) {
+        // cudaLaunchKernelEx takes one grid dimension through launch_dependent; this one has two
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(cdiv(c.dim, 32)), 2);
+        cfg.blockDim = dim3(32, 32);
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 1 : 0;
+        const cudaError_t err = cudaLaunchKernelEx(&cfg, head_dweight_kernel<T>, static_cast<const float*>(hq.partial), hq.ctas,
+                                                   static_cast<T*>(q.dweight), static_cast<const float*>(hk.partial), hk.ctas,
+                                                   static_cast<T*>(k.dweight), p.dim);
+        LCE_COUNT_LAUNCH();
+        if (cuda_failed(err)) return LCE_ERR_CUDA;
+    }
+    return LCE_OK;
+}
+
+template <int MODE>
+int dispatch_heads(const HeadCall& c, const lce_head_rows& q, const lce_head_rows& k, const RopePlan& p, float* partial, cudaStream_t s) {
+    switch (c.dtype) {
+        case LCE_DTYPE_BF16:
+            return c.interleaved ? launch_heads<__nv_bfloat16, true, MODE>(c, q, k, p, partial, s)
+                                 : launch_heads<__nv_bfloat16, false, MODE>(c, q, k, p, partial, s);
+        case LCE_DTYPE_F16:
+            return c.interleaved ? launch_heads<__half, true, MODE>(c, q, k, p, partial, s)
+                                 : launch_heads<__half, false, MODE>(c, q, k, p, partial, s);
+        default:
+            return c.interleaved ? launch_heads<float, true, MODE>(c, q, k, p, partial, s)
+                                 : launch_heads<float, false, MODE>(c, q, k, p, partial, s);
+    }
+}
+
+template <int MODE>
+int heads_call(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, int64_t seq, int64_t dim, const void* positions,
+               int pos_i64, int64_t pos_b, int64_t pos_s, const double* freq, int64_t half, int interleaved, float scale,
+               int inverse, float eps, int dtype, void* ws, size_t ws_bytes, void* stream) {
+    if (!known_dtype(dtype) || batch < 0 || seq < 0 || dim < 1 || half < 0 || 2 * half > dim) return LCE_ERR_ARG;
+    if (dim > kHeadMaxDim || batch > 0x7fffffffll || seq > 0x7fffffffll || batch * seq > (1ll << 40)) return LCE_ERR_TOO_LARGE;
+    HeadCall c{batch, seq, dim, half, interleaved, MODE, dtype, 0};
+    int rc = check_head_rows(q, c);
+    if (rc) return rc;
+    const lce_head_rows none = {};
+    const lce_head_rows& kr = k ? *k : none;
+    if (k && (rc = check_head_rows(k, c))) return rc;
+    const bool work = batch > 0 && seq > 0 && (q->heads > 0 || kr.heads > 0);
+    if (!work && !(MODE == kHeadNormBackward && (q->dweight || kr.dweight))) return LCE_OK;
+    if (work && (!positions || (half > 0 && !freq))) return LCE_ERR_ARG;
+    if (MODE == kHeadNormBackward && (q->dweight || kr.dweight) &&
+        (!ws || ws_bytes < lce_qk_norm_rope_backward_workspace_bytes(dim)))
+        return LCE_ERR_WS_TOO_SMALL;
+    DeviceInfo* d;
+    if ((rc = device_basics(&d))) return rc;
+    c.sm_count = d->sm_count;
+    RopePlan p;
+    p.pos = positions;
+    p.pos_i64 = pos_i64;
+    p.pos_b = pos_b;
+    p.pos_s = pos_s;
+    p.freq = freq;
+    p.half = static_cast<int>(half);
+    p.dim = static_cast<int>(dim);
+    p.items = p.lanes = 1;
+    p.pairs2 = 0;
+    p.seq = seq > 0 ? seq : 1;
+    p.scale = scale;
+    p.sin_sign = inverse ? -1.f : 1.f;
+    p.eps = eps;
+    return dispatch_heads<MODE>(c, *q, kr, p, static_cast<float*>(ws), static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace lce
+
+using namespace lce;
+
+extern "C" {
+
+int lce_rope(const lce_head_rows* rows, int64_t batch, int64_t seq, int64_t dim, const void* positions, int pos_i64,
+             int64_t pos_b, int64_t pos_s, const double* freq, int64_t half, int interleaved, float scale, int inverse,
+             int dtype, void* stream) {
+    return heads_call<kHeadRope>(rows, nullptr, batch, seq, dim, positions, pos_i64, pos_b, pos_s, freq, half, interleaved,
+                                 scale, inverse, 0.f, dtype, nullptr, 0, stream);
+}
+
+int lce_qk_norm_rope_forward(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, int64_t seq, int64_t dim,
+                             const void* positions, int pos_i64, int64_t pos_b, int64_t pos_s, const double* freq,
+                             int64_t half, int interleaved, float scale, float eps, int dtype, void* stream) {
+    if (!k) return LCE_ERR_ARG;
+    return heads_call<kHeadNorm>(q, k, batch, seq, dim, positions, pos_i64, pos_b, pos_s, freq, half, interleaved, scale, 0,
+                                 eps, dtype, nullptr, 0, stream);
+}
+
+size_t lce_qk_norm_rope_backward_workspace_bytes(int64_t dim) {
+    if (dim < 1 || dim > kHeadMaxDim) return 0;
+    return static_cast<size_t>(kHeadMaxCtas + 1) * dim * sizeof(float);
+}
+
+int lce_qk_norm_rope_backward(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, int64_t seq, int64_t dim,
+                              const void* positions, int pos_i64, int64_t pos_b, int64_t pos_s, const double* freq,
+                              int64_t half, int interleaved, float scale, float eps, int dtype, void* ws, size_t ws_bytes,
+                              void* stream) {
+    if (!k) return LCE_ERR_ARG;
+    return heads_call<kHeadNormBackward>(q, k, batch, seq, dim, positions, pos_i64, pos_b, pos_s, freq, half, interleaved,
+                                         scale, 1, eps, dtype, ws, ws_bytes, stream);
+}
+
+}  // extern "C"

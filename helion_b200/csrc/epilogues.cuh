@@ -11,25 +11,12 @@
 #include <type_traits>
 
 #include "gemm_tc.cuh"
+#include "vec.cuh"
 
 namespace lce {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-
-template <class T> struct Cvt;
-template <> struct Cvt<__nv_bfloat16> {
-    static __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-    static __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
-};
-template <> struct Cvt<__half> {
-    static __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-    static __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
-};
-template <> struct Cvt<float> {
-    static __device__ __forceinline__ float to_f(float x) { return x; }
-    static __device__ __forceinline__ float from_f(float x) { return x; }
-};
 
 __device__ __forceinline__ long long load_target(const void* tgt, int is_i64, long long i) {
     return is_i64 ? static_cast<const long long*>(tgt)[i]

@@ -3,14 +3,12 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
-#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
-#include <mutex>
 #include <type_traits>
 
-#include "../../include/helion_lce.h"
+#include "api_common.cuh"
 #include "gemm_simt.cuh"
 #include "gemm_tc.cuh"
 #include "ce_kernels.cuh"
@@ -34,51 +32,23 @@ constexpr int kBN = 256;
 constexpr int kStages1 = 4;  // 48 KB stages, one CTA per tile
 constexpr int kStages2 = 6;  // 32 KB stages, CTA pair per tile
 constexpr size_t kDefaultBlockBytes = 256ull << 20;
-constexpr int kMaxDevices = 64;
 
-struct DeviceInfo {
-    bool ready = false;
-    int index = 0;
-    int sm_count = 0;
-    int cc_major = 0;
-    int* status_ptr = nullptr;
-    unsigned* done_counters = nullptr;  // kDoneSlots of them, zero when idle
-    mutable std::atomic<unsigned> next_done_slot{0};
-};
-
-DeviceInfo g_dev[kMaxDevices];
-std::mutex g_mutex;
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-std::atomic<unsigned long long> g_launches{0};  // kernels this library has launched (all devices)
-#define LCE_COUNT_LAUNCH() g_launches.fetch_add(1, std::memory_order_relaxed)
 
-// The CUDA error behind the last LCE_ERR_CUDA of this thread (lce_last_cuda_error reports its name).
-thread_local cudaError_t t_last_cuda_error = cudaSuccess;
-inline bool cuda_failed(cudaError_t e) {
-    if (e == cudaSuccess) return false;
-    t_last_cuda_error = e;
-    return true;
-}
-
+// device_basics plus what the kernels of this file need: the status word, the completion counters and the
+// tensor-map encoder.
 int device_info(DeviceInfo** out) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return LCE_ERR_CUDA;
-    if (dev < 0 || dev >= kMaxDevices) return LCE_ERR_ARG;
+    DeviceInfo* basics;
+    const int rc = device_basics(&basics);
+    if (rc) return rc;
     std::lock_guard<std::mutex> lock(g_mutex);
-    DeviceInfo& d = g_dev[dev];
+    DeviceInfo& d = *basics;
     if (!d.ready) {
-        d.index = dev;
-        if (cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-            return LCE_ERR_CUDA;
-        if (cudaDeviceGetAttribute(&d.cc_major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
-            return LCE_ERR_CUDA;
-        if (d.cc_major == 10) {
-            void* p = nullptr;
-            if (cudaGetSymbolAddress(&p, g_device_status) != cudaSuccess) return LCE_ERR_CUDA;
-            d.status_ptr = static_cast<int*>(p);
-            if (cudaGetSymbolAddress(&p, g_done_counters) != cudaSuccess) return LCE_ERR_CUDA;
-            d.done_counters = static_cast<unsigned*>(p);
-        }
+        void* p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_device_status) != cudaSuccess) return LCE_ERR_CUDA;
+        d.status_ptr = static_cast<int*>(p);
+        if (cudaGetSymbolAddress(&p, g_done_counters) != cudaSuccess) return LCE_ERR_CUDA;
+        d.done_counters = static_cast<unsigned*>(p);
         d.ready = true;
     }
     if (g_encode == nullptr) {
@@ -90,12 +60,8 @@ int device_info(DeviceInfo** out) {
         g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     }
     *out = &d;
-    return d.cc_major == 10 ? LCE_OK : LCE_ERR_ARCH;
+    return LCE_OK;
 }
-
-inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
-inline size_t align_up(size_t a, size_t b) { return (a + b - 1) / b * b; }
-inline size_t elem_size(int dtype) { return dtype == LCE_DTYPE_F32 ? 4 : 2; }
 
 // 2-D tensor map over a row-major 16-bit matrix: `inner` contiguous elements per row, `outer`
 // rows, `pitch_bytes` between rows; 128-byte swizzle; out-of-range elements read as zero.
@@ -191,30 +157,6 @@ struct Tuning {
     }
 };
 Tuning g_tuning;
-
-// Programmatic dependent launch (HELION_B200_PDL=0 switches it off): kernels that call ptx::grid_dep_wait()
-// before they read anything their predecessor in the stream wrote may be launched while that predecessor is
-// still running; their launch latency and set-up then hide under its tail.
-inline bool pdl_enabled() {
-    static const bool kEnabled = [] { const char* e = getenv("HELION_B200_PDL"); return e ? atoi(e) != 0 : true; }();
-    return kEnabled;
-}
-
-// Launches such a kernel (no dynamic shared memory). Only for kernels that contain the wait.
-template <class... KArgs, class... Args>
-cudaError_t launch_dependent(void (*kern)(KArgs...), int grid, int block, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = 0;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
-}
 
 template <int CG, bool A_MN, bool B_MN, bool IS_BF16, class Epi>
 int launch_tc_cg(const DeviceInfo& d, const Mat& a, const Mat& b, long long M, long long Nn, long long K,
@@ -449,8 +391,6 @@ int launch_simt(const DeviceInfo& d, const Mat& a, bool a_mn, const Mat& b, bool
     LCE_COUNT_LAUNCH();
     return (cuda_failed(cudaGetLastError()) ? LCE_ERR_CUDA : LCE_OK);
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // The tcgen05 path needs 16-bit inputs, 16-byte aligned bases and row pitches (H % 8 == 0).
 int choose_path(int dtype, long long H, const void* x, const void* w, unsigned flags, bool* use_tc) {

@@ -27,72 +27,6 @@ namespace lce {
 constexpr int kRmsMaxThreads = 256;
 constexpr int kRmsMaxPartials = 592;  // backward CTAs = partial dweight rows (4 per SM on 148 SMs)
 
-template <class T>
-struct RmsTile {
-    static constexpr int kVec = 16 / sizeof(T);
-    static constexpr int kMaxVpt = 8;  // 256 threads x 8 vectors: 16384 16-bit or 8192 fp32 columns
-};
-
-// Columns c .. c + VEC of one row as a raw 16-byte vector; columns at or beyond H read as zero.
-template <class T, bool VECTOR>
-__device__ __forceinline__ uint4 rms_load(const T* __restrict__ row, int c, int H) {
-    constexpr int VEC = RmsTile<T>::kVec;
-    if (VECTOR) {
-        return c < H ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
-    } else {
-        alignas(16) T tmp[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) tmp[j] = (c + j < H) ? row[c + j] : Cvt<T>::from_f(0.f);
-        return *reinterpret_cast<const uint4*>(tmp);
-    }
-}
-
-// 16-byte vector <-> floats. The 16-bit forms convert two elements per instruction where the hardware
-// can (bf16 -> fp32 is a shift or a mask of the packed word; fp32 -> 16-bit pairs is one cvt).
-template <class T>
-__device__ __forceinline__ void rms_unpack(const uint4& raw, float (&v)[RmsTile<T>::kVec]) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    if constexpr (std::is_same<T, float>::value) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]);
-    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[2 * j] = __uint_as_float(w[j] << 16);
-            v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-            v[2 * j] = f.x;
-            v[2 * j + 1] = f.y;
-        }
-    }
-}
-
-template <class T>
-__device__ __forceinline__ uint4 rms_pack(const float (&v)[RmsTile<T>::kVec]) {
-    uint32_t w[4];
-    if constexpr (std::is_same<T, float>::value) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(v[j]);
-    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
 // 1 / sqrt(ss / H + eps) from a precomputed 1 / H: the hardware reciprocal square root plus one Newton
 // step (relative error ~1e-7) - an exactly rounded divide and square root would cost every thread more
 // instructions than the rest of its row.
@@ -100,20 +34,6 @@ __device__ __forceinline__ float rms_rstd(float ss, float inv_h, float eps) {
     const float a = fmaf(ss, inv_h, eps);
     const float y = rsqrtf(a);
     return y * fmaf(-0.5f * a * y, y, 1.5f);
-}
-
-template <class T, bool VECTOR>
-__device__ __forceinline__ void rms_store(T* __restrict__ row, int c, int H, const uint4& raw) {
-    constexpr int VEC = RmsTile<T>::kVec;
-    if (VECTOR) {
-        if (c < H) *reinterpret_cast<uint4*>(row + c) = raw;
-    } else {
-        alignas(16) T tmp[VEC];
-        *reinterpret_cast<uint4*>(tmp) = raw;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (c + j < H) row[c + j] = tmp[j];
-    }
 }
 
 template <int N> struct RmsLog2 { static constexpr int value = 1 + RmsLog2<N / 2>::value; };

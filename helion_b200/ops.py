@@ -176,9 +176,11 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """Scratch for one C-ABI call. Small requests (latency-bound problems, where an allocation is a visible
     share of the call) reuse one buffer per (device, stream): calls on one stream run in order, so they may
     share scratch; calls on different streams get different buffers. Large requests are allocated per call and
-    go back to torch's caching allocator afterwards."""
+    go back to torch's caching allocator afterwards. So are all requests while the stream is being captured: a
+    graph keeps using its scratch whenever it is replayed, possibly beside other work of any stream, so its
+    scratch has to come from the graph's own pool."""
     nbytes = max(int(nbytes), 256)
-    if nbytes > _WS_CACHE_MAX:
+    if nbytes > _WS_CACHE_MAX or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index if device.index is not None else torch.cuda.current_device(), _stream(device))
     buf = _ws_cache.get(key)

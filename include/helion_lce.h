@@ -297,6 +297,45 @@ int lce_rmsnorm_backward(const void* dy, const void* x, const void* weight, cons
                          const void* dresidual, void* dx, void* dweight, int64_t n_rows, int64_t hidden, float eps,
                          int dtype, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- rotary positions, and the norm of every query and key head in the same pass --------------
+ * angle_i = position * frequencies[i] (radians, formed in 64 bits), i < half; the first 2 * half <= dim elements
+ * of every head are rotated in pairs: (x[i], x[half + i]), or (x[2i], x[2i + 1]) with interleaved != 0:
+ *   (a, b) -> scale * (a cos - b sin, b cos + a sin);   elements from 2 * half on pass through.
+ * lce_rope with inverse != 0 turns by the negative angles: the backward pass, given the output's gradient as x.
+ * lce_qk_norm_rope_* first normalise each head, n = x * rsqrt(mean(x^2) + eps) * weight, and rotate n; q and k
+ * share positions and frequencies and go in one launch. The backward reads the forward's INPUT (x) and the
+ * gradient of the rotated output (grad), writes the input's gradient to out and, where dweight is not NULL, the
+ * weight's; dweight is summed in a fixed order (the same bits on every run).
+ * Tensors are [batch][seq][heads][dim] with element strides for the first three and dim contiguous; dim is at most
+ * 1024; positions are int32 or int64 at batch * pos_stride_batch + seq * pos_stride_seq (a stride of 0 broadcasts),
+ * any value. Rows in whole 16-byte vectors (pointers, strides, dim and the rotated pairs) take the vector kernels,
+ * everything else a form that stages rows in shared memory. heads, batch or seq of 0 launch nothing, except that
+ * dweight is then set to zero. No counterpart in the reference's fused loss; its rotary op is tritium/ops/rope.py. */
+typedef struct lce_head_rows {
+    const void* x;
+    int64_t x_stride[3]; /* batch, seq, head, in elements */
+    void* out;
+    int64_t out_stride[3];
+    const void* grad; /* backward only */
+    int64_t grad_stride[3];
+    const void* weight; /* [dim]; not read by lce_rope */
+    void* dweight;      /* [dim]; backward only, may be NULL */
+    int64_t heads;
+} lce_head_rows;
+
+int lce_rope(const lce_head_rows* rows, int64_t batch, int64_t seq, int64_t dim, const void* positions,
+             int positions_are_i64, int64_t pos_stride_batch, int64_t pos_stride_seq, const double* frequencies,
+             int64_t half, int interleaved, float scale, int inverse, int dtype, void* stream);
+int lce_qk_norm_rope_forward(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, int64_t seq, int64_t dim,
+                             const void* positions, int positions_are_i64, int64_t pos_stride_batch,
+                             int64_t pos_stride_seq, const double* frequencies, int64_t half, int interleaved,
+                             float scale, float eps, int dtype, void* stream);
+size_t lce_qk_norm_rope_backward_workspace_bytes(int64_t dim);
+int lce_qk_norm_rope_backward(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, int64_t seq, int64_t dim,
+                              const void* positions, int positions_are_i64, int64_t pos_stride_batch,
+                              int64_t pos_stride_seq, const double* frequencies, int64_t half, int interleaved,
+                              float scale, float eps, int dtype, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- test hook (not part of the product interface) -------------------------------------------
  * Test infrastructure only: nothing above depends on it, a binding for the reference needs no stub
  * for it, and it may change without notice.

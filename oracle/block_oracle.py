@@ -1,0 +1,45 @@
+"""Plain float64 definitions of the operators of a decoder block around the head: rotary positions, query / key
+norms, projections with their epilogue and the sampler. What the tests compare the kernels with; any device."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+
+def rope(x, positions, frequencies, interleaved=False, scale=1.0, inverse=False):
+    """float64 rotation of the first 2 * len(frequencies) elements of the last dimension of x [..., heads, dim]."""
+    x = x.double()
+    angle = positions.double()[..., None, None] * frequencies.double()
+    if inverse:
+        angle = -angle
+    cos, sin = torch.cos(angle) * scale, torch.sin(angle) * scale
+    half = frequencies.shape[0]
+    out = x.clone()
+    a, b = (slice(0, 2 * half, 2), slice(1, 2 * half, 2)) if interleaved else (slice(0, half), slice(half, 2 * half))
+    out[..., a] = x[..., a] * cos - x[..., b] * sin
+    out[..., b] = x[..., b] * cos + x[..., a] * sin
+    return out
+
+
+def head_norm(x, weight, eps):
+    x = x.double()
+    return x / torch.sqrt(x.pow(2).mean(-1, keepdim=True) + eps) * weight.double()
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, interleaved=False, scale=1.0):
+    return tuple(rope(head_norm(t, w, eps), positions, frequencies, interleaved, scale)
+                 for t, w in ((q, q_weight), (k, k_weight)))
+
+
+def head_norm_rope_backward(dy, x, weight, positions, frequencies, eps=1e-6, interleaved=False, scale=1.0):
+    """(dx, dweight, magnitude of dweight's terms) from the formula, float64."""
+    g = rope(dy, positions, frequencies, interleaved, scale, inverse=True)
+    x, weight = x.double(), weight.double()
+    rstd = (x.pow(2).mean(-1, keepdim=True) + eps).rsqrt()
+    unit = x * rstd
+    gw = g * weight
+    dx = rstd * (gw - unit * (gw * unit).mean(-1, keepdim=True))
+    terms = (g * unit).flatten(0, -2)
+    return dx, terms.sum(0), terms.abs().sum(0)
