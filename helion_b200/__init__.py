@@ -8,11 +8,12 @@ Importing this package needs no GPU; calling an op needs libhelion_lce.so (built
 from .ce_ops import cross_entropy, cross_entropy_backward
 from .decode_ops import greedy_head, sample_head, topk_head
 from .install import install, uninstall
+from .linear_ops import linear
 from .matmul_ops import matmul, matmul_vec
 from .norm_ops import residual_rmsnorm, rmsnorm, rmsnorm_backward
 from .optim_ops import adamw_step, clip_grad_norm, grad_sumsq
-from .rope_ops import qk_norm_rope, rope, rope_frequencies
 from .ops import linear_cross_entropy, linear_cross_entropy_backward
+from .rope_ops import qk_norm_rope, rope, rope_frequencies
 
 __all__ = [
     "adamw_step",
@@ -22,6 +23,7 @@ __all__ = [
     "grad_sumsq",
     "greedy_head",
     "install",
+    "linear",
     "linear_cross_entropy",
     "linear_cross_entropy_backward",
     "matmul",

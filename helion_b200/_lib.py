@@ -75,6 +75,14 @@ SIGNATURES = {
     "lce_rmsnorm_plan": (c_int, [c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "lce_rmsnorm_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                                      c_int64, ctypes.c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "lce_linear_forward_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int,
+                                                      c_uint]),
+    "lce_linear_forward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                   c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_size_t, c_uint, c_void_p]),
+    "lce_linear_backward_workspace_bytes": (c_size_t, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                                                       c_int64, c_int, c_int, c_uint]),
+    "lce_linear_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_size_t, c_uint, c_void_p]),
     "lce_rope": (c_int, [ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int,
                          ctypes.c_float, c_int, c_int, c_void_p]),
     "lce_qk_norm_rope_forward": (c_int, [ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,

@@ -17,7 +17,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libhelion_lce.so"
-SOURCES = [CSRC / "lce_api.cu", CSRC / "block_api.cu"]
+SOURCES = [CSRC / "lce_api.cu", CSRC / "linear_api.cu", CSRC / "block_api.cu"]
 HEADERS = sorted(CSRC.glob("*.cuh")) + [PKG_DIR.parent / "include" / "helion_lce.h"]
 
 NVCC_FLAGS = [

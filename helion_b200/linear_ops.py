@@ -1,0 +1,157 @@
+"""``linear``: a projection with bias, activation and residual in the epilogue of its matrix product.
+
+The projections of a decoder block are ``act(x @ weight.T + bias) + residual`` with some of the three left out. Run as
+separate operations, each pass over the product costs a read and a write of it; here they ride on the accumulators of
+the GEMM cores that the fused loss uses, and only the result is written (in training also what the activation's
+derivative needs). The backward pass forms ``dy * act'`` and the bias gradient in one pass and leaves two products.
+
+``weight`` is ``[out_features, in_features]`` as it is stored, like the LM head's; the reference launches ``matmul``,
+``add`` and an activation instead (tritium/ops/matmul.py, add.py, gelu.py, relu.py). A new entry point: ``install()``
+rebinds nothing to it.
+"""
+
+from __future__ import annotations
+
+from typing import Any
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import FLOAT_DTYPES, _DTYPE_CODE, _need_cuda, _need_dtype, _on_device, _path_flags, _ptr, _stream, _workspace
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
+
+def _check(x, weight, bias, activation, residual) -> int:
+    _need_cuda("x", x)
+    _need_cuda("weight", weight)
+    _need_dtype("x", x, FLOAT_DTYPES)
+    if x.dim() < 1:
+        raise ValueError("x must have at least 1 dimension shaped (..., in_features).")
+    if weight.dim() != 2:
+        raise ValueError("weight must be a 2D tensor shaped (out_features, in_features).")
+    n, k = weight.shape
+    if x.shape[-1] != k:
+        raise ValueError(f"Shape mismatch: x has last dimension {x.shape[-1]}, weight expects {k}.")
+    if n <= 0 or k <= 0:
+        raise ValueError("out_features and in_features must be positive.")
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise ValueError(f"Shape mismatch: bias has shape {tuple(bias.shape)}, expected ({n},).")
+    if residual is not None and residual.shape != (*x.shape[:-1], n):
+        raise ValueError(f"Shape mismatch: residual has shape {tuple(residual.shape)}, expected {(*x.shape[:-1], n)}.")
+    dtype, device = x.dtype, x.device
+    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if t is not None and t.dtype != dtype:
+            raise ValueError(f"Dtype mismatch: {name} has dtype {t.dtype}, x has dtype {dtype}.")
+        if t is not None and t.device != device:
+            raise ValueError(f"Device mismatch: {name} is on {t.device}, x is on {device}.")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of None, 'relu', 'gelu', 'gelu_tanh', 'silu'; got {activation!r}.")
+    return ACTIVATIONS[activation]
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """``t [..., n]`` as rows of contiguous elements and their pitch; copied where its strides allow no such view."""
+    n = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, n) if t.numel() else t.new_empty((0, n))
+    rows, stride = t.shape[0], t.stride()
+    if (stride[1] != 1 and n > 1) or (rows > 1 and stride[0] < n):
+        t = t.contiguous()
+        return t, n
+    return t, stride[0] if rows > 1 else n
+
+
+def _forward(x, weight, bias, residual, act: int, save: bool):
+    """(out [M, N], pre or None) for x [..., K]."""
+    dtype, dev = _DTYPE_CODE[x.dtype], x.device
+    x2, ldx = _rows(x)
+    w2, ldw = _rows(weight)
+    r2, ldr = _rows(residual) if residual is not None else (None, 0)
+    m, k = x2.shape
+    n = w2.shape[0]
+    b = bias.contiguous() if bias is not None else None
+    out = torch.empty((m, n), dtype=x.dtype, device=dev)
+    pre = torch.empty_like(out) if save and act else None
+    if m == 0:
+        return out, pre
+    L = _lib.lib()
+    flags = _flags(dtype)
+    xp, wp = x2.data_ptr(), w2.data_ptr()
+    need = L.lce_linear_forward_workspace_bytes(xp, ldx, wp, ldw, m, n, k, dtype, flags)
+    ws = _workspace(need, dev) if need else None
+    with _on_device(dev):
+        _lib.check(
+            L.lce_linear_forward(xp, ldx, wp, ldw, _ptr(b), _ptr(r2), ldr, out.data_ptr(), n, _ptr(pre), m, n, k, act, dtype,
+                                 _ptr(ws), need, flags, _stream(dev)),
+            "lce_linear_forward",
+        )
+    return out, pre
+
+
+def _flags(dtype: int) -> int:
+    flags = _path_flags()
+    return flags & ~_lib.FLAG_FORCE_TC if dtype == _lib.DTYPE_F32 else flags  # fp32 has no tensor-core path
+
+
+def _backward(dy, x, weight, pre, act: int, need_x: bool, need_w: bool, need_b: bool):
+    """(dx [M, K], dw [N, K], dbias [N]), each or None."""
+    dtype, dev = _DTYPE_CODE[x.dtype], x.device
+    dy2, ldy = _rows(dy)
+    x2, ldx = _rows(x)
+    w2, ldw = _rows(weight)
+    m, n = dy2.shape
+    k = w2.shape[1]
+    dx = torch.empty((m, k), dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty((n, k), dtype=x.dtype, device=dev) if need_w else None
+    db = torch.empty((n,), dtype=x.dtype, device=dev) if need_b else None
+    L = _lib.lib()
+    flags = _flags(dtype)
+    args = (dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw)
+    need = L.lce_linear_backward_workspace_bytes(*args, m, n, k, act, dtype, flags)
+    ws = _workspace(need, dev)
+    with _on_device(dev):
+        _lib.check(
+            L.lce_linear_backward(*args, _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db), m, n, k, act, dtype, ws.data_ptr(),
+                                  ws.numel(), flags, _stream(dev)),
+            "lce_linear_backward",
+        )
+    return dx, dw, db
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx: Any, x, weight, bias, residual, act):
+        out, pre = _forward(x, weight, bias, residual, act, True)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act = act
+        return out.view(*x.shape[:-1], out.shape[-1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, *grad_outputs):
+        dy = grad_outputs[0]
+        x, weight, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if need[0] or need[1] or need[2]:
+            dx, dw, db = _backward(dy, x, weight, pre, ctx.act, need[0], need[1], need[2])
+            dx = dx.view(x.shape) if dx is not None else None
+        return dx, dw, db, (dy if need[3] else None), None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
+           residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` in one pass over the product, rounded once.
+
+    ``x`` is ``[..., in_features]``, ``weight`` ``[out_features, in_features]``, ``bias`` ``[out_features]``,
+    ``residual`` shaped like the result; all of one type (bf16, fp16, fp32) and device. ``activation`` is ``None``,
+    ``"relu"``, ``"gelu"`` (with the normal distribution function), ``"gelu_tanh"`` or ``"silu"``. Rows may have any
+    pitch; inputs whose elements are not contiguous are copied first. fp32 is computed in fp32 throughout. Differentiable
+    in ``x``, ``weight``, ``bias`` and ``residual``; sums are formed in a fixed order."""
+    act = _check(x, weight, bias, activation, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        return _Linear.apply(x, weight, bias, residual, act)
+    return _forward(x, weight, bias, residual, act, False)[0].view(*x.shape[:-1], weight.shape[0])

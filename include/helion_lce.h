@@ -297,6 +297,35 @@ int lce_rmsnorm_backward(const void* dy, const void* x, const void* weight, cons
                          const void* dresidual, void* dx, void* dweight, int64_t n_rows, int64_t hidden, float eps,
                          int dtype, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- projection with its epilogue --------------------------------------------------------------
+ * out[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + residual[M, N], one rounding at the end; bias and residual may be NULL.
+ * Rows have their pitches (ldx, ldw >= K; ldr, ldo >= N, in elements) and contiguous elements. `pre` ([M, N], contiguous,
+ * may be NULL, ignored for LCE_ACT_NONE) receives what the backward pass derives act' from: pass it on unread.
+ * The backward takes dy = dLoss/dout and writes dx[M, K], dw[N, K], dbias[N] (each contiguous, each may be NULL); the
+ * residual's gradient is dy itself. dbias is summed in a fixed order from the unrounded dy * act', which is rounded to
+ * the element type as the operand of the two products. M = 0 is a sum of nothing: dw and dbias are zeroed.
+ * 16-bit types run on the tcgen05 core whatever the alignment (rows that TMA cannot read are copied to scratch at
+ * another pitch first); fp32 runs on the CUDA-core GEMM, as does everything under LCE_FLAG_FORCE_SIMT.
+ * The workspace depends on the operands' alignment, so its size is asked for with the operands themselves; the
+ * pointers are looked at, not followed. No counterpart in the reference, which launches matmul, add and the
+ * activation one after the other (tritium/ops/matmul.py, add.py, gelu.py, relu.py). */
+#define LCE_ACT_NONE 0
+#define LCE_ACT_RELU 1
+#define LCE_ACT_GELU 2      /* z * Phi(z), the normal distribution function */
+#define LCE_ACT_GELU_TANH 3 /* z / 2 * (1 + tanh(sqrt(2 / pi) * (z + 0.044715 z^3))) */
+#define LCE_ACT_SILU 4      /* z * sigmoid(z) */
+size_t lce_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N,
+                                          int64_t K, int dtype, unsigned flags);
+int lce_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
+                       int64_t ldr, void* out, int64_t ldo, void* pre, int64_t M, int64_t N, int64_t K, int act,
+                       int dtype, void* ws, size_t ws_bytes, unsigned flags, void* stream);
+size_t lce_linear_backward_workspace_bytes(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w,
+                                           int64_t ldw, int64_t M, int64_t N, int64_t K, int act, int dtype,
+                                           unsigned flags);
+int lce_linear_backward(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                        const void* pre, void* dx, void* dw, void* dbias, int64_t M, int64_t N, int64_t K, int act,
+                        int dtype, void* ws, size_t ws_bytes, unsigned flags, void* stream);
+
 /* ---- rotary positions, and the norm of every query and key head in the same pass --------------
  * angle_i = position * frequencies[i] (radians, formed in 64 bits), i < half; the first 2 * half <= dim elements
  * of every head are rotated in pairs: (x[i], x[half + i]), or (x[2i], x[2i + 1]) with interleaved != 0:

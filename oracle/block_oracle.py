@@ -43,3 +43,39 @@ def head_norm_rope_backward(dy, x, weight, positions, frequencies, eps=1e-6, int
     dx = rstd * (gw - unit * (gw * unit).mean(-1, keepdim=True))
     terms = (g * unit).flatten(0, -2)
     return dx, terms.sum(0), terms.abs().sum(0)
+
+
+def activation(z, name):
+    """(act(z), act'(z)) in float64."""
+    z = z.double()
+    if name is None:
+        return z, torch.ones_like(z)
+    if name == "relu":
+        return z.clamp_min(0.0), (z > 0).double()
+    if name == "gelu":
+        cdf = torch.special.ndtr(z)
+        return z * cdf, cdf + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    if name == "gelu_tanh":
+        c = math.sqrt(2 / math.pi)
+        s = torch.sigmoid(2 * c * (z + 0.044715 * z ** 3))
+        return z * s, s + z * s * (1 - s) * 2 * c * (1 + 3 * 0.044715 * z * z)
+    if name == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * (1 - s)
+    raise AssertionError(name)
+
+
+def linear(x, weight, bias=None, act=None, residual=None):
+    """(y, z) in float64."""
+    z = x.double() @ weight.double().t()
+    if bias is not None:
+        z = z + bias.double()
+    y = activation(z, act)[0]
+    return (y if residual is None else y + residual.double()), z
+
+
+def linear_backward(dy, x, weight, bias=None, act=None):
+    """(dx, dw, dbias, dz) in float64, for 2D tensors."""
+    z = linear(x, weight, bias)[1]
+    dz = dy.double() * activation(z, act)[1]
+    return dz @ weight.double(), dz.t() @ x.double(), dz.sum(0), dz
