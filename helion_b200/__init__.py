@@ -6,7 +6,7 @@ Importing this package needs no GPU; calling an op needs libhelion_lce.so (built
 """
 
 from .ce_ops import cross_entropy, cross_entropy_backward
-from .decode_ops import greedy_head, sample_head, topk_head
+from .decode_ops import greedy_head, sample_head, sample_logits, topk_head
 from .install import install, uninstall
 from .linear_ops import linear
 from .matmul_ops import matmul, matmul_vec
@@ -35,6 +35,7 @@ __all__ = [
     "rope",
     "rope_frequencies",
     "sample_head",
+    "sample_logits",
     "topk_head",
     "uninstall",
 ]

@@ -83,6 +83,10 @@ SIGNATURES = {
                                                        c_int64, c_int, c_int, c_uint]),
     "lce_linear_backward": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_size_t, c_uint, c_void_p]),
+    "lce_sample_logits_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "lce_sample_logits": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, ctypes.c_float, c_void_p, c_int,
+                                  c_int64, c_void_p, ctypes.c_float, c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p,
+                                  c_size_t, c_void_p]),
     "lce_rope": (c_int, [ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int,
                          ctypes.c_float, c_int, c_int, c_void_p]),
     "lce_qk_norm_rope_forward": (c_int, [ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,

@@ -1,7 +1,8 @@
 // extern "C" entry points of the operators of a decoder block around the head (declared in include/helion_lce.h):
-// rotary positions and the query / key norms. Argument checks, the choice of kernel form, and the launches.
+// rotary positions, the query / key norms, and the sampler. Argument checks, the choice of kernel form, the launches.
 #include "api_common.cuh"
 #include "rope_kernels.cuh"
+#include "sample_kernels.cuh"
 
 namespace lce {
 namespace {
@@ -217,6 +218,53 @@ int lce_qk_norm_rope_backward(const lce_head_rows* q, const lce_head_rows* k, in
     if (!k) return LCE_ERR_ARG;
     return heads_call<kHeadNormBackward>(q, k, batch, seq, dim, positions, pos_i64, pos_b, pos_s, freq, half, interleaved,
                                          scale, 1, eps, dtype, ws, ws_bytes, stream);
+}
+
+size_t lce_sample_logits_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
+    (void)rows, (void)vocab, (void)dtype;
+    return 0;
+}
+
+int lce_sample_logits(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int dtype, const float* uniform,
+                      const float* temperature, float temperature_all, const void* top_k, int top_k_is_i64, int64_t top_k_all,
+                      const float* top_p, float top_p_all, const float* min_p, float min_p_all, int64_t* token, float* logprob,
+                      void* ws, size_t ws_bytes, void* stream) {
+    if (!known_dtype(dtype) || rows < 0 || vocab < 1 || ld < vocab) return LCE_ERR_ARG;
+    if (vocab > 0x7fffff00ll || rows > 0x7fffff00ll) return LCE_ERR_TOO_LARGE;
+    if (rows == 0) return LCE_OK;
+    if (!logits || !uniform || !token) return LCE_ERR_ARG;
+    if (ws_bytes < lce_sample_logits_workspace_bytes(rows, vocab, dtype)) return LCE_ERR_WS_TOO_SMALL;
+    (void)ws;
+    DeviceInfo* d;
+    const int rc = device_basics(&d);
+    if (rc) return rc;
+    SampleParams p;
+    p.uniform = uniform;
+    p.temperature = temperature;
+    p.top_k = top_k;
+    p.top_p = top_p;
+    p.min_p = min_p;
+    p.temperature_all = temperature_all;
+    p.top_p_all = top_p_all;
+    p.min_p_all = min_p_all;
+    p.top_k_all = top_k_all;
+    p.top_k_i64 = top_k_is_i64;
+    p.token = reinterpret_cast<long long*>(token);
+    p.logprob = logprob;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const unsigned grid = static_cast<unsigned>(rows);
+    switch (dtype) {
+        case LCE_DTYPE_BF16:
+            sample_kernel<__nv_bfloat16><<<grid, kSampleThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(logits), ld, static_cast<int>(vocab), p);
+            break;
+        case LCE_DTYPE_F16:
+            sample_kernel<__half><<<grid, kSampleThreads, 0, s>>>(static_cast<const __half*>(logits), ld, static_cast<int>(vocab), p);
+            break;
+        default:
+            sample_kernel<float><<<grid, kSampleThreads, 0, s>>>(static_cast<const float*>(logits), ld, static_cast<int>(vocab), p);
+    }
+    LCE_COUNT_LAUNCH();
+    return cuda_failed(cudaGetLastError()) ? LCE_ERR_CUDA : LCE_OK;
 }
 
 }  // extern "C"

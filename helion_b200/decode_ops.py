@@ -17,8 +17,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib, parallel
-from .ops import FLOAT_DTYPES, _DTYPE_CODE, _need_contiguous, _need_cuda, _need_dtype, _on_device, _path_flags, _stream, \
-    _workspace
+from .ops import FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _need_contiguous, _need_cuda, _need_dtype, _on_device, _path_flags, \
+    _ptr, _stream, _workspace
 
 
 def greedy_head(hidden: torch.Tensor, weight: torch.Tensor, *, vocab_start: int | None = None,
@@ -254,3 +254,87 @@ def sampling_distribution(hidden: torch.Tensor, weight: torch.Tensor, *, tempera
         vals = vals.masked_fill(remove, float("-inf"))
     probs = torch.softmax(vals, dim=1)
     return idx.reshape(shape + (idx.shape[1],)), probs.reshape(shape + (probs.shape[1],))
+
+
+# ----------------------------------------------------------------------------------------------
+# sampling from logits
+# ----------------------------------------------------------------------------------------------
+def _per_row(name: str, value, shape, dtypes, device) -> tuple[torch.Tensor | None, float]:
+    """(tensor of one value per row or None, scalar)."""
+    if not isinstance(value, torch.Tensor):
+        return None, value
+    _need_cuda(name, value)
+    _need_dtype(name, value, dtypes)
+    if value.shape != shape:
+        raise ValueError(f"Shape mismatch: {name} has shape {tuple(value.shape)}, expected {tuple(shape)}.")
+    if value.device != device:
+        raise ValueError(f"Device mismatch: {name} is on {value.device}, logits is on {device}.")
+    return value.contiguous(), 0
+
+
+def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
+                  top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+                  return_logprob: bool = False):
+    """One token per row of ``logits`` ``[..., vocab]`` (int64, shaped like ``logits.shape[:-1]``), drawn with the given
+    ``uniforms`` (float32 in [0, 1), one per row) - the logits path that ``sample_head`` leaves to its callers: any
+    ``top_k``, any nucleus, or the whole vocabulary.
+
+    The rule is ``sampling_distribution``'s, with ``min_p`` added: ranked by logit (of equal ones the lower index
+    first), the ``top_k`` first are kept (0: all), of those the tokens whose predecessors hold at most ``top_p`` of the
+    top-k's probability (the first always), and of those the ones at least ``min_p`` times as likely as the first. The
+    token is where the kept probabilities, summed in vocabulary order, pass ``uniforms``; the same inputs give the same
+    tokens on every run. ``temperature`` 0 takes the first maximum. Each of the four is one value or a tensor of one per
+    row (float32; ``top_k`` int32 or int64), taken as float32; in a tensor, ``top_k`` < 1,
+    ``top_p`` >= 1 and ``min_p`` <= 0 switch the filter off, ``top_p`` <= 0 and ``min_p`` > 1 keep the most likely tokens
+    only, and a ``temperature`` <= 0 is greedy.
+
+    Weights and their sums are 64-bit, so that a draw next to a boundary between two tokens goes to the right one.
+    NaN logits count as ``-inf``; a row of nothing but ``-inf`` gives ``-1``. With ``return_logprob`` the result is
+    ``(tokens, logprobs)``: float32 log-probabilities under the distribution that was drawn from (0 for greedy rows,
+    ``-inf`` for ``-1``). Not differentiable. No counterpart in the reference but its rule (examples/common.py:263-306)."""
+    _need_cuda("logits", logits)
+    _need_cuda("uniforms", uniforms)
+    _need_dtype("logits", logits, FLOAT_DTYPES)
+    _need_dtype("uniforms", uniforms, (torch.float32,))
+    if logits.dim() < 1:
+        raise ValueError("logits must have at least 1 dimension shaped (..., vocab_size).")
+    vocab = logits.shape[-1]
+    if vocab <= 0:
+        raise ValueError("vocab_size must be positive.")
+    shape, dev = logits.shape[:-1], logits.device
+    if uniforms.shape != shape:
+        raise ValueError(f"Shape mismatch: uniforms has shape {tuple(uniforms.shape)}, expected {tuple(shape)}.")
+    if uniforms.device != dev:
+        raise ValueError(f"Device mismatch: uniforms is on {uniforms.device}, logits is on {dev}.")
+    t, t_all = _per_row("temperature", temperature, shape, (torch.float32,), dev)
+    k, k_all = _per_row("top_k", top_k, shape, INDEX_DTYPES, dev)
+    p, p_all = _per_row("top_p", top_p, shape, (torch.float32,), dev)
+    m, m_all = _per_row("min_p", min_p, shape, (torch.float32,), dev)
+    if t is None and not 0 <= t_all < float("inf"):
+        raise ValueError("temperature must be >= 0 and finite")
+    if k is None and k_all < 0:
+        raise ValueError("top_k must be >= 0")
+    if p is None and not 0.0 < p_all <= 1.0:
+        raise ValueError("top_p must satisfy 0 < top_p <= 1")
+    if m is None and not 0.0 <= m_all <= 1.0:
+        raise ValueError("min_p must satisfy 0 <= min_p <= 1")
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab) if logits.numel() else logits.new_empty((0, vocab))
+    rows = flat.shape[0]
+    if (vocab > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < vocab):
+        flat = flat.contiguous()
+    token = torch.empty(shape, dtype=torch.int64, device=dev)
+    logprob = torch.empty(shape, dtype=torch.float32, device=dev) if return_logprob else None
+    if rows:
+        L = _lib.lib()
+        code = _DTYPE_CODE[logits.dtype]
+        need = L.lce_sample_logits_workspace_bytes(rows, vocab, code)
+        ws = _workspace(need, dev) if need else None
+        with _on_device(dev):
+            _lib.check(
+                L.lce_sample_logits(flat.data_ptr(), flat.stride(0) if rows > 1 else vocab, rows, vocab, code,
+                                    uniforms.contiguous().data_ptr(), _ptr(t), t_all, _ptr(k),
+                                    int(k is not None and k.dtype == torch.int64), int(k_all), _ptr(p), p_all, _ptr(m), m_all,
+                                    token.data_ptr(), _ptr(logprob), _ptr(ws), need, _stream(dev)),
+                "lce_sample_logits",
+            )
+    return (token, logprob) if return_logprob else token

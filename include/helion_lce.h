@@ -365,6 +365,24 @@ int lce_qk_norm_rope_backward(const lce_head_rows* q, const lce_head_rows* k, in
                               int64_t pos_stride_seq, const double* frequencies, int64_t half, int interleaved,
                               float scale, float eps, int dtype, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- drawing tokens from logits ------------------------------------------------------------------
+ * One token per row of logits[rows, vocab] (rows ld >= vocab elements apart) from given uniform numbers:
+ *   weight_j = exp((l_j - max) / temperature); ranked by logit, larger first, of equal logits the lower index first, kept
+ *   are the top_k first (top_k < 1 or >= vocab: all), of those the ones whose predecessors' weights sum to at most top_p
+ *   of the top_k's sum (top_p >= 1: all; the first always), and of those the ones with weight_j >= min_p;
+ *   token = the first index whose kept weights up to it, in vocabulary order, exceed uniform * (kept weights' sum).
+ * Weights and sums are 64-bit. temperature, top_k, top_p and min_p come as one value per row (a device pointer, [rows];
+ * top_k int32 or int64) or, where the pointer is NULL, as the scalar behind it. uniform is clamped to [0, 1): at 1 or more
+ * the last kept token is taken, a NaN counts as 0. A temperature that is not positive takes the first maximum.
+ * NaN logits count as -inf; a row with nothing above -inf gives token -1 and logprob -inf; +inf logits share all weight.
+ * logprob ([rows], may be NULL) receives log(weight_token / kept weights' sum). This is the whole-vocabulary
+ * counterpart of lce_topk_head's candidates; the reference's rule is sample_next_token (examples/common.py:263-306). */
+size_t lce_sample_logits_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
+int lce_sample_logits(const void* logits, int64_t ld, int64_t rows, int64_t vocab, int dtype, const float* uniform,
+                      const float* temperature, float temperature_all, const void* top_k, int top_k_is_i64,
+                      int64_t top_k_all, const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                      int64_t* token, float* logprob, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- test hook (not part of the product interface) -------------------------------------------
  * Test infrastructure only: nothing above depends on it, a binding for the reference needs no stub
  * for it, and it may change without notice.

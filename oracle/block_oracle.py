@@ -79,3 +79,34 @@ def linear_backward(dy, x, weight, bias=None, act=None):
     z = linear(x, weight, bias)[1]
     dz = dy.double() * activation(z, act)[1]
     return dz @ weight.double(), dz.t() @ x.double(), dz.sum(0), dz
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(token, logprob) of one row, float64 on the host; the four parameters already rounded to float32."""
+    l = logits.detach().double().cpu()
+    l = torch.where(torch.isnan(l), -math.inf, l)
+    top = float(l.max())
+    if top == -math.inf:
+        return -1, -math.inf
+    first = int(torch.nonzero(l == top)[0, 0])
+    if not temperature > 0:
+        return first, 0.0
+    if top == math.inf:
+        w = (l == math.inf).double()
+    else:
+        w = torch.where(l == -math.inf, 0.0, torch.exp((l - top) / temperature))
+    ranked = torch.argsort(l, descending=True, stable=True)
+    if 0 < top_k < len(l):
+        ranked = ranked[:int(top_k)]
+    ws = w[ranked]
+    ahead = torch.cumsum(ws, 0) - ws
+    keep = ws > 0
+    if top_p < 1:
+        keep &= ahead <= top_p * ws.sum()
+        keep[0] = True
+    keep &= ws >= min(max(min_p, 0.0), 1.0)
+    index = torch.sort(ranked[keep]).values
+    line = torch.cumsum(w[index], 0)
+    u = min(max(float(u), 0.0), 1.0) if u == u else 0.0
+    at = min(int(torch.searchsorted(line, u * line[-1], right=True)), len(index) - 1)
+    return int(index[at]), math.log(float(w[index[at]] / line[-1]))
