@@ -184,6 +184,52 @@ int heads_call(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, in
     return dispatch_heads<MODE>(c, *q, kr, p, static_cast<float*>(ws), static_cast<cudaStream_t>(stream));
 }
 
+// ---------------------------------------------------------------------------------------------
+// sampler
+// ---------------------------------------------------------------------------------------------
+constexpr long long kSampleSliceBytes = 64 << 10;       // a CTA's share of a row: two CTAs and more fit an SM
+constexpr long long kSampleMaxSliceBytes = 160 << 10;   // beyond it a CTA re-reads its share from L2
+
+// CTAs per row: enough that a share fits shared memory well and, for few rows, that the GPU is busy - as long as a share
+// is worth the cluster's barriers.
+template <class T>
+int launch_sample(const DeviceInfo& d, const void* logits, long long ld, long long rows, long long vocab, const SampleParams& p,
+                  cudaStream_t s) {
+    constexpr int VEC = RmsTile<T>::kVec;
+    const long long n_vec = cdiv(vocab + VEC - 1, VEC);
+    int ctas = 1;
+    while (ctas < kSampleMaxCluster &&
+           (cdiv(n_vec, ctas) * 16 > kSampleSliceBytes || (rows * ctas < 2 * d.sm_count && vocab / (2 * ctas) >= 2048)))
+        ctas *= 2;
+    if (rows * ctas > 0x7fffffffll) return LCE_ERR_TOO_LARGE;
+    const int per_warp = static_cast<int>(cdiv(n_vec, static_cast<long long>(ctas) * kSampleWarps));
+    const long long slice = static_cast<long long>(per_warp) * kSampleWarps * 16;
+    const int in_smem = slice <= kSampleMaxSliceBytes ? 1 : 0;
+    auto kern = sample_kernel<T>;
+    static std::atomic<bool> opted_in[kMaxDevices];  // setting the attribute twice from two threads is harmless
+    if (!opted_in[d.index].load(std::memory_order_acquire)) {
+        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSampleMaxSliceBytes))))
+            return LCE_ERR_CUDA;
+        opted_in[d.index].store(true, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
+    cfg.blockDim = dim3(kSampleThreads);
+    cfg.dynamicSmemBytes = in_smem ? static_cast<size_t>(slice) : 0;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, static_cast<const T*>(logits), ld, static_cast<int>(vocab), ctas, per_warp,
+                                               in_smem, p);
+    LCE_COUNT_LAUNCH();
+    return cuda_failed(err) ? LCE_ERR_CUDA : LCE_OK;
+}
+
 }  // namespace
 }  // namespace lce
 
@@ -252,19 +298,11 @@ int lce_sample_logits(const void* logits, int64_t ld, int64_t rows, int64_t voca
     p.token = reinterpret_cast<long long*>(token);
     p.logprob = logprob;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>(rows);
     switch (dtype) {
-        case LCE_DTYPE_BF16:
-            sample_kernel<__nv_bfloat16><<<grid, kSampleThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(logits), ld, static_cast<int>(vocab), p);
-            break;
-        case LCE_DTYPE_F16:
-            sample_kernel<__half><<<grid, kSampleThreads, 0, s>>>(static_cast<const __half*>(logits), ld, static_cast<int>(vocab), p);
-            break;
-        default:
-            sample_kernel<float><<<grid, kSampleThreads, 0, s>>>(static_cast<const float*>(logits), ld, static_cast<int>(vocab), p);
+        case LCE_DTYPE_BF16: return launch_sample<__nv_bfloat16>(*d, logits, ld, rows, vocab, p, s);
+        case LCE_DTYPE_F16: return launch_sample<__half>(*d, logits, ld, rows, vocab, p, s);
+        default: return launch_sample<float>(*d, logits, ld, rows, vocab, p, s);
     }
-    LCE_COUNT_LAUNCH();
-    return cuda_failed(cudaGetLastError()) ? LCE_ERR_CUDA : LCE_OK;
 }
 
 }  // extern "C"

@@ -11,6 +11,17 @@
 // Weights and their sums are 64 bits: with 32, a draw that falls within 1e-7 of a boundary between two of 100000 tokens
 // - one in a hundred rows - would go to the wrong one. A NaN counts as -inf; a row with nothing above -inf gives
 // token -1; among +inf all weight is shared equally; a temperature that is not positive takes the first maximum.
+//
+// No sort. A prefix of the order is a threshold on the logit and a number of ties, and both are found by counting:
+//   1. a cluster of 1..8 CTAs takes a row; each keeps its slice in shared memory, so the logits are read once;
+//   2. a histogram of (max - l) / temperature in steps of 1/64 brackets the threshold: exactly for top_k, and for top_p
+//      between bounds, since a bin's weights are known to e^(1/64) from its count;
+//   3. for top_p one pass sums all weights, and those above the bracket, in 64 bits;
+//   4. histograms over the ordered bits of the logits inside the bracket (2048 bins each) narrow it to a single value;
+//      only elements inside the bracket need their weight for that;
+//   5. one pass sums the kept weights by warp, the sums find the warp that holds u times the total, and that warp
+//      finds the index.
+// Histograms are counts (integer atomics in shared memory) and sums have a fixed order: the same tokens on every run.
 #pragma once
 
 #include "ptx.cuh"
@@ -18,7 +29,13 @@
 
 namespace lce {
 
-constexpr int kSampleThreads = 1024;
+constexpr int kSampleThreads = 512;
+constexpr int kSampleWarps = kSampleThreads / 32;
+constexpr int kSampleMaxCluster = 8;
+constexpr int kSampleBins = 2048;
+constexpr float kSampleBinsPerNat = 64.f;
+constexpr int kSampleTable = 128;
+static_assert(kSampleBins == 4 * kSampleThreads, "a thread owns four bins");
 
 struct SampleParams {
     const float* uniform;      // [rows]
@@ -33,185 +50,702 @@ struct SampleParams {
     float* logprob;  // or nullptr
 };
 
-// The bits of a float in an order-preserving unsigned form; NaN sorts with -inf.
+// The bits of a float that is no NaN in an order-preserving unsigned form.
 __device__ __forceinline__ uint32_t sample_key(float v) {
-    if (!(v == v)) v = -INFINITY;
-    v += 0.f;  // -0 and +0 are equal logits
-    const uint32_t u = __float_as_uint(v);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t u = __float_as_uint(v + 0.f);  // -0 and +0 are equal logits
+    return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float sample_key_value(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
-constexpr uint32_t kSampleNone = 0x007fffffu;  // the key of -inf
 
-struct SampleRow {
-    double inv_t;
-    float top;  // the largest logit
-    __device__ __forceinline__ double weight(uint32_t key) const {
-        if (key == kSampleNone) return 0.0;
-        const float v = sample_key_value(key);
+// What a CTA of the cluster tells the others at an exchange.
+struct SampleSlot {
+    double d[3];
+    long long n;
+    uint32_t u, pad;
+};
+
+struct SampleShared {
+    uint32_t hist[2][kSampleBins];
+    double table[kSampleTable];  // 2^(i / 128)
+    SampleSlot slots[2][kSampleMaxCluster];
+    double wd[3][kSampleWarps];
+    long long wn[kSampleWarps];
+    uint32_t wu[kSampleWarps];
+    double total_d[2];
+    unsigned first_u, first_l;
+    unsigned bin;
+    long long before, count;
+};
+
+__device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster_s64(uint32_t addr, long long v) {
+    asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// The weights of one row.
+struct SampleWeights {
+    double top_d, inv_t;
+    float top;
+    float inv_t32;
+    const double* table;
+    // exp(x) for x <= 0 by a table of 2^(i / 128) and a polynomial (Tang, 1989): x = n ln2 / 128 + r, |r| <= ln2 / 256,
+    // exp(x) = 2^(n >> 7) 2^((n & 127) / 128) (1 + r + r^2 / 2 + r^3 / 6 + r^4 / 24): relative error below 1e-14
+    __device__ __forceinline__ double exp_below(double x) const {
+        constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+        const double nm = fma(x, 184.6649652337873105, kMagic);  // 128 / ln 2
+        const int n = __double2loint(nm);
+        const double r = fma(nm - kMagic, -0.005415212348514945209, x);  // ln 2 / 128
+        const double q = fma(r * r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), r);
+        double t = table[n & (kSampleTable - 1)];
+        t = __hiloint2double(__double2hiint(t) + ((n >> 7) << 20), __double2loint(t));
+        return fma(t, q, t);
+    }
+    __device__ __forceinline__ double operator()(float v) const {
         if (v == top) return 1.0;
-        if (top == INFINITY) return 0.0;
-        return exp((static_cast<double>(v) - static_cast<double>(top)) * inv_t);
+        const double x = (static_cast<double>(v) - top_d) * inv_t;
+        return x > -700.0 && top < INFINITY ? exp_below(x) : 0.0;
+    }
+    // bin of the first histogram; does not increase with v
+    __device__ __forceinline__ int bin(float v) const {
+        const float z = v == top ? 0.f : (top - v) * inv_t32;
+        return static_cast<int>(fminf(z, static_cast<float>(kSampleBins - 1)));
     }
 };
 
 template <class V>
-__device__ __forceinline__ V sample_block_sum(V v, V* red) {
+__device__ __forceinline__ V sample_warp_sum(V v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <class V>
+__device__ __forceinline__ V sample_warp_scan(V v) {  // inclusive
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V up = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
+// Sum of the values of the threads before this one; `tmp` holds one value per warp.
+template <class V>
+__device__ __forceinline__ V sample_block_before(V v, V* tmp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const V incl = sample_warp_scan(v);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    if (lane == 31) tmp[warp] = incl;
     __syncthreads();
-    V s = red[0];
-    for (int i = 1; i < kSampleThreads / 32; ++i) s += red[i];
-    return s;
+    V base = 0;
+    for (int i = 0; i < warp; ++i) base += tmp[i];
+    const V up = __shfl_up_sync(0xffffffffu, incl, 1);
+    return base + (lane == 0 ? V(0) : up);
 }
 
 template <class T>
-__global__ void __launch_bounds__(kSampleThreads)
-sample_kernel(const T* __restrict__ logits, long long ld, int vocab, const SampleParams p) {
-    __shared__ double red_d[32];
-    __shared__ long long red_i[32];
-    __shared__ unsigned long long best;
-    __shared__ double part_d[kSampleThreads];
-    __shared__ long long part_i[kSampleThreads];
-    const long long row = blockIdx.x;
-    const T* l = logits + row * ld;
-    const int t = threadIdx.x;
-    auto key_at = [&](int i) { return sample_key(Cvt<T>::to_f(l[i])); };
+__global__ void __launch_bounds__(kSampleThreads, 2)
+sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas, int vectors_per_warp, int in_smem,
+              const SampleParams p) {
+    constexpr int VEC = RmsTile<T>::kVec;
+    extern __shared__ __align__(16) unsigned char sample_slice[];
+    __shared__ SampleShared sh;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int rank = static_cast<int>(ptx::cluster_ctarank());
+    const long long row = blockIdx.x / n_ctas;
 
-    // the first maximum
-    unsigned long long mine = 0;
-    for (int i = t; i < vocab; i += kSampleThreads) {
-        const unsigned long long k = (static_cast<unsigned long long>(key_at(i)) << 32) | (0xffffffffu - static_cast<uint32_t>(i));
-        mine = k > mine ? k : mine;
+    // The row in 16-byte vectors that start on 16-byte boundaries: the first and the last may reach past it.
+    const T* l = logits + row * ld;
+    const int head = static_cast<int>((reinterpret_cast<uintptr_t>(l) & 15u) / sizeof(T));  // elements before the row
+    const T* aligned = l - head;
+    const int n_vec = static_cast<int>((static_cast<long long>(vocab) + head + VEC - 1) / VEC);
+    const int cta_vec0 = rank * kSampleWarps * vectors_per_warp;
+    const int v0 = min(n_vec, cta_vec0 + warp * vectors_per_warp), v1 = min(n_vec, v0 + vectors_per_warp);
+    uint4* slice = reinterpret_cast<uint4*>(sample_slice);
+
+    // One vector of the row; what is outside the row, and NaN, as -inf.
+    auto read = [&](int v) {
+        const long long i0 = static_cast<long long>(v) * VEC - head;
+        uint4 raw;
+        if (i0 >= 0 && i0 + VEC <= vocab) {
+            raw = *reinterpret_cast<const uint4*>(aligned + static_cast<long long>(v) * VEC);
+        } else {
+            alignas(16) T tmp[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                tmp[j] = i0 + j >= 0 && i0 + j < vocab ? l[i0 + j] : Cvt<T>::from_f(-INFINITY);
+            raw = *reinterpret_cast<const uint4*>(tmp);
+        }
+        float x[VEC];
+        rms_unpack<T>(raw, x);
+        bool nan = false;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) nan |= !(x[j] == x[j]);
+        if (nan) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) x[j] = x[j] == x[j] ? x[j] : -INFINITY;
+            raw = rms_pack<T>(x);
+        }
+        return raw;
+    };
+    // All elements of this warp's share: f(values, index of the first)
+    auto scan = [&](auto&& f) {
+        for (int v = v0 + lane; v < v1; v += 32) {
+            const uint4 raw = in_smem ? slice[v - cta_vec0] : read(v);
+            float x[VEC];
+            rms_unpack<T>(raw, x);
+            f(x);
+        }
+    };
+    int slot_parity = 0;
+    // Every CTA's values to every CTA; returns this exchange's slots. Two sets alternate: a CTA writes a set again only
+    // behind the next exchange's barrier, which all reach after they have read this one.
+    auto exchange = [&](double d0, double d1, double d2, long long n, uint32_t u) -> const SampleSlot* {
+        SampleSlot* mine = &sh.slots[slot_parity][rank];
+        if (t < n_ctas) {
+            const uint32_t a = ptx::map_to_cta(ptx::smem_u32(mine), t);
+            st_cluster_f64(a, d0);
+            st_cluster_f64(a + 8, d1);
+            st_cluster_f64(a + 16, d2);
+            st_cluster_s64(a + 24, n);
+            ptx::st_shared_cluster_u32(a + 32, u);
+        }
+        __syncthreads();
+        ptx::cluster_sync_all();
+        const SampleSlot* all = sh.slots[slot_parity];
+        slot_parity ^= 1;
+        return all;
+    };
+
+    // ---- 1. the slice and the maximum
+    float top = -INFINITY;
+    for (int v = v0 + lane; v < v1; v += 32) {
+        const uint4 raw = read(v);
+        if (in_smem) slice[v - cta_vec0] = raw;
+        float x[VEC];
+        rms_unpack<T>(raw, x);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) top = fmaxf(top, x[j]);
     }
-    if (t == 0) best = 0;
-    __syncthreads();
-    atomicMax(&best, mine);
-    __syncthreads();
-    const uint32_t top_key = static_cast<uint32_t>(best >> 32);
-    const int first = static_cast<int>(0xffffffffu - static_cast<uint32_t>(best));
+    if (t < kSampleTable) sh.table[t] = exp2(t / static_cast<double>(kSampleTable));
+    for (int i = t; i < kSampleBins; i += kSampleThreads) sh.hist[0][i] = sh.hist[1][i] = 0;
+    {
+        uint32_t k = __reduce_max_sync(0xffffffffu, sample_key(top));
+        if (lane == 0) sh.wu[warp] = k;
+        __syncthreads();
+        k = 0;
+        for (int i = 0; i < kSampleWarps; ++i) k = max(k, sh.wu[i]);
+        const SampleSlot* all = exchange(0, 0, 0, 0, k);
+        for (int c = 0; c < n_ctas; ++c) k = max(k, all[c].u);
+        top = sample_key_value(k);
+    }
     const float temp = p.temperature ? p.temperature[row] : p.temperature_all;
-    if (top_key == kSampleNone || !(temp > 0.f)) {
-        if (t == 0) {
-            p.token[row] = top_key == kSampleNone ? -1 : first;
-            if (p.logprob) p.logprob[row] = top_key == kSampleNone ? -INFINITY : 0.f;
+    if (top == -INFINITY || !(temp > 0.f)) {  // the same for the whole cluster
+        uint32_t first = 0xffffffffu;
+        if (top != -INFINITY) {
+            for (int v = v0 + lane; v < v1; v += 32) {
+                const uint4 raw = in_smem ? slice[v - cta_vec0] : read(v);
+                float x[VEC];
+                rms_unpack<T>(raw, x);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    if (x[j] == top) first = min(first, static_cast<uint32_t>(v) * VEC + j - head);
+            }
+        }
+        first = __reduce_min_sync(0xffffffffu, first);
+        __syncthreads();
+        if (lane == 0) sh.wu[warp] = first;
+        __syncthreads();
+        for (int i = 0; i < kSampleWarps; ++i) first = min(first, sh.wu[i]);
+        const SampleSlot* all = exchange(0, 0, 0, 0, first);
+        for (int c = 0; c < n_ctas; ++c) first = min(first, all[c].u);
+        if (rank == 0 && t == 0) {
+            p.token[row] = top == -INFINITY ? -1 : static_cast<long long>(first);
+            if (p.logprob) p.logprob[row] = top == -INFINITY ? -INFINITY : 0.f;
         }
         return;
     }
-    SampleRow r;
-    r.inv_t = 1.0 / static_cast<double>(temp);
-    r.top = sample_key_value(top_key);
+    SampleWeights weight;
+    weight.top = top;
+    weight.top_d = top;
+    weight.inv_t = 1.0 / static_cast<double>(temp);
+    weight.inv_t32 = fminf(kSampleBinsPerNat / temp, 1e30f);
+    weight.table = sh.table;
 
-    // the largest key such that at least `k` keys are at or above it; ties of it kept in index order
-    uint32_t bound = kSampleNone + 1;  // smallest key that may be kept
-    long long ties = vocab;            // how many keys equal to `bound` are kept
-    long long k = p.top_k ? (p.top_k_i64 ? static_cast<const long long*>(p.top_k)[row] : static_cast<const int*>(p.top_k)[row]) : p.top_k_all;
-    auto count_from = [&](uint32_t key) {
-        long long c = 0;
-        for (int i = t; i < vocab; i += kSampleThreads) c += key_at(i) >= key;
-        return sample_block_sum(c, red_i);
-    };
-    auto mass_above = [&](uint32_t key) {
-        double m = 0;
-        for (int i = t; i < vocab; i += kSampleThreads) {
-            const uint32_t q = key_at(i);
-            if (q > key) m += r.weight(q);
+    // ---- histograms
+    int hist_parity = 0;
+    // The counts of bins 4t .. 4t + 3 over the whole cluster, f(value) the bin or -1. Two histograms alternate: one is
+    // cleared while the other is in use, a barrier after all CTAs have read it.
+    auto histogram = [&](auto&& f) -> uint4 {
+        uint32_t* h = sh.hist[hist_parity];
+        scan([&](const float (&x)[VEC]) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const int b = f(x[j]);
+                if (b >= 0) atomicAdd(&h[b], 1u);
+            }
+        });
+        __syncthreads();
+        ptx::cluster_sync_all();
+        uint4 sum = make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < n_ctas; ++c) {
+            const uint4 o = ld_cluster_v4(ptx::map_to_cta(ptx::smem_u32(&h[4 * t]), c));
+            sum.x += o.x;
+            sum.y += o.y;
+            sum.z += o.z;
+            sum.w += o.w;
         }
-        return sample_block_sum(m, red_d);
+        hist_parity ^= 1;
+        return sum;
     };
-    if (k > 0 && k < vocab && count_from(bound) > k) {
-        uint32_t lo = bound, hi = top_key;  // count_from(lo) > k
+    auto clear_other = [&]() {  // the histogram after next: read by all before the barrier that has just passed
+        uint32_t* h = sh.hist[hist_parity];
+        for (int i = t; i < kSampleBins; i += kSampleThreads) h[i] = 0;
+        __syncthreads();
+    };
+    // The keys of one bin of weight.bin, as a range: 32 points at a time, all warps alike.
+    auto first_key_of_bin_at_most = [&](int b) {  // the smallest key whose value falls in bin b or an earlier one
+        uint32_t lo = 0x007fffffu, hi = sample_key(top);  // hi does
         while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo + 1) / 2;
-            if (count_from(mid) >= k) lo = mid;
-            else hi = mid - 1;
+            const uint64_t span = hi - lo;
+            const uint32_t at = lo + static_cast<uint32_t>(span * lane / 32);
+            const unsigned yes = __ballot_sync(0xffffffffu, weight.bin(sample_key_value(at)) <= b);
+            const int i = yes ? __ffs(yes) - 1 : 32;  // points i .. 31 and hi do
+            const uint32_t new_hi = i < 32 ? lo + static_cast<uint32_t>(span * i / 32) : hi;
+            if (i > 0) lo = lo + static_cast<uint32_t>(span * (i - 1) / 32) + 1;
+            hi = new_hi;
         }
-        bound = lo;
-        ties = k - (bound == top_key ? 0 : count_from(bound + 1));
+        return hi;
+    };
+
+    // What is kept: values above `bound`, and `ties` of those equal to it in index order. -inf: everything.
+    float bound = -INFINITY;
+    long long ties = 0;
+    long long k = p.top_k ? (p.top_k_i64 ? static_cast<const long long*>(p.top_k)[row] : static_cast<const int*>(p.top_k)[row]) : p.top_k_all;
+
+    // ---- 2., 4. top_k: the k-th value
+    if (k > 0 && k < vocab) {
+        uint32_t lo = 0, hi = 0;
+        int shift = -1;  // -1: the first histogram
+        long long above = 0;  // values above the bracket
+        bool all = true;  // fewer than k values above -inf
+        for (int round = 0; round < 4; ++round) {  // the first histogram, then 32 bits in steps of 11
+            const uint4 c = shift < 0 ? histogram([&](float v) { return v > -INFINITY ? weight.bin(v) : -1; })
+                                      : histogram([&](float v) {
+                                            const uint32_t q = sample_key(v);
+                                            return q >= lo && q <= hi ? static_cast<int>((hi - q) >> shift) : -1;
+                                        });
+            clear_other();
+            const long long cs[4] = {c.x, c.y, c.z, c.w};
+            long long run = above + sample_block_before<long long>(cs[0] + cs[1] + cs[2] + cs[3], sh.wn);
+            if (t == 0) sh.bin = kSampleBins;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (run < k && k <= run + cs[j]) {
+                    sh.bin = 4 * t + j;
+                    sh.before = run;
+                }
+                run += cs[j];
+            }
+            __syncthreads();
+            const uint32_t b = sh.bin;
+            above = sh.before;
+            if (b == kSampleBins) break;
+            all = false;
+            if (shift == 0) {
+                lo = hi = hi - b;
+                break;
+            }
+            if (shift < 0) {
+                lo = first_key_of_bin_at_most(static_cast<int>(b));
+                hi = b == 0 ? sample_key(top) : first_key_of_bin_at_most(static_cast<int>(b) - 1) - 1;
+            } else {
+                hi -= b << shift;
+                lo = max(lo, hi - ((1u << shift) - 1u));
+            }
+            shift = 0;
+            while (((hi - lo) >> shift) >= kSampleBins) ++shift;
+        }
+        if (!all) {
+            bound = sample_key_value(lo);
+            ties = k - above;
+        }
     }
+
+    // ---- 2., 3., 4. top_p: the smallest value whose predecessors' weights stay within the limit
     const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
     if (top_p < 1.f) {
-        const long long equal = count_from(bound) - count_from(bound + 1);
-        const double z = mass_above(bound) + (equal < ties ? equal : ties) * r.weight(bound);
-        const double limit = static_cast<double>(top_p) * z;
-        uint32_t lo = bound, hi = top_key;  // the smallest key with mass_above <= limit
-        while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if (mass_above(mid) <= limit) hi = mid;
-            else lo = mid + 1;
+        const float floor_value = bound;  // only values above it take part; `extra` is the ties' weight
+        const double extra = ties > 0 ? ties * weight(bound) : 0.0;
+        const double share = top_p > 0.f ? static_cast<double>(top_p) : 0.0;
+        uint32_t lo, hi;      // the bracket
+        double above = 0, limit;  // weight above the bracket; the largest sum of predecessors
+        bool found = false;   // the threshold is in the bracket
+        {
+            const uint4 c = histogram([&](float v) { return v > floor_value ? weight.bin(v) : -1; });
+            clear_other();
+            const double cs[4] = {double(c.x), double(c.y), double(c.z), double(c.w)};
+            double up[4], low[4];
+            // weights of bin b are within e^-((b + 1) / 64) .. e^-(b / 64), and 1e-4 for the bin's 32-bit arithmetic
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double e = weight.exp_below(-(4 * t + j) / static_cast<double>(kSampleBinsPerNat));
+                up[j] = cs[j] * e * 1.0001;
+                low[j] = 4 * t + j == kSampleBins - 1 ? 0.0 : cs[j] * e * (0.9845 * 0.9999);  // e^(-1/64) = 0.98450
+            }
+            const double up_sum = up[0] + up[1] + up[2] + up[3], low_sum = low[0] + low[1] + low[2] + low[3];
+            double up_run = sample_block_before<double>(up_sum, sh.wd[0]);
+            double low_run = sample_block_before<double>(low_sum, sh.wd[1]);
+            if (t == kSampleThreads - 1) {
+                sh.total_d[0] = up_run + up_sum;
+                sh.total_d[1] = low_run + low_sum;
+                sh.first_u = sh.first_l = kSampleBins - 1;
+            }
+            __syncthreads();
+            const double least = share * (sh.total_d[1] + extra), most = share * (sh.total_d[0] + extra);
+#pragma unroll
+            for (int j = 3; j >= 0; --j) {
+                // the first bin whose upper sum may pass the limit, the first whose lower sum must
+                double u = up_run, w = low_run;
+                for (int i = 0; i <= j; ++i) {
+                    u += up[i];
+                    w += low[i];
+                }
+                if (cs[j] > 0 && u >= least) atomicMin(&sh.first_u, static_cast<unsigned>(4 * t + j));
+                if (cs[j] > 0 && w > most) atomicMin(&sh.first_l, static_cast<unsigned>(4 * t + j));
+            }
+            __syncthreads();
+            const int b1 = static_cast<int>(sh.first_u), b2 = max(b1, static_cast<int>(sh.first_l));
+            hi = b1 == 0 ? sample_key(top) : first_key_of_bin_at_most(b1 - 1) - 1;
+            lo = b2 == kSampleBins - 1 ? 0x00800000u : first_key_of_bin_at_most(b2);
+            double s[3] = {0, 0, 0};  // above, inside, below
+            scan([&](const float (&x)[VEC]) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    if (x[j] > floor_value) {
+                        const double w = weight(x[j]);
+                        const uint32_t q = sample_key(x[j]);
+                        if (q > hi) s[0] += w;
+                        else if (q >= lo) s[1] += w;
+                        else s[2] += w;
+                    }
+                }
+            });
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                s[i] = sample_warp_sum(s[i]);
+                if (lane == 0) sh.wd[i][warp] = s[i];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                s[i] = 0;
+                for (int w = 0; w < kSampleWarps; ++w) s[i] += sh.wd[i][w];
+            }
+            const SampleSlot* all = exchange(s[0], s[1], s[2], 0, 0);
+            s[0] = s[1] = s[2] = 0;
+            for (int c2 = 0; c2 < n_ctas; ++c2) {
+                s[0] += all[c2].d[0];
+                s[1] += all[c2].d[1];
+                s[2] += all[c2].d[2];
+            }
+            const double all_above = s[0] + s[1] + s[2];
+            limit = share * (all_above + extra);
+            const uint32_t floor_key = sample_key(floor_value);
+            if (all_above <= limit) {
+                above = all_above;  // every value above the floor is kept
+            } else if (s[0] > limit) {  // outside the bounds' bracket (they leave room for rounding, but to be sure)
+                found = true;
+                lo = hi + 1;
+                hi = sample_key(top);
+                above = 0;
+            } else if (s[0] + s[1] > limit) {
+                found = true;
+                lo = max(lo, floor_key + 1);
+                above = s[0];
+            } else {
+                found = true;
+                hi = lo - 1;
+                lo = floor_key + 1;
+                above = s[0] + s[1];
+            }
         }
-        const double above = mass_above(lo), w = r.weight(lo);
-        if (lo != bound) ties = vocab;
-        bound = lo;
-        // tie number j (from 0) is kept while above + j w <= limit; the very first always
-        long long most = w > 0 ? static_cast<long long>(fmin((limit - above) / w, 4e9)) : vocab;
-        while (above + most * w <= limit && most < vocab) ++most;
-        while (most > 0 && above + (most - 1) * w > limit) --most;
-        if (bound == top_key && most < 1) most = 1;
-        ties = most < ties ? most : ties;
+        if (!found) {
+            // the ties of the floor, one after the other
+            const double w = ties > 0 ? weight(bound) : 0.0;
+            if (w > 0) {
+                const double room = (limit - above) / w;
+                const long long most = room < 0 ? 0 : static_cast<long long>(fmin(room, 4e9)) + 1;
+                ties = most < ties ? most : ties;
+            }
+        } else {
+            // every round narrows the bracket to one bin, or by one bin that has values: a few rounds, thousands at the worst
+            for (int round = 0; round < 1 << 16; ++round) {
+                int shift = 0;
+                while (((hi - lo) >> shift) >= kSampleBins) ++shift;
+                const uint4 c = histogram([&](float v) {
+                    const uint32_t q = sample_key(v);
+                    return q >= lo && q <= hi ? static_cast<int>((hi - q) >> shift) : -1;
+                });
+                clear_other();
+                const double cs[4] = {double(c.x), double(c.y), double(c.z), double(c.w)};
+                double up[4], low[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t off = static_cast<uint32_t>(4 * t + j) << shift, last = off + ((1u << shift) - 1u);
+                    const bool in = off <= hi - lo;
+                    up[j] = in && cs[j] > 0 ? cs[j] * weight(sample_key_value(hi - off)) : 0.0;
+                    low[j] = in && cs[j] > 0 ? (shift == 0 ? up[j] : cs[j] * weight(sample_key_value(hi - min(last, hi - lo)))) : 0.0;
+                }
+                const double up_run = above + sample_block_before<double>(up[0] + up[1] + up[2] + up[3], sh.wd[0]);
+                const double low_run = above + sample_block_before<double>(low[0] + low[1] + low[2] + low[3], sh.wd[1]);
+                if (t == 0) sh.first_u = sh.first_l = kSampleBins;
+                __syncthreads();
+                // a hair of room on both sides while the bins hold several values; none once they are single ones
+                const double hair = shift == 0 ? 0.0 : 1e-9 * limit;
+                unsigned last_full = 0;
+                double u = up_run, w = low_run;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    u += up[j];
+                    w += low[j];
+                    if (cs[j] > 0) {
+                        last_full = 4 * t + j + 1;
+                        if (u > limit - hair) atomicMin(&sh.first_u, static_cast<unsigned>(4 * t + j));
+                        if (w > limit + hair) atomicMin(&sh.first_l, static_cast<unsigned>(4 * t + j));
+                    }
+                }
+                last_full = __reduce_max_sync(0xffffffffu, last_full);
+                if (lane == 0) sh.wu[warp] = last_full;
+                __syncthreads();
+                for (int i = 0; i < kSampleWarps; ++i) last_full = max(last_full, sh.wu[i]);
+                // the bracket holds the threshold, so a bin that no sum passes stands for the last one that has values
+                const uint32_t b1 = min(sh.first_u, last_full - 1), b2 = max(b1, min(sh.first_l, last_full - 1));
+                if (shift == 0) {
+                    // the sums of single values are exact: predecessors of this one stay within the limit
+                    __syncthreads();
+                    double run = up_run;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (static_cast<uint32_t>(4 * t + j) == b1) {
+                            sh.total_d[0] = run;
+                            sh.count = static_cast<long long>(cs[j]);
+                        }
+                        run += up[j];
+                    }
+                    __syncthreads();
+                    bound = sample_key_value(hi - b1);
+                    const double w1 = weight(bound), ahead = sh.total_d[0];
+                    const long long equal = sh.count;
+                    // tie number i (from 0) is kept while ahead + i w <= limit; the very first value always
+                    long long most = equal;
+                    if (w1 > 0) {
+                        const double room = (limit - ahead) / w1;
+                        most = room < 0 ? 0 : static_cast<long long>(fmin(room, 4e9)) + 1;
+                    }
+                    if (bound == top && most < 1) most = 1;
+                    ties = most < equal ? most : equal;
+                    break;
+                }
+                // weights of the bins before b1, and of b1, exactly
+                const uint32_t b1_hi = hi - (b1 << shift);
+                const uint32_t b1_lo = max(lo, b1_hi - ((1u << shift) - 1u));
+                const uint32_t b2_hi = hi - (b2 << shift);
+                const uint32_t b2_lo = max(lo, b2_hi - ((1u << shift) - 1u));
+                double s[2] = {0, 0};
+                scan([&](const float (&x)[VEC]) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) {
+                        const uint32_t q = sample_key(x[j]);
+                        if (q <= hi && q >= b1_lo) {
+                            const double wv = weight(x[j]);
+                            if (q > b1_hi) s[0] += wv;
+                            else s[1] += wv;
+                        }
+                    }
+                });
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    s[i] = sample_warp_sum(s[i]);
+                    if (lane == 0) sh.wd[i][warp] = s[i];
+                }
+                __syncthreads();
+                s[0] = s[1] = 0;
+                for (int i = 0; i < kSampleWarps; ++i) {
+                    s[0] += sh.wd[0][i];
+                    s[1] += sh.wd[1][i];
+                }
+                const SampleSlot* all = exchange(s[0], s[1], 0, 0, 0);
+                s[0] = s[1] = 0;
+                for (int c2 = 0; c2 < n_ctas; ++c2) {
+                    s[0] += all[c2].d[0];
+                    s[1] += all[c2].d[1];
+                }
+                if (b1 == b2 || above + s[0] + s[1] > limit) {
+                    above += s[0];
+                    hi = b1_hi;
+                    lo = b1_lo;
+                } else {
+                    above += s[0] + s[1];
+                    hi = b1_lo - 1;
+                    lo = b2_lo;
+                }
+            }
+        }
     }
     const float min_row = p.min_p ? p.min_p[row] : p.min_p_all;
     const double min_p = min_row > 0.f ? fminf(min_row, 1.f) : 0.0;
 
-    // in vocabulary order: thread t owns a run of indices
-    const int per = (vocab + kSampleThreads - 1) / kSampleThreads;
-    const int i0 = min(vocab, t * per), i1 = min(vocab, i0 + per);
-    long long equal = 0;
-    for (int i = i0; i < i1; ++i) equal += key_at(i) == bound;
-    part_i[t] = equal;
-    __syncthreads();
-    long long before = 0;
-    for (int j = 0; j < t; ++j) before += part_i[j];
-    auto kept = [&](uint32_t q, long long& rank) {
-        const bool in = q > bound || (q == bound && rank < ties);
-        rank += q == bound;
-        const double w = in ? r.weight(q) : 0.0;
+    // ---- 5. the kept weights by warp
+    auto kept_weight = [&](float v) {
+        const double w = weight(v);
         return w >= min_p ? w : 0.0;
     };
+    const double w_tie = ties > 0 ? kept_weight(bound) : 0.0;
     double sum = 0;
-    long long rank = before;
-    for (int i = i0; i < i1; ++i) sum += kept(key_at(i), rank);
-    part_d[t] = sum;
+    long long equal = 0;
+    scan([&](const float (&x)[VEC]) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            if (x[j] > bound) sum += kept_weight(x[j]);
+            else if (x[j] == bound) ++equal;
+        }
+    });
+    sum = sample_warp_sum(sum);
+    equal = sample_warp_sum(equal);
     __syncthreads();
-    double ahead = 0, total = 0;
-    for (int j = 0; j < kSampleThreads; ++j) {
-        if (j == t) ahead = total;
-        total += part_d[j];
+    if (lane == 0) {
+        sh.wd[0][warp] = sum;
+        sh.wn[warp] = equal;
     }
+    __syncthreads();
+    sum = 0;
+    equal = 0;
+    for (int i = 0; i < kSampleWarps; ++i) {
+        sum += sh.wd[0][i];
+        equal += sh.wn[i];
+    }
+    const SampleSlot* all = exchange(sum, 0, 0, equal, 0);
+    auto ties_kept = [&](long long before, long long n) {
+        const long long left = ties - before;
+        return left <= 0 ? 0ll : (left < n ? left : n);
+    };
     float u = p.uniform[row];
     u = u > 0.f ? u : 0.f;
-    const double target = static_cast<double>(u) * total;
-    // the last kept index stands in where u is 1 or more
-    const bool owner = ahead <= target && target < ahead + sum;
-    if (t == 0) best = 0;
-    __syncthreads();
-    if (sum > 0 && (owner || target >= total)) {
-        double run = ahead;
-        rank = before;
-        int pick = -1;
-        double wp = 0;
-        for (int i = i0; i < i1; ++i) {
-            const double w = kept(key_at(i), rank);
-            if (w > 0) {
-                pick = i;
-                wp = w;
-                run += w;
-                if (run > target) break;
+    double everything = 0;
+    {
+        long long before = 0;
+        for (int c = 0; c < n_ctas; ++c) {
+            everything += all[c].d[0] + ties_kept(before, all[c].n) * w_tie;
+            before += all[c].n;
+        }
+    }
+    // The CTA whose sum passes the target, then the warp of it; where rounding (or u >= 1) leaves the target behind all
+    // sums, the last one that holds anything.
+    double target = static_cast<double>(u) * everything, run = 0, start = 0;
+    long long before = 0, tie_start = 0;
+    int owner = -1;
+    for (int c = 0; c < n_ctas; ++c) {
+        const double s = all[c].d[0] + ties_kept(before, all[c].n) * w_tie;
+        if (s > 0) {
+            owner = c;
+            start = run;
+            tie_start = before;
+            if (run + s > target) break;
+        }
+        run += s;
+        before += all[c].n;
+    }
+    if (rank != owner) return;
+    target -= start;
+    run = start = 0;
+    before = tie_start;
+    owner = -1;
+    for (int i = 0; i < kSampleWarps; ++i) {
+        const double s = sh.wd[0][i] + ties_kept(before, sh.wn[i]) * w_tie;
+        if (s > 0) {
+            owner = i;
+            start = run;
+            tie_start = before;
+            if (run + s > target) break;
+        }
+        run += s;
+        before += sh.wn[i];
+    }
+    if (warp != owner) return;
+    target -= start;
+    // the index: 32 vectors at a time
+    double passed = 0;
+    long long ties_passed = tie_start;
+    long long last = -1;  // of this lane's kept elements
+    double last_w = 0;
+    for (int base = v0; base < v1; base += 32) {
+        const int v = base + lane;
+        float x[VEC];
+        int n_equal = 0;
+        if (v < v1) {
+            const uint4 raw = in_smem ? slice[v - cta_vec0] : read(v);
+            rms_unpack<T>(raw, x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) x[j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) n_equal += x[j] == bound && v < v1;
+        const int equal_incl = sample_warp_scan(n_equal);
+        long long tie = ties_passed + equal_incl - n_equal;
+        double w[VEC], lane_sum = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            w[j] = 0;
+            if (x[j] > bound) w[j] = kept_weight(x[j]);
+            else if (x[j] == bound && v < v1 && tie++ < ties) w[j] = w_tie;
+            lane_sum += w[j];
+            if (w[j] > 0) {
+                last = static_cast<long long>(v) * VEC + j - head;
+                last_w = w[j];
             }
         }
-        atomicMax(&best, static_cast<unsigned long long>(pick + 1));
-        __syncwarp(__activemask());
-        part_d[t] = wp;
+        const double incl = sample_warp_scan(lane_sum);
+        const unsigned hit = __ballot_sync(0xffffffffu, lane_sum > 0 && passed + incl > target);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) {
+                double r = passed + (incl - lane_sum);
+                bool done = false;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    r += w[j];
+                    if (!done && w[j] > 0 && r > target) {
+                        done = true;
+                        last = static_cast<long long>(v) * VEC + j - head;
+                        last_w = w[j];
+                    }
+                }
+                p.token[row] = last;
+                if (p.logprob) p.logprob[row] = static_cast<float>(log(last_w / everything));
+            }
+            return;
+        }
+        passed += __shfl_sync(0xffffffffu, incl, 31);
+        ties_passed += __shfl_sync(0xffffffffu, equal_incl, 31);
     }
-    __syncthreads();
-    if (t == 0) {
-        const int pick = static_cast<int>(best) - 1;
-        p.token[row] = pick;
-        if (p.logprob) p.logprob[row] = static_cast<float>(log(part_d[pick / per] / total));
+    // rounding left the target behind the last kept element, or u is 1: that element
+    const uint32_t best = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(last + 1));
+    if (static_cast<uint32_t>(last + 1) == best) {
+        p.token[row] = last;
+        if (p.logprob) p.logprob[row] = static_cast<float>(log(last_w / everything));
     }
 }
 

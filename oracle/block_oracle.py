@@ -82,15 +82,17 @@ def linear_backward(dy, x, weight, bias=None, act=None):
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
-    """(token, logprob) of one row, float64 on the host; the four parameters already rounded to float32."""
+    """{token: logprob} of one row, float64 on the host; the four parameters already rounded to float32. One token,
+    unless the draw lies on a boundary to within the rounding of a 64-bit sum: V additions in any order are good to
+    V 2^-53 of the sum, here and in what is compared, so a draw within V 2^-52 of a boundary may go to either side."""
     l = logits.detach().double().cpu()
     l = torch.where(torch.isnan(l), -math.inf, l)
     top = float(l.max())
     if top == -math.inf:
-        return -1, -math.inf
+        return {-1: -math.inf}
     first = int(torch.nonzero(l == top)[0, 0])
     if not temperature > 0:
-        return first, 0.0
+        return {first: 0.0}
     if top == math.inf:
         w = (l == math.inf).double()
     else:
@@ -108,5 +110,6 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     index = torch.sort(ranked[keep]).values
     line = torch.cumsum(w[index], 0)
     u = min(max(float(u), 0.0), 1.0) if u == u else 0.0
-    at = min(int(torch.searchsorted(line, u * line[-1], right=True)), len(index) - 1)
-    return int(index[at]), math.log(float(w[index[at]] / line[-1]))
+    room = len(l) * 2.0 ** -52 * float(line[-1])
+    low, high = (min(int(torch.searchsorted(line, u * line[-1] + d, right=True)), len(index) - 1) for d in (-room, room))
+    return {int(index[at]): math.log(float(w[index[at]] / line[-1])) for at in range(low, high + 1)}

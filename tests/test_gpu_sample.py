@@ -1,9 +1,10 @@
 """sample_logits against its definition in float64: filters alone and together, ties, masks, values that are not
 finite, strides, batch sizes, capture. GPU only.
 
-Tokens have to be equal. Both sides form weights and sums in 64 bits, relative error below V x 2^-50 of a sum, so a draw
-has to lie within 1e-10 of a boundary to go elsewhere: the uniforms below are fixed, and cases in which a draw lies
-exactly ON a boundary use weights and uniforms whose sums are exact. Log-probabilities are rounded to float32 once."""
+Tokens have to be equal. Both sides form weights and sums in 64 bits; where the definition puts a draw ON a boundary
+between two tokens (periodic weights and a uniform of 1/2 do), the rounding of a 64-bit sum decides, and the oracle
+names both. Boundaries between sums that are exact - of equal weights - are tested by value. Log-probabilities are
+rounded to float32 once."""
 
 from __future__ import annotations
 
@@ -53,10 +54,10 @@ def _check(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         return v[i] if isinstance(v, list) else v
 
     for i in range(rows):
-        want, lp = block_oracle.sample(logits[i], float(u[i]), _f32(row(temperature, i)), row(top_k, i), _f32(row(top_p, i)),
-                                       _f32(row(min_p, i)))
-        assert int(token[i]) == want, f"row {i}: {int(token[i])}, not {want}"
-        got = float(logprob[i])
+        want = block_oracle.sample(logits[i], float(u[i]), _f32(row(temperature, i)), row(top_k, i), _f32(row(top_p, i)),
+                                   _f32(row(min_p, i)))
+        assert int(token[i]) in want, f"row {i}: {int(token[i])}, not {want}"
+        got, lp = float(logprob[i]), want[int(token[i])]
         assert got == lp or abs(got - lp) <= 2.0 ** -23 * abs(lp) + 1e-9, f"row {i}: logprob {got}, not {lp}"
     return token, logprob
 
