@@ -34,7 +34,7 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleMaxCluster = 8;
 constexpr int kSampleBins = 2048;
 constexpr float kSampleBinsPerNat = 64.f;
-constexpr int kSampleTable = 128;
+constexpr int kSampleTable = 512;
 static_assert(kSampleBins == 4 * kSampleThreads, "a thread owns four bins");
 
 struct SampleParams {
@@ -50,14 +50,25 @@ struct SampleParams {
     float* logprob;  // or nullptr
 };
 
-// The bits of a float that is no NaN in an order-preserving unsigned form.
-__device__ __forceinline__ uint32_t sample_key(float v) {
-    const uint32_t u = __float_as_uint(v + 0.f);  // -0 and +0 are equal logits
-    return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
-}
-__device__ __forceinline__ float sample_key_value(uint32_t key) {
-    return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
-}
+// The order-preserving unsigned form of a logit that is no NaN: the bits of the float, without those that the type
+// leaves empty, so that neighbouring logits have neighbouring keys.
+template <class T>
+struct SampleKey {
+    static constexpr int kLow = std::is_same<T, __nv_bfloat16>::value ? 16 : (std::is_same<T, __half>::value ? 13 : 0);
+    static constexpr uint32_t kZero = 0x80000000u >> kLow;
+    static constexpr uint32_t kNone = 0x007fffffu >> kLow;  // -inf
+    static __device__ __forceinline__ uint32_t of(float v) {
+        const uint32_t u = __float_as_uint(v + 0.f);  // -0 and +0 are equal logits
+        return (u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u)) >> kLow;
+    }
+    static __device__ __forceinline__ float value(uint32_t key) {
+        const uint32_t k = key << kLow;
+        return __uint_as_float(key >= kZero ? k & 0x7fffffffu : ~(k | ((1u << kLow) - 1u)));
+    }
+    // Bounds for comparing logits as floats: the key below zero's belongs to -0, which no logit has but all zeros equal.
+    static __device__ __forceinline__ float at_least(uint32_t key) { return value(key == kZero - 1 ? kZero : key); }
+    static __device__ __forceinline__ float at_most(uint32_t key) { return value(key == kZero - 1 ? kZero - 2 : key); }
+};
 
 // What a CTA of the cluster tells the others at an exchange.
 struct SampleSlot {
@@ -91,33 +102,32 @@ __device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
     return v;
 }
 
-// The weights of one row.
+// The weights of one row (whose maximum is finite).
 struct SampleWeights {
     double top_d, inv_t;
     float top;
     float inv_t32;
     const double* table;
-    // exp(x) for x <= 0 by a table of 2^(i / 128) and a polynomial (Tang, 1989): x = n ln2 / 128 + r, |r| <= ln2 / 256,
-    // exp(x) = 2^(n >> 7) 2^((n & 127) / 128) (1 + r + r^2 / 2 + r^3 / 6 + r^4 / 24): relative error below 1e-14
+    __device__ __forceinline__ double exponent(float v) const { return (static_cast<double>(v) - top_d) * inv_t; }
+    // exp(x) for -700 < x <= 0 by a table of 2^(i / 512) and a polynomial (Tang, 1989): x = n ln2 / 512 + r,
+    // |r| <= ln2 / 1024, exp(x) = 2^(n >> 9) 2^((n & 511) / 512) (1 + r + r^2 / 2 + r^3 / 6): relative error below 1e-14
     __device__ __forceinline__ double exp_below(double x) const {
         constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
-        const double nm = fma(x, 184.6649652337873105, kMagic);  // 128 / ln 2
+        const double nm = fma(x, 738.6598609349492420, kMagic);  // 512 / ln 2
         const int n = __double2loint(nm);
-        const double r = fma(nm - kMagic, -0.005415212348514945209, x);  // ln 2 / 128
-        const double q = fma(r * r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), r);
+        const double r = fma(nm - kMagic, -0.001353803087128736302, x);  // ln 2 / 512
+        const double q = fma(r * r, fma(r, 1.0 / 6, 0.5), r);
         double t = table[n & (kSampleTable - 1)];
-        t = __hiloint2double(__double2hiint(t) + ((n >> 7) << 20), __double2loint(t));
+        t = __hiloint2double(__double2hiint(t) + ((n >> 9) << 20), __double2loint(t));
         return fma(t, q, t);
     }
     __device__ __forceinline__ double operator()(float v) const {
-        if (v == top) return 1.0;
-        const double x = (static_cast<double>(v) - top_d) * inv_t;
-        return x > -700.0 && top < INFINITY ? exp_below(x) : 0.0;
+        const double x = exponent(v);
+        return x > -700.0 ? exp_below(x) : 0.0;
     }
     // bin of the first histogram; does not increase with v
     __device__ __forceinline__ int bin(float v) const {
-        const float z = v == top ? 0.f : (top - v) * inv_t32;
-        return static_cast<int>(fminf(z, static_cast<float>(kSampleBins - 1)));
+        return static_cast<int>(fminf((top - v) * inv_t32, static_cast<float>(kSampleBins - 1)));
     }
 };
 
@@ -157,6 +167,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
 sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas, int vectors_per_warp, int in_smem,
               const SampleParams p) {
     constexpr int VEC = RmsTile<T>::kVec;
+    using Key = SampleKey<T>;
     extern __shared__ __align__(16) unsigned char sample_slice[];
     __shared__ SampleShared sh;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -197,14 +208,29 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         }
         return raw;
     };
-    // All elements of this warp's share: f(values, index of the first)
+    float top = -INFINITY;
+    // A vector as floats. Where the maximum is +inf, all of it is shared among the +inf: they become 0, the rest -inf.
+    auto fetch = [&](int v, float (&x)[VEC]) {
+        const uint4 raw = in_smem ? slice[v - cta_vec0] : read(v);
+        rms_unpack<T>(raw, x);
+        if (top == INFINITY) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) x[j] = x[j] == INFINITY ? 0.f : -INFINITY;
+        }
+    };
+    // The vectors of this warp's share.
     auto scan = [&](auto&& f) {
         for (int v = v0 + lane; v < v1; v += 32) {
-            const uint4 raw = in_smem ? slice[v - cta_vec0] : read(v);
             float x[VEC];
-            rms_unpack<T>(raw, x);
+            fetch(v, x);
             f(x);
         }
+    };
+    auto largest = [&](const float (&x)[VEC]) {
+        float m = x[0];
+#pragma unroll
+        for (int j = 1; j < VEC; ++j) m = fmaxf(m, x[j]);
+        return m;
     };
     int slot_parity = 0;
     // Every CTA's values to every CTA; returns this exchange's slots. Two sets alternate: a CTA writes a set again only
@@ -227,7 +253,6 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
     };
 
     // ---- 1. the slice and the maximum
-    float top = -INFINITY;
     for (int v = v0 + lane; v < v1; v += 32) {
         const uint4 raw = read(v);
         if (in_smem) slice[v - cta_vec0] = raw;
@@ -239,26 +264,25 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
     if (t < kSampleTable) sh.table[t] = exp2(t / static_cast<double>(kSampleTable));
     for (int i = t; i < kSampleBins; i += kSampleThreads) sh.hist[0][i] = sh.hist[1][i] = 0;
     {
-        uint32_t k = __reduce_max_sync(0xffffffffu, sample_key(top));
+        uint32_t k = __reduce_max_sync(0xffffffffu, Key::of(top));
         if (lane == 0) sh.wu[warp] = k;
         __syncthreads();
-        k = 0;
         for (int i = 0; i < kSampleWarps; ++i) k = max(k, sh.wu[i]);
         const SampleSlot* all = exchange(0, 0, 0, 0, k);
         for (int c = 0; c < n_ctas; ++c) k = max(k, all[c].u);
-        top = sample_key_value(k);
+        top = Key::value(k);
     }
     const float temp = p.temperature ? p.temperature[row] : p.temperature_all;
     if (top == -INFINITY || !(temp > 0.f)) {  // the same for the whole cluster
         uint32_t first = 0xffffffffu;
         if (top != -INFINITY) {
+            const float largest_value = top == INFINITY ? 0.f : top;
             for (int v = v0 + lane; v < v1; v += 32) {
-                const uint4 raw = in_smem ? slice[v - cta_vec0] : read(v);
                 float x[VEC];
-                rms_unpack<T>(raw, x);
+                fetch(v, x);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
-                    if (x[j] == top) first = min(first, static_cast<uint32_t>(v) * VEC + j - head);
+                    if (x[j] == largest_value) first = min(first, static_cast<uint32_t>(v) * VEC + j - head);
             }
         }
         first = __reduce_min_sync(0xffffffffu, first);
@@ -275,24 +299,24 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         return;
     }
     SampleWeights weight;
-    weight.top = top;
-    weight.top_d = top;
+    weight.top = top == INFINITY ? 0.f : top;  // fetch() goes by `top` itself
+    weight.top_d = weight.top;
     weight.inv_t = 1.0 / static_cast<double>(temp);
     weight.inv_t32 = fminf(kSampleBinsPerNat / temp, 1e30f);
     weight.table = sh.table;
 
     // ---- histograms
     int hist_parity = 0;
-    // The counts of bins 4t .. 4t + 3 over the whole cluster, f(value) the bin or -1. Two histograms alternate: one is
+    // The counts of bins 4t .. 4t + 3 over the whole cluster, f(value) the bin. Two histograms alternate: one is
     // cleared while the other is in use, a barrier after all CTAs have read it.
-    auto histogram = [&](auto&& f) -> uint4 {
+    // Only values within [low, high] count.
+    auto histogram = [&](float low, float high, auto&& f) -> uint4 {
         uint32_t* h = sh.hist[hist_parity];
         scan([&](const float (&x)[VEC]) {
+            if (largest(x) < low) return;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const int b = f(x[j]);
-                if (b >= 0) atomicAdd(&h[b], 1u);
-            }
+            for (int j = 0; j < VEC; ++j)
+                if (x[j] >= low && x[j] <= high) atomicAdd(&h[f(x[j])], 1u);
         });
         __syncthreads();
         ptx::cluster_sync_all();
@@ -314,11 +338,11 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
     };
     // The keys of one bin of weight.bin, as a range: 32 points at a time, all warps alike.
     auto first_key_of_bin_at_most = [&](int b) {  // the smallest key whose value falls in bin b or an earlier one
-        uint32_t lo = 0x007fffffu, hi = sample_key(top);  // hi does
+        uint32_t lo = Key::kNone, hi = Key::of(weight.top);  // hi does
         while (lo < hi) {
             const uint64_t span = hi - lo;
             const uint32_t at = lo + static_cast<uint32_t>(span * lane / 32);
-            const unsigned yes = __ballot_sync(0xffffffffu, weight.bin(sample_key_value(at)) <= b);
+            const unsigned yes = __ballot_sync(0xffffffffu, weight.bin(Key::value(at)) <= b);
             const int i = yes ? __ffs(yes) - 1 : 32;  // points i .. 31 and hi do
             const uint32_t new_hi = i < 32 ? lo + static_cast<uint32_t>(span * i / 32) : hi;
             if (i > 0) lo = lo + static_cast<uint32_t>(span * (i - 1) / 32) + 1;
@@ -327,6 +351,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         return hi;
     };
 
+    const float lowest = Key::value(Key::kNone + 1);  // the smallest finite value
     // What is kept: values above `bound`, and `ties` of those equal to it in index order. -inf: everything.
     float bound = -INFINITY;
     long long ties = 0;
@@ -339,11 +364,9 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         long long above = 0;  // values above the bracket
         bool all = true;  // fewer than k values above -inf
         for (int round = 0; round < 4; ++round) {  // the first histogram, then 32 bits in steps of 11
-            const uint4 c = shift < 0 ? histogram([&](float v) { return v > -INFINITY ? weight.bin(v) : -1; })
-                                      : histogram([&](float v) {
-                                            const uint32_t q = sample_key(v);
-                                            return q >= lo && q <= hi ? static_cast<int>((hi - q) >> shift) : -1;
-                                        });
+            const uint4 c = shift < 0 ? histogram(lowest, weight.top, [&](float v) { return weight.bin(v); })
+                                      : histogram(Key::at_least(lo), Key::at_most(hi),
+                                                  [&](float v) { return static_cast<int>((hi - Key::of(v)) >> shift); });
             clear_other();
             const long long cs[4] = {c.x, c.y, c.z, c.w};
             long long run = above + sample_block_before<long long>(cs[0] + cs[1] + cs[2] + cs[3], sh.wn);
@@ -368,7 +391,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
             }
             if (shift < 0) {
                 lo = first_key_of_bin_at_most(static_cast<int>(b));
-                hi = b == 0 ? sample_key(top) : first_key_of_bin_at_most(static_cast<int>(b) - 1) - 1;
+                hi = b == 0 ? Key::of(weight.top) : first_key_of_bin_at_most(static_cast<int>(b) - 1) - 1;
             } else {
                 hi -= b << shift;
                 lo = max(lo, hi - ((1u << shift) - 1u));
@@ -377,13 +400,16 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
             while (((hi - lo) >> shift) >= kSampleBins) ++shift;
         }
         if (!all) {
-            bound = sample_key_value(lo);
+            bound = Key::value(lo);
             ties = k - above;
         }
     }
 
     // ---- 2., 3., 4. top_p: the smallest value whose predecessors' weights stay within the limit
     const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
+    bool carry = false;  // whether this thread's weights above the bracket are summed already, as `carried`
+    double carried = 0;
+    float carry_low = 0, carry_high = 0;  // the bracket
     if (top_p < 1.f) {
         const float floor_value = bound;  // only values above it take part; `extra` is the ties' weight
         const double extra = ties > 0 ? ties * weight(bound) : 0.0;
@@ -392,7 +418,8 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         double above = 0, limit;  // weight above the bracket; the largest sum of predecessors
         bool found = false;   // the threshold is in the bracket
         {
-            const uint4 c = histogram([&](float v) { return v > floor_value ? weight.bin(v) : -1; });
+            const float low_end = floor_value == -INFINITY ? lowest : Key::value(Key::of(floor_value) + 1);
+            const uint4 c = histogram(low_end, weight.top, [&](float v) { return weight.bin(v); });
             clear_other();
             const double cs[4] = {double(c.x), double(c.y), double(c.z), double(c.w)};
             double up[4], low[4];
@@ -426,21 +453,28 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
             }
             __syncthreads();
             const int b1 = static_cast<int>(sh.first_u), b2 = max(b1, static_cast<int>(sh.first_l));
-            hi = b1 == 0 ? sample_key(top) : first_key_of_bin_at_most(b1 - 1) - 1;
-            lo = b2 == kSampleBins - 1 ? 0x00800000u : first_key_of_bin_at_most(b2);
-            double s[3] = {0, 0, 0};  // above, inside, below
+            hi = b1 == 0 ? Key::of(weight.top) : first_key_of_bin_at_most(b1 - 1) - 1;
+            lo = b2 == kSampleBins - 1 ? Key::kNone + 1 : first_key_of_bin_at_most(b2);
+            double s[3] = {0, 0, 0};  // all, inside and above the bracket, above it
+            const float in_low = Key::at_least(lo), in_high = Key::at_most(hi);
             scan([&](const float (&x)[VEC]) {
+                const bool reaches = largest(x) >= in_low;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    if (x[j] > floor_value) {
-                        const double w = weight(x[j]);
-                        const uint32_t q = sample_key(x[j]);
-                        if (q > hi) s[0] += w;
-                        else if (q >= lo) s[1] += w;
-                        else s[2] += w;
+                    const double e = weight.exponent(x[j]);
+                    const double w = weight.exp_below(e);
+                    if (e > -700.0 && x[j] > floor_value) {
+                        s[0] += w;
+                        if (reaches) {
+                            if (x[j] >= in_low) s[1] += w;
+                            if (x[j] > in_high) s[2] += w;
+                        }
                     }
                 }
             });
+            carried = s[2];
+            carry_low = in_low;
+            carry_high = in_high;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
@@ -460,25 +494,25 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
                 s[1] += all[c2].d[1];
                 s[2] += all[c2].d[2];
             }
-            const double all_above = s[0] + s[1] + s[2];
-            limit = share * (all_above + extra);
-            const uint32_t floor_key = sample_key(floor_value);
-            if (all_above <= limit) {
-                above = all_above;  // every value above the floor is kept
-            } else if (s[0] > limit) {  // outside the bounds' bracket (they leave room for rounding, but to be sure)
+            limit = share * (s[0] + extra);
+            const uint32_t floor_key = Key::of(floor_value);
+            if (s[0] <= limit) {
+                above = s[0];  // every value above the floor is kept
+                found = false;
+            } else if (s[2] > limit) {  // outside the bounds' bracket (they leave room for rounding, but to be sure)
                 found = true;
                 lo = hi + 1;
-                hi = sample_key(top);
+                hi = Key::of(weight.top);
                 above = 0;
-            } else if (s[0] + s[1] > limit) {
-                found = true;
+            } else if (s[1] > limit) {
+                found = carry = true;
                 lo = max(lo, floor_key + 1);
-                above = s[0];
+                above = s[2];
             } else {
                 found = true;
                 hi = lo - 1;
                 lo = floor_key + 1;
-                above = s[0] + s[1];
+                above = s[1];
             }
         }
         if (!found) {
@@ -494,10 +528,8 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
             for (int round = 0; round < 1 << 16; ++round) {
                 int shift = 0;
                 while (((hi - lo) >> shift) >= kSampleBins) ++shift;
-                const uint4 c = histogram([&](float v) {
-                    const uint32_t q = sample_key(v);
-                    return q >= lo && q <= hi ? static_cast<int>((hi - q) >> shift) : -1;
-                });
+                const uint4 c = histogram(Key::at_least(lo), Key::at_most(hi),
+                                          [&](float v) { return static_cast<int>((hi - Key::of(v)) >> shift); });
                 clear_other();
                 const double cs[4] = {double(c.x), double(c.y), double(c.z), double(c.w)};
                 double up[4], low[4];
@@ -505,8 +537,8 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t off = static_cast<uint32_t>(4 * t + j) << shift, last = off + ((1u << shift) - 1u);
                     const bool in = off <= hi - lo;
-                    up[j] = in && cs[j] > 0 ? cs[j] * weight(sample_key_value(hi - off)) : 0.0;
-                    low[j] = in && cs[j] > 0 ? (shift == 0 ? up[j] : cs[j] * weight(sample_key_value(hi - min(last, hi - lo)))) : 0.0;
+                    up[j] = in && cs[j] > 0 ? cs[j] * weight(Key::value(hi - off)) : 0.0;
+                    low[j] = in && cs[j] > 0 ? (shift == 0 ? up[j] : cs[j] * weight(Key::value(hi - min(last, hi - lo)))) : 0.0;
                 }
                 const double up_run = above + sample_block_before<double>(up[0] + up[1] + up[2] + up[3], sh.wd[0]);
                 const double low_run = above + sample_block_before<double>(low[0] + low[1] + low[2] + low[3], sh.wd[1]);
@@ -545,7 +577,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
                         run += up[j];
                     }
                     __syncthreads();
-                    bound = sample_key_value(hi - b1);
+                    bound = Key::value(hi - b1);
                     const double w1 = weight(bound), ahead = sh.total_d[0];
                     const long long equal = sh.count;
                     // tie number i (from 0) is kept while ahead + i w <= limit; the very first value always
@@ -554,7 +586,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
                         const double room = (limit - ahead) / w1;
                         most = room < 0 ? 0 : static_cast<long long>(fmin(room, 4e9)) + 1;
                     }
-                    if (bound == top && most < 1) most = 1;
+                    if (bound == weight.top && most < 1) most = 1;
                     ties = most < equal ? most : equal;
                     break;
                 }
@@ -564,13 +596,14 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
                 const uint32_t b2_hi = hi - (b2 << shift);
                 const uint32_t b2_lo = max(lo, b2_hi - ((1u << shift) - 1u));
                 double s[2] = {0, 0};
+                const float f_hi = Key::at_most(hi), f1_hi = Key::at_most(b1_hi), f1_lo = Key::at_least(b1_lo);
                 scan([&](const float (&x)[VEC]) {
+                    if (largest(x) < f1_lo) return;
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
-                        const uint32_t q = sample_key(x[j]);
-                        if (q <= hi && q >= b1_lo) {
+                        if (x[j] <= f_hi && x[j] >= f1_lo) {
                             const double wv = weight(x[j]);
-                            if (q > b1_hi) s[0] += wv;
+                            if (x[j] > f1_hi) s[0] += wv;
                             else s[1] += wv;
                         }
                     }
@@ -616,13 +649,28 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
     const double w_tie = ties > 0 ? kept_weight(bound) : 0.0;
     double sum = 0;
     long long equal = 0;
-    scan([&](const float (&x)[VEC]) {
+    if (carry && min_p == 0.0) {  // what is left to add lies inside the bracket
+        sum = carried;
+        scan([&](const float (&x)[VEC]) {
+            if (largest(x) < carry_low) return;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            if (x[j] > bound) sum += kept_weight(x[j]);
-            else if (x[j] == bound) ++equal;
-        }
-    });
+            for (int j = 0; j < VEC; ++j) {
+                if (x[j] >= carry_low && x[j] <= carry_high) {
+                    if (x[j] > bound) sum += weight(x[j]);
+                    else if (x[j] == bound) ++equal;
+                }
+            }
+        });
+    } else {
+        scan([&](const float (&x)[VEC]) {
+            if (largest(x) < bound) return;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (x[j] > bound) sum += kept_weight(x[j]);
+                else if (x[j] == bound) ++equal;
+            }
+        });
+    }
     sum = sample_warp_sum(sum);
     equal = sample_warp_sum(equal);
     __syncthreads();
@@ -696,8 +744,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         float x[VEC];
         int n_equal = 0;
         if (v < v1) {
-            const uint4 raw = in_smem ? slice[v - cta_vec0] : read(v);
-            rms_unpack<T>(raw, x);
+            fetch(v, x);
         } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) x[j] = -INFINITY;
