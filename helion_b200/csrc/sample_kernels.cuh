@@ -14,10 +14,10 @@
 //
 // No sort. A prefix of the order is a threshold on the logit and a number of ties, and both are found by counting:
 //   1. a cluster of 1..8 CTAs takes a row; each keeps its slice in shared memory, so the logits are read once;
-//   2. a histogram of (max - l) / temperature in steps of 1/64 brackets the threshold: exactly for top_k, and for top_p
-//      between bounds, since a bin's weights are known to e^(1/64) from its count;
+//   2. a histogram of (max - l) / temperature brackets the threshold: exactly for top_k, and for top_p between bounds,
+//      since a bin's weights are known to the bin's width from its count;
 //   3. for top_p one pass sums all weights, and those above the bracket, in 64 bits;
-//   4. histograms over the ordered bits of the logits inside the bracket (2048 bins each) narrow it to a single value;
+//   4. histograms over the ordered bits of the logits inside the bracket narrow it to a single value;
 //      only elements inside the bracket need their weight for that;
 //   5. one pass sums the kept weights by warp, the sums find the warp that holds u times the total, and that warp
 //      finds the index.
@@ -32,10 +32,7 @@ namespace lce {
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleMaxCluster = 8;
-constexpr int kSampleBins = 2048;
-constexpr float kSampleBinsPerNat = 64.f;
 constexpr int kSampleTable = 512;
-static_assert(kSampleBins == 4 * kSampleThreads, "a thread owns four bins");
 
 struct SampleParams {
     const float* uniform;      // [rows]
@@ -70,6 +67,15 @@ struct SampleKey {
     static __device__ __forceinline__ float at_most(uint32_t key) { return value(key == kZero - 1 ? kZero - 2 : key); }
 };
 
+// Bins of a histogram, and how many of them the first one has per unit of (max - l) / temperature (32 units in all).
+// Every CTA reads all the others' bins, at some 30 bytes per ns through the cluster: with 2048 bins a round on 8 CTAs
+// took 4.8 us, 2.2 of them for that. With 512, logits of 16 bits around zero took more rounds (256 x 128256 bf16: 247 us
+// against 217).
+constexpr int kSampleBins = 1024;
+constexpr int kSampleBinsPerThread = kSampleBins / kSampleThreads;
+constexpr float kSampleBinsPerNat = kSampleBins / 32;
+constexpr double kSampleBinStep = 0.969233234476344055;  // exp(-1 / kSampleBinsPerNat)
+
 // What a CTA of the cluster tells the others at an exchange.
 struct SampleSlot {
     double d[3];
@@ -82,7 +88,7 @@ struct SampleShared {
     double table[kSampleTable];  // 2^(i / 128)
     SampleSlot slots[2][kSampleMaxCluster];
     double wd[3][kSampleWarps];
-    long long wn[kSampleWarps];
+    long long wn[1][kSampleWarps];
     uint32_t wu[kSampleWarps];
     double total_d[2];
     unsigned first_u, first_l;
@@ -96,10 +102,8 @@ __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
 __device__ __forceinline__ void st_cluster_s64(uint32_t addr, long long v) {
     asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
-__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void ld_cluster(uint32_t addr, uint32_t (&v)[2]) {
+    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory");
 }
 
 // The weights of one row (whose maximum is finite).
@@ -125,9 +129,9 @@ struct SampleWeights {
         const double x = exponent(v);
         return x > -700.0 ? exp_below(x) : 0.0;
     }
-    // bin of the first histogram; does not increase with v
-    __device__ __forceinline__ int bin(float v) const {
-        return static_cast<int>(fminf((top - v) * inv_t32, static_cast<float>(kSampleBins - 1)));
+    // bin of the first histogram, of `bins`; does not increase with v
+    __device__ __forceinline__ int bin(float v, int bins) const {
+        return static_cast<int>(fminf((top - v) * inv_t32, static_cast<float>(bins - 1)));
     }
 };
 
@@ -148,18 +152,26 @@ __device__ __forceinline__ V sample_warp_scan(V v) {  // inclusive
     return v;
 }
 
-// Sum of the values of the threads before this one; `tmp` holds one value per warp.
-template <class V>
-__device__ __forceinline__ V sample_block_before(V v, V* tmp) {
+// Sums of the values of the threads before this one, for N values side by side; `tmp` holds one value per warp for each.
+template <int N, class V>
+__device__ __forceinline__ void sample_block_before(V (&v)[N], V (*tmp)[kSampleWarps]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const V incl = sample_warp_scan(v);
+    V incl[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) incl[i] = sample_warp_scan(v[i]);
     __syncthreads();
-    if (lane == 31) tmp[warp] = incl;
+    if (lane == 31) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) tmp[i][warp] = incl[i];
+    }
     __syncthreads();
-    V base = 0;
-    for (int i = 0; i < warp; ++i) base += tmp[i];
-    const V up = __shfl_up_sync(0xffffffffu, incl, 1);
-    return base + (lane == 0 ? V(0) : up);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const V warps = sample_warp_scan(lane < kSampleWarps ? tmp[i][lane] : V(0));
+        const V base = __shfl_sync(0xffffffffu, warps, warp == 0 ? 0 : warp - 1);
+        const V up = __shfl_up_sync(0xffffffffu, incl[i], 1);
+        v[i] = (warp == 0 ? V(0) : base) + (lane == 0 ? V(0) : up);
+    }
 }
 
 template <class T>
@@ -168,6 +180,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
               const SampleParams p) {
     constexpr int VEC = RmsTile<T>::kVec;
     using Key = SampleKey<T>;
+    constexpr int kBins = kSampleBins, PER = kSampleBinsPerThread;
     extern __shared__ __align__(16) unsigned char sample_slice[];
     __shared__ SampleShared sh;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -262,7 +275,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         for (int j = 0; j < VEC; ++j) top = fmaxf(top, x[j]);
     }
     if (t < kSampleTable) sh.table[t] = exp2(t / static_cast<double>(kSampleTable));
-    for (int i = t; i < kSampleBins; i += kSampleThreads) sh.hist[0][i] = sh.hist[1][i] = 0;
+    for (int i = t; i < kBins; i += kSampleThreads) sh.hist[0][i] = sh.hist[1][i] = 0;
     {
         uint32_t k = __reduce_max_sync(0xffffffffu, Key::of(top));
         if (lane == 0) sh.wu[warp] = k;
@@ -307,10 +320,10 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
 
     // ---- histograms
     int hist_parity = 0;
-    // The counts of bins 4t .. 4t + 3 over the whole cluster, f(value) the bin. Two histograms alternate: one is
+    // The counts of this thread's bins (PER t and on) over the whole cluster, f(value) the bin. Two histograms alternate: one is
     // cleared while the other is in use, a barrier after all CTAs have read it.
     // Only values within [low, high] count.
-    auto histogram = [&](float low, float high, auto&& f) -> uint4 {
+    auto histogram = [&](float low, float high, uint32_t* sum, auto&& f) {
         uint32_t* h = sh.hist[hist_parity];
         scan([&](const float (&x)[VEC]) {
             if (largest(x) < low) return;
@@ -320,35 +333,49 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         });
         __syncthreads();
         ptx::cluster_sync_all();
-        uint4 sum = make_uint4(0, 0, 0, 0);
-        for (int c = 0; c < n_ctas; ++c) {
-            const uint4 o = ld_cluster_v4(ptx::map_to_cta(ptx::smem_u32(&h[4 * t]), c));
-            sum.x += o.x;
-            sum.y += o.y;
-            sum.z += o.z;
-            sum.w += o.w;
-        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sum[j] = 0;
+        uint32_t o[kSampleMaxCluster][PER] = {};
+#pragma unroll
+        for (int c = 0; c < kSampleMaxCluster; ++c)  // all in flight together
+            if (c < n_ctas) ld_cluster(ptx::map_to_cta(ptx::smem_u32(&h[PER * t]), c), o[c]);
+#pragma unroll
+        for (int c = 0; c < kSampleMaxCluster; ++c)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) sum[j] += o[c][j];
         hist_parity ^= 1;
-        return sum;
     };
     auto clear_other = [&]() {  // the histogram after next: read by all before the barrier that has just passed
         uint32_t* h = sh.hist[hist_parity];
-        for (int i = t; i < kSampleBins; i += kSampleThreads) h[i] = 0;
+        for (int i = t; i < kBins; i += kSampleThreads) h[i] = 0;
         __syncthreads();
     };
-    // The keys of one bin of weight.bin, as a range: 32 points at a time, all warps alike.
-    auto first_key_of_bin_at_most = [&](int b) {  // the smallest key whose value falls in bin b or an earlier one
+    // The smallest key whose value falls in bin b of weight.bin or an earlier one, by 32 points at a time.
+    auto first_key_of_bin_at_most = [&](int b) {
         uint32_t lo = Key::kNone, hi = Key::of(weight.top);  // hi does
         while (lo < hi) {
             const uint64_t span = hi - lo;
             const uint32_t at = lo + static_cast<uint32_t>(span * lane / 32);
-            const unsigned yes = __ballot_sync(0xffffffffu, weight.bin(Key::value(at)) <= b);
+            const unsigned yes = __ballot_sync(0xffffffffu, weight.bin(Key::value(at), kBins) <= b);
             const int i = yes ? __ffs(yes) - 1 : 32;  // points i .. 31 and hi do
             const uint32_t new_hi = i < 32 ? lo + static_cast<uint32_t>(span * i / 32) : hi;
             if (i > 0) lo = lo + static_cast<uint32_t>(span * (i - 1) / 32) + 1;
             hi = new_hi;
         }
         return hi;
+    };
+    // The keys of bins b1 .. b2, found by two warps side by side.
+    auto bracket_of_bins = [&](int b1, int b2, uint32_t& lo, uint32_t& hi) {
+        if (warp == 0) {
+            const uint32_t k = b2 == kBins - 1 ? Key::kNone + 1 : first_key_of_bin_at_most(b2);
+            if (lane == 0) sh.first_l = k;
+        } else if (warp == 1) {
+            const uint32_t k = b1 == 0 ? Key::of(weight.top) : first_key_of_bin_at_most(b1 - 1) - 1;
+            if (lane == 0) sh.first_u = k;
+        }
+        __syncthreads();
+        lo = sh.first_l;
+        hi = sh.first_u;
     };
 
     const float lowest = Key::value(Key::kNone + 1);  // the smallest finite value
@@ -363,19 +390,22 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         int shift = -1;  // -1: the first histogram
         long long above = 0;  // values above the bracket
         bool all = true;  // fewer than k values above -inf
-        for (int round = 0; round < 4; ++round) {  // the first histogram, then 32 bits in steps of 11
-            const uint4 c = shift < 0 ? histogram(lowest, weight.top, [&](float v) { return weight.bin(v); })
-                                      : histogram(Key::at_least(lo), Key::at_most(hi),
-                                                  [&](float v) { return static_cast<int>((hi - Key::of(v)) >> shift); });
+        for (int round = 0; round < 6; ++round) {  // the first histogram, then the bracket in steps of 10 bits
+            uint32_t cs[PER];
+            if (shift < 0) histogram(lowest, weight.top, cs, [&](float v) { return weight.bin(v, kBins); });
+            else histogram(Key::at_least(lo), Key::at_most(hi), cs, [&](float v) { return static_cast<int>((hi - Key::of(v)) >> shift); });
             clear_other();
-            const long long cs[4] = {c.x, c.y, c.z, c.w};
-            long long run = above + sample_block_before<long long>(cs[0] + cs[1] + cs[2] + cs[3], sh.wn);
-            if (t == 0) sh.bin = kSampleBins;
+            long long before[1] = {0};
+#pragma unroll
+            for (int j = 0; j < PER; ++j) before[0] += cs[j];
+            sample_block_before<1>(before, sh.wn);
+            long long run = above + before[0];
+            if (t == 0) sh.bin = kBins;
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < PER; ++j) {
                 if (run < k && k <= run + cs[j]) {
-                    sh.bin = 4 * t + j;
+                    sh.bin = PER * t + j;
                     sh.before = run;
                 }
                 run += cs[j];
@@ -383,21 +413,20 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
             __syncthreads();
             const uint32_t b = sh.bin;
             above = sh.before;
-            if (b == kSampleBins) break;
+            if (b == kBins) break;
             all = false;
             if (shift == 0) {
                 lo = hi = hi - b;
                 break;
             }
             if (shift < 0) {
-                lo = first_key_of_bin_at_most(static_cast<int>(b));
-                hi = b == 0 ? Key::of(weight.top) : first_key_of_bin_at_most(static_cast<int>(b) - 1) - 1;
+                bracket_of_bins(static_cast<int>(b), static_cast<int>(b), lo, hi);
             } else {
                 hi -= b << shift;
                 lo = max(lo, hi - ((1u << shift) - 1u));
             }
             shift = 0;
-            while (((hi - lo) >> shift) >= kSampleBins) ++shift;
+            while (((hi - lo) >> shift) >= kBins) ++shift;
         }
         if (!all) {
             bound = Key::value(lo);
@@ -419,42 +448,40 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
         bool found = false;   // the threshold is in the bracket
         {
             const float low_end = floor_value == -INFINITY ? lowest : Key::value(Key::of(floor_value) + 1);
-            const uint4 c = histogram(low_end, weight.top, [&](float v) { return weight.bin(v); });
+            uint32_t cs[PER];
+            histogram(low_end, weight.top, cs, [&](float v) { return weight.bin(v, kBins); });
             clear_other();
-            const double cs[4] = {double(c.x), double(c.y), double(c.z), double(c.w)};
-            double up[4], low[4];
-            // weights of bin b are within e^-((b + 1) / 64) .. e^-(b / 64), and 1e-4 for the bin's 32-bit arithmetic
+            double up[PER], low[PER], sums[2] = {0, 0};
+            // weights of bin b are within e^-((b + 1) / kPerNat) .. e^-(b / kPerNat), and 1e-4 for the bin's 32-bit arithmetic
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const double e = weight.exp_below(-(4 * t + j) / static_cast<double>(kSampleBinsPerNat));
+            for (int j = 0; j < PER; ++j) {
+                const double e = weight.exp_below(-(PER * t + j) / static_cast<double>(kSampleBinsPerNat));
                 up[j] = cs[j] * e * 1.0001;
-                low[j] = 4 * t + j == kSampleBins - 1 ? 0.0 : cs[j] * e * (0.9845 * 0.9999);  // e^(-1/64) = 0.98450
+                low[j] = PER * t + j == kBins - 1 ? 0.0 : cs[j] * e * (kSampleBinStep * 0.9999);
+                sums[0] += up[j];
+                sums[1] += low[j];
             }
-            const double up_sum = up[0] + up[1] + up[2] + up[3], low_sum = low[0] + low[1] + low[2] + low[3];
-            double up_run = sample_block_before<double>(up_sum, sh.wd[0]);
-            double low_run = sample_block_before<double>(low_sum, sh.wd[1]);
+            const double up_sum = sums[0], low_sum = sums[1];
+            sample_block_before<2>(sums, sh.wd);
             if (t == kSampleThreads - 1) {
-                sh.total_d[0] = up_run + up_sum;
-                sh.total_d[1] = low_run + low_sum;
-                sh.first_u = sh.first_l = kSampleBins - 1;
+                sh.total_d[0] = sums[0] + up_sum;
+                sh.total_d[1] = sums[1] + low_sum;
+                sh.first_u = sh.first_l = kBins - 1;
             }
             __syncthreads();
             const double least = share * (sh.total_d[1] + extra), most = share * (sh.total_d[0] + extra);
 #pragma unroll
-            for (int j = 3; j >= 0; --j) {
+            for (int j = 0; j < PER; ++j) {
                 // the first bin whose upper sum may pass the limit, the first whose lower sum must
-                double u = up_run, w = low_run;
-                for (int i = 0; i <= j; ++i) {
-                    u += up[i];
-                    w += low[i];
-                }
-                if (cs[j] > 0 && u >= least) atomicMin(&sh.first_u, static_cast<unsigned>(4 * t + j));
-                if (cs[j] > 0 && w > most) atomicMin(&sh.first_l, static_cast<unsigned>(4 * t + j));
+                sums[0] += up[j];
+                sums[1] += low[j];
+                if (cs[j] > 0 && sums[0] >= least) atomicMin(&sh.first_u, static_cast<unsigned>(PER * t + j));
+                if (cs[j] > 0 && sums[1] > most) atomicMin(&sh.first_l, static_cast<unsigned>(PER * t + j));
             }
             __syncthreads();
             const int b1 = static_cast<int>(sh.first_u), b2 = max(b1, static_cast<int>(sh.first_l));
-            hi = b1 == 0 ? Key::of(weight.top) : first_key_of_bin_at_most(b1 - 1) - 1;
-            lo = b2 == kSampleBins - 1 ? Key::kNone + 1 : first_key_of_bin_at_most(b2);
+            __syncthreads();
+            bracket_of_bins(b1, b2, lo, hi);
             double s[3] = {0, 0, 0};  // all, inside and above the bracket, above it
             const float in_low = Key::at_least(lo), in_high = Key::at_most(hi);
             scan([&](const float (&x)[VEC]) {
@@ -527,35 +554,36 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
             // every round narrows the bracket to one bin, or by one bin that has values: a few rounds, thousands at the worst
             for (int round = 0; round < 1 << 16; ++round) {
                 int shift = 0;
-                while (((hi - lo) >> shift) >= kSampleBins) ++shift;
-                const uint4 c = histogram(Key::at_least(lo), Key::at_most(hi),
-                                          [&](float v) { return static_cast<int>((hi - Key::of(v)) >> shift); });
+                while (((hi - lo) >> shift) >= kBins) ++shift;
+                uint32_t cs[PER];
+                histogram(Key::at_least(lo), Key::at_most(hi), cs, [&](float v) { return static_cast<int>((hi - Key::of(v)) >> shift); });
                 clear_other();
-                const double cs[4] = {double(c.x), double(c.y), double(c.z), double(c.w)};
-                double up[4], low[4];
+                double up[PER], low[PER], sums[2] = {0, 0};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t off = static_cast<uint32_t>(4 * t + j) << shift, last = off + ((1u << shift) - 1u);
-                    const bool in = off <= hi - lo;
-                    up[j] = in && cs[j] > 0 ? cs[j] * weight(Key::value(hi - off)) : 0.0;
-                    low[j] = in && cs[j] > 0 ? (shift == 0 ? up[j] : cs[j] * weight(Key::value(hi - min(last, hi - lo)))) : 0.0;
+                for (int j = 0; j < PER; ++j) {
+                    const uint32_t off = static_cast<uint32_t>(PER * t + j) << shift, last = off + ((1u << shift) - 1u);
+                    const bool in = off <= hi - lo && cs[j] > 0;
+                    up[j] = in ? cs[j] * weight(Key::value(hi - off)) : 0.0;
+                    low[j] = in ? (shift == 0 ? up[j] : cs[j] * weight(Key::value(hi - min(last, hi - lo)))) : 0.0;
+                    sums[0] += up[j];
+                    sums[1] += low[j];
                 }
-                const double up_run = above + sample_block_before<double>(up[0] + up[1] + up[2] + up[3], sh.wd[0]);
-                const double low_run = above + sample_block_before<double>(low[0] + low[1] + low[2] + low[3], sh.wd[1]);
-                if (t == 0) sh.first_u = sh.first_l = kSampleBins;
+                sample_block_before<2>(sums, sh.wd);
+                const double up_run = above + sums[0], low_run = above + sums[1];
+                if (t == 0) sh.first_u = sh.first_l = kBins;
                 __syncthreads();
                 // a hair of room on both sides while the bins hold several values; none once they are single ones
                 const double hair = shift == 0 ? 0.0 : 1e-9 * limit;
                 unsigned last_full = 0;
                 double u = up_run, w = low_run;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < PER; ++j) {
                     u += up[j];
                     w += low[j];
                     if (cs[j] > 0) {
-                        last_full = 4 * t + j + 1;
-                        if (u > limit - hair) atomicMin(&sh.first_u, static_cast<unsigned>(4 * t + j));
-                        if (w > limit + hair) atomicMin(&sh.first_l, static_cast<unsigned>(4 * t + j));
+                        last_full = PER * t + j + 1;
+                        if (u > limit - hair) atomicMin(&sh.first_u, static_cast<unsigned>(PER * t + j));
+                        if (w > limit + hair) atomicMin(&sh.first_l, static_cast<unsigned>(PER * t + j));
                     }
                 }
                 last_full = __reduce_max_sync(0xffffffffu, last_full);
@@ -569,8 +597,8 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
                     __syncthreads();
                     double run = up_run;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (static_cast<uint32_t>(4 * t + j) == b1) {
+                    for (int j = 0; j < PER; ++j) {
+                        if (static_cast<uint32_t>(PER * t + j) == b1) {
                             sh.total_d[0] = run;
                             sh.count = static_cast<long long>(cs[j]);
                         }
@@ -676,14 +704,14 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
     __syncthreads();
     if (lane == 0) {
         sh.wd[0][warp] = sum;
-        sh.wn[warp] = equal;
+        sh.wn[0][warp] = equal;
     }
     __syncthreads();
     sum = 0;
     equal = 0;
     for (int i = 0; i < kSampleWarps; ++i) {
         sum += sh.wd[0][i];
-        equal += sh.wn[i];
+        equal += sh.wn[0][i];
     }
     const SampleSlot* all = exchange(sum, 0, 0, equal, 0);
     auto ties_kept = [&](long long before, long long n) {
@@ -722,7 +750,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
     before = tie_start;
     owner = -1;
     for (int i = 0; i < kSampleWarps; ++i) {
-        const double s = sh.wd[0][i] + ties_kept(before, sh.wn[i]) * w_tie;
+        const double s = sh.wd[0][i] + ties_kept(before, sh.wn[0][i]) * w_tie;
         if (s > 0) {
             owner = i;
             start = run;
@@ -730,7 +758,7 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
             if (run + s > target) break;
         }
         run += s;
-        before += sh.wn[i];
+        before += sh.wn[0][i];
     }
     if (warp != owner) return;
     target -= start;
