@@ -69,10 +69,11 @@ struct TileCtx {
     int row_in_tile;  // 0..127, the row this thread owns
     int bn;           // tile width in columns
     int k_slice;      // which slice of the contraction this tile holds (0 unless K is split)
-    float* stage;     // this warp's 32 x 33 floats of shared memory for re-shaping a chunk, or nullptr
+    float* stage;     // this warp's 32 x 33 floats of shared memory for re-shaping a chunk (256 more follow), or nullptr
 };
 
-constexpr int kStageFloatsPerWarp = 32 * 33;
+constexpr int kStageBiasOffset = 32 * 33;  // behind the re-shaping area: 256 floats for a tile's slice of a bias
+constexpr int kStageFloatsPerWarp = kStageBiasOffset + 256;
 
 template <int BN, int STAGES, int CG>
 struct GemmSmem {

@@ -7,6 +7,9 @@
 namespace lce {
 namespace {
 
+// The row pitch of what a forward saves for its backward: whole 16-byte vectors whatever the type.
+inline long long pre_pitch(long long N) { return cdiv(N, 8) * 8; }
+
 constexpr long long kDzCtas = 592;  // CTAs that the column sums of the backward aim for (4 per SM on 148 SMs)
 
 // Scratch of one product C[M, N] = A[M, K] B[N, K]^T: slabs of a split contraction.
@@ -69,7 +72,8 @@ int product(const DeviceInfo& d, const ProductPlan& p, const Operand& a, const O
     ep.t = tail;
     ep.scratch = p.splits > 1 ? static_cast<float*>(scratch) : nullptr;
     ep.slab_floats = p.slab_floats;
-    ep.wide = wide_stores(tail.out, tail.ldo);
+    ep.wide_out = wide_stores(tail.out, tail.ldo);
+    ep.wide_residual = wide_stores(tail.residual, tail.ldr);
     const Mat am{a.ptr, a.rows, a.cols, a.ld}, bm{b.ptr, b.rows, b.cols, b.ld};
     int rc = LCE_ERR_ARG;
     if (p.use_tc) {
@@ -155,13 +159,13 @@ int linear_backward_impl(const DeviceInfo& d, BackwardPlan& b, const void* dy, l
     if (dbias || (products && b.copy_dz)) {
         constexpr int VEC = 16 / sizeof(T);
         const dim3 grid(static_cast<unsigned>(cdiv(N, 32 * VEC)), static_cast<unsigned>(b.slabs));
-        linear_dz_kernel<T, VEC><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), ldy, static_cast<const T*>(pre),
+        linear_dz_kernel<T, VEC><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), ldy, static_cast<const T*>(pre), pre_pitch(N),
                                                       b.copy_dz ? dz : nullptr, b.ldz, dbias ? sums : nullptr, M,
                                                       static_cast<int>(N), b.rows_per_slab, act);
         LCE_COUNT_LAUNCH();
         if (cuda_failed(cudaGetLastError())) return LCE_ERR_CUDA;
         if (dbias) {
-            const cudaError_t err = launch_dependent(linear_dbias_kernel<T>, static_cast<int>(cdiv(N, 256)), 256, s,
+            const cudaError_t err = launch_dependent(linear_dbias_kernel<T>, static_cast<int>(cdiv(N, 32)), 1024, s,
                                                      static_cast<const float*>(sums), static_cast<int>(b.slabs),
                                                      static_cast<int>(N), static_cast<T*>(dbias));
             LCE_COUNT_LAUNCH();
@@ -221,7 +225,7 @@ int lce_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
 #define LCE_LINEAR_FORWARD(T)                                                                                              \
     forward_impl<T>(*d, xo, wo, p, M, N, K,                                                                                \
                     LinearTail<T>{static_cast<T*>(out), ldo, act == LCE_ACT_NONE ? nullptr : static_cast<T*>(pre),         \
-                                  static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<int>(M),  \
+                                  pre_pitch(N), static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<int>(M),  \
                                   static_cast<int>(N), act},                                                               \
                     scratch, s)
     switch (dtype) {

@@ -73,7 +73,7 @@ def _forward(x, weight, bias, residual, act: int, save: bool):
     n = w2.shape[0]
     b = bias.contiguous() if bias is not None else None
     out = torch.empty((m, n), dtype=x.dtype, device=dev)
-    pre = torch.empty_like(out) if save and act else None
+    pre = torch.empty((m, (n + 7) // 8 * 8), dtype=x.dtype, device=dev) if save and act else None
     if m == 0:
         return out, pre
     L = _lib.lib()

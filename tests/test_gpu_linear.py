@@ -271,7 +271,8 @@ def test_outputs_stay_inside_their_buffers(m, k, n, ldo, dtype):
     code = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}[dtype]
     x, w, b, r, dy = _case(m, k, n, dtype, grad=False)
     out = torch.full((m + 2, ldo), 7.0, dtype=dtype, device=DEV)
-    pre = torch.full((m * n + 64,), 7.0, dtype=dtype, device=DEV)
+    saved = m * ((n + 7) // 8 * 8)
+    pre = torch.full((saved + 64,), 7.0, dtype=dtype, device=DEV)
     need = L.lce_linear_forward_workspace_bytes(x.data_ptr(), k, w.data_ptr(), k, m, n, k, code, 0)
     ws = torch.full((need + 512,), 90, dtype=torch.uint8, device=DEV)
     s = torch.cuda.current_stream().cuda_stream
@@ -279,7 +280,7 @@ def test_outputs_stay_inside_their_buffers(m, k, n, ldo, dtype):
                                     pre.data_ptr(), m, n, k, 4, code, ws.data_ptr(), need, 0, s), "lce_linear_forward")
     torch.cuda.synchronize()
     assert torch.equal(out[:m, :n], helion_b200.linear(x, w, b, activation="silu", residual=r))
-    assert bool((out[m:] == 7.0).all()) and bool((out[:, n:] == 7.0).all()) and bool((pre[m * n:] == 7.0).all())
+    assert bool((out[m:] == 7.0).all()) and bool((out[:, n:] == 7.0).all()) and bool((pre[saved:] == 7.0).all())
     assert bool((ws[need:] == 90).all())
     grads = [torch.full((size + 64,), 7.0, dtype=dtype, device=DEV) for size in (m * k, n * k, n)]
     args = (dy.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), k)
