@@ -125,7 +125,9 @@ int launch_tc_cg(const DeviceInfo& d, const Mat& a, const Mat& b, long long M, l
     // about 32 MB of them (the two L2 partitions of 63 MB each also hold the streaming operand).
     const long long kBandBytes = static_cast<long long>(g_tuning.band_mb.load(std::memory_order_relaxed)) << 20;
     const int kHintMode = g_tuning.hint_mode.load(std::memory_order_relaxed);
-    constexpr int kStages = CG == 2 ? kStages2 : kStages1;
+    constexpr int kEpiWarps = EpiWarps<Epi, CG>::value;
+    constexpr int kStages = kEpiWarps == 8 ? kStages2 - 1 : (CG == 2 ? kStages2 : kStages1);  // the warps' areas take a stage
+    static_assert(kEpiWarps == 4 || CG == 2, "eight epilogue warps beside CTA pairs only");
     const int dtype = IS_BF16 ? LCE_DTYPE_BF16 : LCE_DTYPE_F16;
     CUtensorMap tma, tmb;
     int rc;
@@ -143,7 +145,7 @@ int launch_tc_cg(const DeviceInfo& d, const Mat& a, const Mat& b, long long M, l
     // every k slice must hold at least one block
     if (k_splits < 1 || (k_splits - 1) * cdiv(k_blocks, k_splits) >= k_blocks) return LCE_ERR_ARG;
     auto kern = gemm_tc_kernel<kBN, kStages, CG, A_MN, B_MN, IS_BF16, Epi>;
-    constexpr int smem = GemmSmem<kBN, kStages, CG>::kTotalBytes;
+    constexpr int smem = GemmSmem<kBN, kStages, CG, kEpiWarps>::kTotalBytes;
     // per kernel instantiation and device; setting the attribute twice from two threads is harmless
     static std::atomic<bool> smem_opted_in[kMaxDevices];
     if (!smem_opted_in[d.index].load(std::memory_order_acquire)) {
@@ -156,7 +158,7 @@ int launch_tc_cg(const DeviceInfo& d, const Mat& a, const Mat& b, long long M, l
     const int grid = static_cast<int>(work < slots ? work : slots) * CG;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kGemmThreads);
+    cfg.blockDim = dim3(64 + 32 * kEpiWarps);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     // The kernel waits for its predecessor in the stream itself (ptx::grid_dep_wait after its set-up), so it may

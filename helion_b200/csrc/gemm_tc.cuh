@@ -12,7 +12,7 @@
 // CTA layout (192 threads):
 //   warp 0      TMA producer   (one elected lane)
 //   warp 1      tensor-memory allocator + tcgen05.mma issuer (one elected lane)
-//   warps 2-5   epilogue; warp w owns TMEM lanes 32*(w%4) .. 32*(w%4)+31
+//   warps 2-5   epilogue; warp w owns TMEM lanes 32*(w%4) .. 32*(w%4)+31 (warps 2-9 for some epilogues: EpiWarps)
 // Pipelines: STAGES-deep smem ring (full/empty mbarriers) between producer and issuer, and two
 // accumulator buffers in TMEM (tmem_full/tmem_empty) so the epilogue of tile i overlaps the main
 // loop of tile i+1. Tiles are dealt to a persistent grid either round-robin (static) or, for launches of
@@ -53,7 +53,14 @@ namespace lce {
 constexpr int kBM = 128;      // accumulator tile rows per CTA (= TMEM lanes)
 constexpr int kBK = 64;       // k elements per pipeline stage (= one 128-byte swizzle row)
 constexpr int kUmmaK = 16;    // k elements per tcgen05.mma for 16-bit operands
-constexpr int kGemmThreads = 192;
+constexpr int kGemmThreads = 192;  // with four epilogue warps
+
+// Epilogue warps of a CTA: 4, or 8 for an epilogue that would not keep up otherwise (each half of them then takes half of
+// a tile's columns; warp w owns TMEM lanes 32*(w%4) .. either way). Specialised beside such an epilogue.
+template <class Epi, int CG>
+struct EpiWarps {
+    static constexpr int value = 4;
+};
 
 // error codes written to the device status word
 constexpr int kDevErrProducerTimeout = 101;
@@ -70,19 +77,20 @@ struct TileCtx {
     int bn;           // tile width in columns
     int k_slice;      // which slice of the contraction this tile holds (0 unless K is split)
     float* stage;     // this warp's 32 x 33 floats of shared memory for re-shaping a chunk (256 more follow), or nullptr
+    int col_begin = 0, col_end = 0;  // the columns of the tile that this warp handles (tensor-core path)
 };
 
 constexpr int kStageBiasOffset = 32 * 33;  // behind the re-shaping area: 256 floats for a tile's slice of a bias
 constexpr int kStageFloatsPerWarp = kStageBiasOffset + 256;
 
-template <int BN, int STAGES, int CG>
+template <int BN, int STAGES, int CG, int EPI_WARPS = 4>
 struct GemmSmem {
     static constexpr int kABytes = kBM * kBK * 2;
     static constexpr int kBRows = BN / CG;  // B rows (n indices) this CTA stages
     static constexpr int kBBytes = kBRows * kBK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
     static constexpr int kBarrierBytes = 256;
-    static constexpr int kEpiStageBytes = 4 * kStageFloatsPerWarp * 4;  // one re-shaping area per epilogue warp
+    static constexpr int kEpiStageBytes = EPI_WARPS * kStageFloatsPerWarp * 4;  // one re-shaping area per epilogue warp
     // 1024 bytes of slack so the ring can be aligned to the swizzle atom by hand
     static constexpr int kTotalBytes = STAGES * kStageBytes + kBarrierBytes + kEpiStageBytes + 1024;
 };
@@ -139,12 +147,14 @@ struct SecondGemm {
 };
 
 template <int BN, int STAGES, int CG, bool A_MN, bool B_MN, bool IS_BF16, class Epi, class Second = NoSecondGemm>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(64 + 32 * EpiWarps<Epi, CG>::value, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                int m_tiles, int n_tiles, int k_blocks, int k_splits, int raster, int l2_hints,
                const typename Epi::Params ep, int* __restrict__ status, int* __restrict__ sched_counter,
                unsigned* __restrict__ done_counter, const __grid_constant__ Second second = Second{}) {
-    using S = GemmSmem<BN, STAGES, CG>;
+    constexpr int kEpiWarps = EpiWarps<Epi, CG>::value;
+    using S = GemmSmem<BN, STAGES, CG, kEpiWarps>;
+    static_assert(kEpiWarps == 4 || (kEpiWarps == 8 && BN % 128 == 0), "epilogue warps");
     static_assert(CG == 1 || CG == 2, "cta group");
     static_assert(BN % (64 * CG) == 0 && BN >= 64 && BN <= 256, "tile width");
     static_assert(2 * BN <= 512, "two accumulator buffers must fit in tensor memory");
@@ -216,13 +226,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
         for (int b = 0; b < 2; ++b) {
             ptx::mbar_init(tfull_bar(b), 1);
-            ptx::mbar_init(tempty_bar(b), 4 * CG);  // one arrival per epilogue warp of the group
+            ptx::mbar_init(tempty_bar(b), kEpiWarps * CG);  // one arrival per epilogue warp of the group
         }
         ptx::mbar_init(drain_bar, 1);
         for (int q = 0; q < kSchedSlots; ++q) {
             ptx::mbar_init(sfull_bar(q), 1);  // the leader's producer publishes
             // readers of a slot: MMA issuer, the epilogue warps of the group, the peer's producer
-            ptx::mbar_init(sempty_bar(q), 1 + 4 * CG + (CG - 1));
+            ptx::mbar_init(sempty_bar(q), 1 + kEpiWarps * CG + (CG - 1));
         }
         *abort_flag = 0;
         ptx::fence_mbar_init();
@@ -447,6 +457,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
     } else {
         // ------------------------------------------------------------------ epilogue warps
         const int quarter = warp & 3;
+        constexpr int kCols = BN / (kEpiWarps / 4);  // columns this warp handles, from col_begin
+        const int col_begin = (warp - 2) / 4 * kCols;
         uint32_t local_tile = 0;
         bool ok = true;
         typename Epi::State st;
@@ -458,7 +470,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             const uint32_t buf = local_tile & 1u;
             const uint32_t buf_phase = (local_tile >> 1) & 1u;
             TileCtx tc{m_tile, n_tile, it.n_tiles, quarter * 32 + lane, BN, it.w / it.total_units,
-                       reinterpret_cast<float*>(gen_bar_base + S::kBarrierBytes) + (warp - 2) * kStageFloatsPerWarp};
+                       reinterpret_cast<float*>(gen_bar_base + S::kBarrierBytes) + (warp - 2) * kStageFloatsPerWarp,
+                       col_begin, col_begin + kCols};
             const typename Epi::Params* epp = &ep;  // this product's epilogue parameters
             if constexpr (kDual) {
                 if (it.sec) epp = &second.ep;
@@ -471,17 +484,31 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             ptx::tc_fence_after_sync();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BN;
             // two chunks in flight: the tensor-memory read of the next chunk runs under the work on this one
-            static_assert((BN / 32) % 2 == 0, "chunks are taken in pairs");
-            float va[32], vb[32];
-            ptx::tmem_ld_32x32(taddr, va);
+            static_assert((kCols / 32) % 2 == 0, "chunks are taken in pairs");
+            if constexpr (kEpiWarps == 4) {
+                float va[32], vb[32];
+                ptx::tmem_ld_32x32(taddr + col_begin, va);
 #pragma unroll 1
-            for (int c = 0; c < BN / 32; c += 2) {
-                ptx::tmem_ld_wait();
-                ptx::tmem_ld_32x32(taddr + (c + 1) * 32, vb);
-                Epi::chunk(st, *epp, tc, c * 32, va);
-                ptx::tmem_ld_wait();
-                if (c + 2 < BN / 32) ptx::tmem_ld_32x32(taddr + (c + 2) * 32, va);
-                Epi::chunk(st, *epp, tc, (c + 1) * 32, vb);
+                for (int c = col_begin / 32; c < (col_begin + kCols) / 32; c += 2) {
+                    ptx::tmem_ld_wait();
+                    ptx::tmem_ld_32x32(taddr + (c + 1) * 32, vb);
+                    Epi::chunk(st, *epp, tc, c * 32, va);
+                    ptx::tmem_ld_wait();
+                    if (c + 2 < (col_begin + kCols) / 32) ptx::tmem_ld_32x32(taddr + (c + 2) * 32, va);
+                    Epi::chunk(st, *epp, tc, (c + 1) * 32, vb);
+                }
+            } else {
+                // a scheduler's other epilogue warp works meanwhile; the registers are worth more to the epilogue
+#pragma unroll 1
+                for (int c = col_begin; c < col_begin + kCols; c += 64) {
+                    float v[32];
+                    ptx::tmem_ld_32x32(taddr + c, v);
+                    ptx::tmem_ld_wait();
+                    Epi::chunk(st, *epp, tc, c, v);
+                    ptx::tmem_ld_32x32(taddr + c + 32, v);
+                    ptx::tmem_ld_wait();
+                    Epi::chunk(st, *epp, tc, c + 32, v);
+                }
             }
             // all TMEM reads of this buffer are done: hand it back to the MMA issuer
             ptx::tc_fence_before_sync();

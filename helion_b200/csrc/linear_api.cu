@@ -10,7 +10,7 @@ namespace {
 // The row pitch of what a forward saves for its backward: whole 16-byte vectors whatever the type.
 inline long long pre_pitch(long long N) { return cdiv(N, 8) * 8; }
 
-constexpr long long kDzCtas = 592;  // CTAs that the column sums of the backward aim for (4 per SM on 148 SMs)
+constexpr long long kDzCtas = 444;  // CTAs that the column sums of the backward aim for (3 per SM on 148 SMs, one wave)
 
 // Scratch of one product C[M, N] = A[M, K] B[N, K]^T: slabs of a split contraction.
 struct ProductPlan {
@@ -63,33 +63,61 @@ int place_operand(Operand& o, char*& ws, cudaStream_t s) {
     return cuda_failed(cudaGetLastError()) ? LCE_ERR_CUDA : LCE_OK;
 }
 
-// C = act(A B^T + bias) + residual; an operand is K-major ([mn, K] rows) or MN-major ([K, mn] rows).
-template <class T, bool A_MN, bool B_MN>
-int product(const DeviceInfo& d, const ProductPlan& p, const Operand& a, const Operand& b, long long M, long long N,
-            long long K, const LinearTail<T>& tail, void* scratch, cudaStream_t s) {
-    using Epi = EpiLinear<T>;
+template <class Epi, class T>
+typename Epi::Params epilogue_params(const ProductPlan& p, const LinearTail<T>& tail, void* scratch) {
     typename Epi::Params ep;
     ep.t = tail;
     ep.scratch = p.splits > 1 ? static_cast<float*>(scratch) : nullptr;
     ep.slab_floats = p.slab_floats;
     ep.wide_out = wide_stores(tail.out, tail.ldo);
     ep.wide_residual = wide_stores(tail.residual, tail.ldr);
+    return ep;
+}
+
+template <class T, bool A_MN, bool B_MN, int ACT, bool HEAVY>
+int product_tc(const DeviceInfo& d, const ProductPlan& p, const Mat& a, const Mat& b, long long M, long long N, long long K,
+               const LinearTail<T>& tail, void* scratch, cudaStream_t s) {
+    using Epi = EpiLinear<T, ACT, HEAVY>;
+    // tiles that run together share a B panel when there are many row tiles, an A panel otherwise
+    const int m_fastest = cdiv(M, kBM) >= cdiv(N, kBN) ? 1 : 0;
+    return launch_tc<A_MN, B_MN, std::is_same<T, __nv_bfloat16>::value, Epi>(d, p.cg, a, b, M, N, K, m_fastest,
+                                                                            epilogue_params<Epi>(p, tail, scratch), s, p.splits);
+}
+
+// C = act(A B^T + bias) + residual; an operand is K-major ([mn, K] rows) or MN-major ([K, mn] rows). Only K-major operands
+// come with an activation, a residual or saved values (the forward).
+template <class T, bool A_MN, bool B_MN>
+int product(const DeviceInfo& d, const ProductPlan& p, const Operand& a, const Operand& b, long long M, long long N,
+            long long K, const LinearTail<T>& tail, void* scratch, cudaStream_t s) {
     const Mat am{a.ptr, a.rows, a.cols, a.ld}, bm{b.ptr, b.rows, b.cols, b.ld};
     int rc = LCE_ERR_ARG;
     if (p.use_tc) {
         if constexpr (sizeof(T) == 2) {
-            constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-            // tiles that run together share a B panel when there are many row tiles, an A panel otherwise
-            const int m_fastest = cdiv(M, kBM) >= cdiv(N, kBN) ? 1 : 0;
-            rc = launch_tc<A_MN, B_MN, kBf16, Epi>(d, p.cg, am, bm, M, N, K, m_fastest, ep, s, p.splits);
+            // a split contraction leaves as plain sums; linear_reduce_kernel finishes them
+            const bool light = (tail.act == kActNone && tail.residual == nullptr) || p.splits > 1;
+            if constexpr (A_MN || B_MN) {
+                rc = product_tc<T, A_MN, B_MN, kActNone, false>(d, p, am, bm, M, N, K, tail, scratch, s);
+            } else if (light) {
+                rc = product_tc<T, false, false, kActNone, false>(d, p, am, bm, M, N, K, tail, scratch, s);
+            } else {
+                switch (tail.act) {
+                    case kActNone: rc = product_tc<T, false, false, kActNone, true>(d, p, am, bm, M, N, K, tail, scratch, s); break;
+                    case kActRelu: rc = product_tc<T, false, false, kActRelu, true>(d, p, am, bm, M, N, K, tail, scratch, s); break;
+                    case kActGelu: rc = product_tc<T, false, false, kActGelu, true>(d, p, am, bm, M, N, K, tail, scratch, s); break;
+                    case kActGeluTanh: rc = product_tc<T, false, false, kActGeluTanh, true>(d, p, am, bm, M, N, K, tail, scratch, s); break;
+                    case kActSilu: rc = product_tc<T, false, false, kActSilu, true>(d, p, am, bm, M, N, K, tail, scratch, s); break;
+                    default: break;
+                }
+            }
         }
     } else {
-        rc = launch_simt<T, Epi>(d, am, A_MN, bm, B_MN, M, N, K, ep, s, p.splits);
+        using Epi = EpiLinear<T, kActAny, false>;
+        rc = launch_simt<T, Epi>(d, am, A_MN, bm, B_MN, M, N, K, epilogue_params<Epi>(p, tail, scratch), s, p.splits);
     }
     if (rc == LCE_OK && p.splits > 1) {
         const long long quads = cdiv(N, 4) * M;
         const int blocks = static_cast<int>(cdiv(quads, 256) < 4096 ? cdiv(quads, 256) : 4096);
-        const cudaError_t err = launch_dependent(linear_reduce_kernel<T>, blocks, 256, s, static_cast<const float*>(ep.scratch),
+        const cudaError_t err = launch_dependent(linear_reduce_kernel<T>, blocks, 256, s, static_cast<const float*>(scratch),
                                                  p.splits, p.slab_floats, static_cast<int>(cdiv(N, p.bn)), p.bn, tail);
         LCE_COUNT_LAUNCH();
         if (cuda_failed(err)) rc = LCE_ERR_CUDA;
@@ -145,6 +173,14 @@ BackwardPlan plan_linear_backward(const void* dy, long long ldy, const void* x, 
     return b;
 }
 
+template <class T, int ACT>
+void launch_dz(const BackwardPlan& b, const void* dy, long long ldy, const void* pre, T* dz, float* sums, long long M, long long N,
+               cudaStream_t s) {
+    const dim3 grid(static_cast<unsigned>(cdiv(N, 32 * (16 / sizeof(T)))), static_cast<unsigned>(b.slabs));
+    linear_dz_kernel<T, ACT><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), ldy, static_cast<const T*>(pre), pre_pitch(N),
+                                                  b.copy_dz ? dz : nullptr, b.ldz, sums, M, static_cast<int>(N), b.rows_per_slab);
+}
+
 template <class T>
 int linear_backward_impl(const DeviceInfo& d, BackwardPlan& b, const void* dy, long long ldy, const void* pre, void* dx, void* dw,
                          void* dbias, long long M, long long N, long long K, int act, char* ws, cudaStream_t s) {
@@ -157,11 +193,13 @@ int linear_backward_impl(const DeviceInfo& d, BackwardPlan& b, const void* dy, l
     ws += b.sums_bytes;
     const bool products = dx || dw;
     if (dbias || (products && b.copy_dz)) {
-        constexpr int VEC = 16 / sizeof(T);
-        const dim3 grid(static_cast<unsigned>(cdiv(N, 32 * VEC)), static_cast<unsigned>(b.slabs));
-        linear_dz_kernel<T, VEC><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), ldy, static_cast<const T*>(pre), pre_pitch(N),
-                                                      b.copy_dz ? dz : nullptr, b.ldz, dbias ? sums : nullptr, M,
-                                                      static_cast<int>(N), b.rows_per_slab, act);
+        switch (act) {
+            case kActRelu: launch_dz<T, kActRelu>(b, dy, ldy, pre, dz, dbias ? sums : nullptr, M, N, s); break;
+            case kActGelu: launch_dz<T, kActGelu>(b, dy, ldy, pre, dz, dbias ? sums : nullptr, M, N, s); break;
+            case kActGeluTanh: launch_dz<T, kActGeluTanh>(b, dy, ldy, pre, dz, dbias ? sums : nullptr, M, N, s); break;
+            case kActSilu: launch_dz<T, kActSilu>(b, dy, ldy, pre, dz, dbias ? sums : nullptr, M, N, s); break;
+            default: launch_dz<T, kActNone>(b, dy, ldy, pre, dz, dbias ? sums : nullptr, M, N, s); break;
+        }
         LCE_COUNT_LAUNCH();
         if (cuda_failed(cudaGetLastError())) return LCE_ERR_CUDA;
         if (dbias) {

@@ -16,66 +16,128 @@ namespace lce {
 
 enum LinearAct { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
 
-// sigmoid(t) = r for t >= 0 and e r below, with e = exp(-|t|) and r = 1 / (1 + e) in [1/2, 1]: nothing overflows, and
-// sigmoid(-t) is as exact as sigmoid(t). e is the square of exp(-|t| / 2) so that a product with it keeps results that
-// e itself would flush to zero. FAST: the hardware's base-2 exponential and reciprocal (relative error ~1e-6, for
-// results of 16 bits).
-template <bool FAST>
-struct Sigmoid {
-    float h, r;
-    bool positive;
-    __device__ __forceinline__ explicit Sigmoid(float t) {
-        positive = t >= 0.f;
-        h = FAST ? ptx::ex2(-0.5f * kLog2e * fabsf(t)) : expf(-0.5f * fabsf(t));
-        r = FAST ? __fdividef(1.f, fmaf(h, h, 1.f)) : 1.f / fmaf(h, h, 1.f);
-    }
-    __device__ __forceinline__ float times(float z) const { return (positive ? z : z * h * h) * r; }  // z sigmoid(t)
-    __device__ __forceinline__ float other() const { return (positive ? h * h : 1.f) * r; }           // 1 - sigmoid(t)
-};
 constexpr float kGeluC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 
-// The normal distribution function: Phi(-a) = exp(-a^2 / 2) g(a) for a >= 0, Phi(a) = 1 - Phi(-a). g falls smoothly from
-// 1/2; for 16-bit results it is a polynomial in 1 / (1 + 0.26 a), fitted here by reweighted least squares to 3.4e-7 of
-// its value for a up to 14 (with the 32-bit exponential 2e-6 up to a = 6). CUDA's normcdff would cost three times the
-// instructions, and the epilogue has to keep up with the tensor cores.
-struct NormalFast {
-    float h, g;  // exp(-a^2 / 4), g(a)
-    bool positive;
-    __device__ __forceinline__ explicit NormalFast(float z) {
-        const float a = fabsf(z), t = __fdividef(1.f, fmaf(0.26f, a, 1.f));
-        positive = z >= 0.f;
-        h = ptx::ex2(-0.36067376f * (a * a));
-        float p = fmaf(-0.07724009f, t, 0.24633712f);
-        p = fmaf(p, t, -0.135466f);
-        p = fmaf(p, t, 0.19220619f);
-        p = fmaf(p, t, 0.06021739f);
-        p = fmaf(p, t, 0.11097057f);
-        p = fmaf(p, t, 0.10293892f);
-        g = fmaf(p, t, 3.572605e-05f);
-    }
-    __device__ __forceinline__ float times(float z) const {  // z Phi(z)
-        const float tail = (z * h) * (h * g);
-        return positive ? z - tail : tail;
-    }
-    __device__ __forceinline__ float density() const { return 0.3989422804014327f * (h * h); }
+// ---- activations ----------------------------------------------------------------------------------
+// All three smooth ones are z times a distribution function F with F(-a) = 1 - F(a), so that with a = |z|
+//   act(z)  = max(z, 0) - a F(-a)            nothing overflows, and small results of negative z keep their digits
+//   act'(z) = [z >= 0] - sign(z) (F(-a) - a f(a))      f the density
+// silu: F the logistic function of z; gelu_tanh: the logistic function of u(z) = 2 sqrt(2/pi) (z + 0.044715 z^3); gelu:
+// the normal distribution. exp(-x) enters as the square of exp(-x / 2), so that a product with it keeps results that the
+// exponential itself would flush to zero.
+//
+// For 16-bit results (FAST) the exponential and the reciprocal are the hardware's, 1e-6 relative, and two elements share
+// an instruction where the hardware has it (fma, mul and add of fp32 pairs): at a contraction of 1024 a tile's epilogue
+// has to be done in 8000 cycles of its four schedulers. The normal distribution is
+//   F(-a) = exp(-a^2 / 2) g(a),  g a polynomial in 1 / (1 + 0.26 a)
+// fitted here by reweighted least squares to 3.4e-7 of g for a up to 14 (with the exponential 2e-6 up to a = 6).
+struct Pair {
+    unsigned long long v;
 };
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+__device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v)); }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ Pair reciprocal2(Pair x) {
+    float a, b;
+    split(x, a, b);
+    return pair(fast_reciprocal(a), fast_reciprocal(b));
+}
+__device__ __forceinline__ Pair exp2_2(Pair x) {
+    float a, b;
+    split(x, a, b);
+    return pair(ptx::ex2(a), ptx::ex2(b));
+}
+// -|z|, an infinity as the largest finite value (whose weight is 0 all the same) and a NaN as it is.
+__device__ __forceinline__ float minus_abs(float z) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(-fabsf(z)), "f"(-3.402823466e38f));
+    return y;
+}
 
-// act(z) of N values at a time; `act` is the same for the whole launch.
-template <bool FAST, int N>
-__device__ __forceinline__ void linear_act(float (&z)[N], int act) {
-    if (act == kActRelu) {
+// h = exp(-x / 2) and q with F(-a) = h h q, for a pair of -a.
+template <int ACT>
+__device__ __forceinline__ void distribution2(Pair na, Pair& h, Pair& q) {
+    if constexpr (ACT == kActGelu) {
+        const Pair t = reciprocal2(fma2(na, both(-0.26f), both(1.f)));
+        h = exp2_2((na * both(-0.36067376f)) * na);
+        Pair p = fma2(both(-0.07724009f), t, both(0.24633712f));
+        p = fma2(p, t, both(-0.135466f));
+        p = fma2(p, t, both(0.19220619f));
+        p = fma2(p, t, both(0.06021739f));
+        p = fma2(p, t, both(0.11097057f));
+        p = fma2(p, t, both(0.10293892f));
+        q = fma2(p, t, both(3.572605e-05f));
+    } else {
+        Pair x = na;  // -x
+        if constexpr (ACT == kActGeluTanh) x = na * fma2(na * both(2.f * kGeluC * kGeluA), na, both(2.f * kGeluC));
+        h = exp2_2(x * both(0.5f * kLog2e));
+        q = reciprocal2(fma2(h, h, both(1.f)));
+    }
+}
+// The same for one value of a logistic one in full 32-bit accuracy.
+template <int ACT>
+__device__ __forceinline__ void distribution(float a, float& h, float& q) {
+    static_assert(ACT == kActGeluTanh || ACT == kActSilu, "gelu goes by normcdff");
+    const float x = ACT == kActGeluTanh ? 2.f * kGeluC * a * fmaf(kGeluA * a, a, 1.f) : a;
+    h = expf(-0.5f * x);
+    q = 1.f / fmaf(h, h, 1.f);
+}
+
+// act(z) of N values.
+template <bool FAST, int ACT, int N>
+__device__ __forceinline__ void linear_act(float (&z)[N]) {
+    if constexpr (ACT == kActRelu) {
 #pragma unroll
         for (int j = 0; j < N; ++j) z[j] = z[j] <= 0.f ? 0.f : z[j];  // a NaN stays one
-    } else if (act == kActGelu) {
+    } else if constexpr (ACT != kActNone && FAST) {
+        static_assert(N % 2 == 0, "pairs");
 #pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = FAST ? NormalFast(z[j]).times(z[j]) : z[j] * normcdff(z[j]);
-    } else if (act == kActGeluTanh) {  // (1 + tanh(u)) / 2 = sigmoid(2u)
+        for (int j = 0; j < N; j += 2) {
+            const Pair na = pair(minus_abs(z[j]), minus_abs(z[j + 1]));
+            Pair h, q;
+            distribution2<ACT>(na, h, q);
+            split(fma2(na * h, h * q, pair(fmaxf(z[j], 0.f), fmaxf(z[j + 1], 0.f))), z[j], z[j + 1]);
+        }
+    } else if constexpr (ACT == kActGelu) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = Sigmoid<FAST>(2.f * kGeluC * z[j] * fmaf(kGeluA * z[j], z[j], 1.f)).times(z[j]);
-    } else if (act == kActSilu) {
+        for (int j = 0; j < N; ++j) z[j] = z[j] * normcdff(z[j]);
+    } else if constexpr (ACT != kActNone) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = Sigmoid<FAST>(z[j]).times(z[j]);
+        for (int j = 0; j < N; ++j) {
+            float h, q;
+            distribution<ACT>(fabsf(z[j]), h, q);
+            z[j] = (z[j] >= 0.f ? z[j] : z[j] * h * h) * q;
+        }
+    }
+}
+template <bool FAST, int N>
+__device__ __forceinline__ void linear_act(float (&z)[N], int act) {
+    switch (act) {
+        case kActRelu: linear_act<FAST, kActRelu>(z); break;
+        case kActGelu: linear_act<FAST, kActGelu>(z); break;
+        case kActGeluTanh: linear_act<FAST, kActGeluTanh>(z); break;
+        case kActSilu: linear_act<FAST, kActSilu>(z); break;
+        default: break;
     }
 }
 
@@ -86,36 +148,43 @@ __device__ __forceinline__ void linear_saved(const float (&z)[N], int act, float
     for (int j = 0; j < N; ++j) saved[j] = act == kActRelu ? (z[j] > 0.f ? 1.f : 0.f) : z[j];
 }
 
-// g *= act'(.) from what the forward saved.
-template <bool FAST, int N>
-__device__ __forceinline__ void linear_slope(float (&g)[N], const float (&pre)[N], int act) {
-    if (act == kActRelu) {
+// g *= act'(.) from what the forward saved. a f(a) is 0.3989 a h h for the normal distribution and x' F(-a) F(a) for the
+// logistic ones (x' = a for silu; for gelu_tanh a du/da, which may overflow against a zero far out).
+template <bool FAST, int ACT, int N>
+__device__ __forceinline__ void linear_slope(float (&g)[N], const float (&pre)[N]) {
+    if constexpr (ACT == kActRelu) {
 #pragma unroll
         for (int j = 0; j < N; ++j) g[j] *= pre[j];
-    } else if (act == kActGelu) {
+    } else if constexpr (ACT == kActGelu && FAST) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const Pair na = pair(minus_abs(pre[j]), minus_abs(pre[j + 1]));
+            Pair h, q;
+            distribution2<ACT>(na, h, q);
+            float d[2];  // F(-a) - a f(a)
+            split((h * h) * fma2(na, both(0.3989422804014327f), q), d[0], d[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) g[j + i] *= pre[j + i] >= 0.f ? 1.f - d[i] : d[i];
+        }
+    } else if constexpr (ACT == kActGelu) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) g[j] *= fmaf(pre[j] * 0.3989422804014327f, expf(-0.5f * pre[j] * pre[j]), normcdff(pre[j]));
+    } else if constexpr (ACT != kActNone) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
+            const float a = fabsf(pre[j]);
+            float h, q;
             if constexpr (FAST) {
-                const NormalFast n(pre[j]);
-                g[j] *= fmaf(pre[j], n.density(), n.times(1.f));
+                const float x = ACT == kActGeluTanh ? 2.f * kGeluC * a * fmaf(kGeluA * a, a, 1.f) : a;
+                h = ptx::ex2(-0.5f * kLog2e * x);
+                q = fast_reciprocal(fmaf(h, h, 1.f));
             } else {
-                g[j] *= fmaf(pre[j] * 0.3989422804014327f, expf(-0.5f * pre[j] * pre[j]), normcdff(pre[j]));
+                distribution<ACT>(a, h, q);
             }
-        }
-    } else if (act == kActGeluTanh) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const Sigmoid<FAST> t(2.f * kGeluC * pre[j] * fmaf(kGeluA * pre[j], pre[j], 1.f));
-            const float s = t.times(1.f), both = s * t.other();
-            // far out the cubic may overflow against a zero
-            g[j] *= both == 0.f ? s : fmaf(2.f * kGeluC * pre[j] * fmaf(3.f * kGeluA * pre[j], pre[j], 1.f), both, s);
-        }
-    } else if (act == kActSilu) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const Sigmoid<FAST> t(pre[j]);
-            const float s = t.times(1.f), both = s * t.other();
-            g[j] *= both == 0.f ? s : fmaf(pre[j], both, s);
+            const float low = h * h * q;  // F(-a); F(a) = q
+            const float x1 = ACT == kActGeluTanh ? 2.f * kGeluC * a * fmaf(3.f * kGeluA * a, a, 1.f) : a;
+            const float d = low == 0.f ? 0.f : fmaf(-x1 * q, low, low);
+            g[j] *= pre[j] >= 0.f ? 1.f - d : d;
         }
     }
 }
@@ -248,7 +317,19 @@ __device__ __forceinline__ void pack32(const float (&v)[32], uint4 (&raw)[4]) {
     }
 }
 
-template <class T>
+// ACT: the activation, or kActAny to go by the call's (CUDA-core GEMM, split contractions). HEAVY: for calls with an
+// activation, a residual or saved values.
+constexpr int kActAny = -1;
+template <class T, int ACT, bool HEAVY>
+struct EpiLinear;
+// A heavy epilogue runs on eight warps beside CTA pairs: with four, 8192 x 1024 x 4096 with gelu took 129 us where eight
+// take 101 (the product alone 60); without any of it four warps and a sixth stage are faster (60 against 66 us).
+template <class T, int ACT>
+struct EpiWarps<EpiLinear<T, ACT, true>, 2> {
+    static constexpr int value = 8;
+};
+
+template <class T, int ACT, bool HEAVY>
 struct EpiLinear {
     static constexpr bool kHasFinish = false;
     struct Params {
@@ -261,19 +342,24 @@ struct EpiLinear {
     // leave when the second half is there.
     struct State {
         int row;
-        uint4 next[sizeof(T) == 2 ? 8 : 1];
-        uint4 saved[sizeof(T) == 2 ? 4 : 1];
+        uint4 next[sizeof(T) == 2 && HEAVY ? 8 : 1];
+        uint4 saved[sizeof(T) == 2 && HEAVY ? 4 : 1];
     };
+    template <int N>
+    static __device__ __forceinline__ void activate(float (&v)[N], int act) {
+        if constexpr (ACT == kActAny) linear_act<LinearTail<T>::kFast>(v, act);
+        else linear_act<LinearTail<T>::kFast, ACT>(v);
+    }
     static __device__ __forceinline__ void begin(State& st, const Params& p, const TileCtx& tc) {
         st.row = tc.m_tile * kBM + tc.row_in_tile;
         if constexpr (sizeof(T) == 2) {
             if (p.scratch != nullptr || tc.stage == nullptr) return;
             const LinearTail<T>& t = p.t;
-            const int lane = tc.row_in_tile & 31, col0 = tc.n_tile * tc.bn, row_base = st.row - lane;
-            if (t.bias != nullptr) {  // the tile's slice of the bias, as floats, behind the re-shaping area
+            const int lane = tc.row_in_tile & 31, col0 = tc.n_tile * tc.bn + tc.col_begin, row_base = st.row - lane;
+            if (t.bias != nullptr) {  // this warp's slice of the bias, as floats, behind the re-shaping area
                 float* bias = tc.stage + kStageBiasOffset;
                 __syncwarp();  // the previous tile's has been read
-                for (int c = lane * 8; c < tc.bn; c += 256) {
+                for (int c = lane * 8; c < tc.col_end - tc.col_begin; c += 256) {
                     float b[8];
                     load_row<T>(t.bias + col0 + c, b, t.cols - col0 - c);
                     *reinterpret_cast<float4*>(bias + c) = make_float4(b[0], b[1], b[2], b[3]);
@@ -281,8 +367,9 @@ struct EpiLinear {
                 }
                 __syncwarp();
             }
-            if (t.residual != nullptr && p.wide_residual)
-                lines_fetch<T>(lane, t.residual + static_cast<long long>(row_base) * t.ldr + col0, t.ldr, t.rows - row_base, t.cols - col0, st.next);
+            if constexpr (HEAVY)
+                if (t.residual != nullptr && p.wide_residual)
+                    lines_fetch<T>(lane, t.residual + static_cast<long long>(row_base) * t.ldr + col0, t.ldr, t.rows - row_base, t.cols - col0, st.next);
         }
     }
     static __device__ __forceinline__ void chunk(State& st, const Params& p, const TileCtx& tc, int col0, float (&v)[32]) {
@@ -315,7 +402,7 @@ struct EpiLinear {
             linear_saved(v, t.act, saved);
             store_row32<T>(t.pre + static_cast<long long>(st.row) * t.ldp + gcol0, saved, valid);
         }
-        linear_act<LinearTail<T>::kFast>(v, t.act);
+        activate(v, t.act);
         if (t.residual != nullptr) {
             float r[32];
             load_row<T>(t.residual + static_cast<long long>(st.row) * t.ldr + gcol0, r, valid);
@@ -331,7 +418,7 @@ struct EpiLinear {
         const int row_base = st.row - lane, blk0 = gcol0 - half * 32;
         const int rows = t.rows - row_base, cols = t.cols - blk0;  // of the 64-column block
         if (t.bias != nullptr) {
-            const float4* b = reinterpret_cast<const float4*>(tc.stage + kStageBiasOffset + col0);
+            const float4* b = reinterpret_cast<const float4*>(tc.stage + kStageBiasOffset + col0 - tc.col_begin);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float4 x = b[i];
@@ -341,54 +428,64 @@ struct EpiLinear {
                 v[4 * i + 3] += x.w;
             }
         }
-        uint4 keep[4];
-        if (t.pre != nullptr) {
-            float saved[32];
-            linear_saved(v, t.act, saved);
-            pack32<T>(saved, keep);
-        }
-        linear_act<true>(v, t.act);
-        if (t.residual != nullptr) {
-            if (half == 0) {
-                const T* src = t.residual + static_cast<long long>(row_base) * t.ldr + blk0;
-                if (p.wide_residual) {
-                    lines_put(tc.stage, lane, st.next);
-                    if (col0 + 64 < tc.bn) lines_fetch<T>(lane, src + 64, t.ldr, rows, cols - 64, st.next);
-                } else {
-                    lines_to_area<T>(tc.stage, lane, src, t.ldr, rows, cols);
-                }
-                __syncwarp();
-            }
-            uint4 r[4];
-            area_get(tc.stage, lane, half, r);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float e[8];
-                rms_unpack<T>(r[i], e);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[i * 8 + j] += e[j];
-            }
-        }
         uint4 y[4];
-        pack32<T>(v, y);
-        area_put(tc.stage, lane, half, y);
-        if (half == 0) {
+        if constexpr (!HEAVY) {
+            pack32<T>(v, y);
+            area_put(tc.stage, lane, half, y);
+            if (half == 0) return;
+        } else {
+            uint4 keep[4];
             if (t.pre != nullptr) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st.saved[i] = keep[i];
+                float saved[32];
+                linear_saved(v, t.act, saved);
+                pack32<T>(saved, keep);
             }
-            return;
+            activate(v, t.act);
+            if (t.residual != nullptr) {
+                if (half == 0) {
+                    const T* src = t.residual + static_cast<long long>(row_base) * t.ldr + blk0;
+                    if (p.wide_residual) {
+                        lines_put(tc.stage, lane, st.next);
+                        if (col0 + 64 < tc.col_end) lines_fetch<T>(lane, src + 64, t.ldr, rows, cols - 64, st.next);
+                    } else {
+                        lines_to_area<T>(tc.stage, lane, src, t.ldr, rows, cols);
+                    }
+                    __syncwarp();
+                }
+                uint4 r[4];
+                area_get(tc.stage, lane, half, r);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float e[8];
+                    rms_unpack<T>(r[i], e);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i * 8 + j] += e[j];
+                }
+            }
+            pack32<T>(v, y);
+            area_put(tc.stage, lane, half, y);
+            if (half == 0) {
+                if (t.pre != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st.saved[i] = keep[i];
+                }
+                return;
+            }
+            if (t.pre != nullptr) {
+                __syncwarp();
+                area_to_lines<T>(tc.stage, lane, t.out + static_cast<long long>(row_base) * t.ldo + blk0, t.ldo, rows, cols, p.wide_out != 0);
+                __syncwarp();
+                area_put(tc.stage, lane, 0, st.saved);
+                area_put(tc.stage, lane, 1, keep);
+                __syncwarp();
+                area_to_lines<T>(tc.stage, lane, t.pre + static_cast<long long>(row_base) * t.ldp + blk0, t.ldp, rows, cols, true);
+                __syncwarp();
+                return;
+            }
         }
         __syncwarp();
         area_to_lines<T>(tc.stage, lane, t.out + static_cast<long long>(row_base) * t.ldo + blk0, t.ldo, rows, cols, p.wide_out != 0);
         __syncwarp();
-        if (t.pre != nullptr) {
-            area_put(tc.stage, lane, 0, st.saved);
-            area_put(tc.stage, lane, 1, keep);
-            __syncwarp();
-            area_to_lines<T>(tc.stage, lane, t.pre + static_cast<long long>(row_base) * t.ldp + blk0, t.ldp, rows, cols, true);
-            __syncwarp();
-        }
     }
     static __device__ __forceinline__ void end(State&, const Params&, const TileCtx&) {}
 };
@@ -449,40 +546,55 @@ repitch_kernel(const T* __restrict__ src, long long lds, T* __restrict__ dst, lo
 
 // dz = dy * act'(pre), rounded, and the column sums of the unrounded dz over this CTA's rows.
 // A CTA of 256 threads owns 32 x VEC columns and the row slab [slab * rows_per_slab, ...): 32 column groups x 8 rows
-// at a time, two of them in flight. Bound by the bytes: dy and pre in, dz out. partial: [slabs][cols] (nullptr: no sums);
+// at a time, four of them in flight. Bound by the bytes: dy and pre in, dz out. partial: [slabs][cols] (nullptr: no sums);
 // dz nullptr: sums only (no activation, dz = dy). Columns of dz up to its pitch, behind the last, are set to zero.
-template <class T, int VEC>
-__global__ void __launch_bounds__(256)
+template <class T, int ACT>
+__global__ void __launch_bounds__(256, 3)
 linear_dz_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ pre, long long ldp, T* __restrict__ dz, long long ldz,
-                 float* __restrict__ partial, long long rows, int cols, long long rows_per_slab, int act) {
-    constexpr int U = 2;
+                 float* __restrict__ partial, long long rows, int cols, long long rows_per_slab) {
+    constexpr int U = 4, VEC = 16 / sizeof(T);
     __shared__ float sums[8][32 * VEC + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = (blockIdx.x * 32 + lane) * VEC;
     const long long row_begin = blockIdx.y * rows_per_slab, row_end = min(rows, row_begin + rows_per_slab);
     const int valid = cols - col;
+    const bool whole = valid >= VEC && ldy % VEC == 0 && (reinterpret_cast<uintptr_t>(dy) & 15u) == 0;
     float acc[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
     if (valid > 0) {
         for (long long row0 = row_begin + warp; row0 < row_end; row0 += 8 * U) {
-            float g[U][VEC], z[U][VEC];
+            uint4 rg[U], rz[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const long long row = row0 + 8 * u;
-                if (row < row_end) {
-                    load_row<T, VEC>(dy + row * ldy + col, g[u], valid);
-                    if (act != kActNone) load_row<T, VEC>(pre + row * ldp + col, z[u], valid);
+                rg[u] = rz[u] = make_uint4(0u, 0u, 0u, 0u);
+                if (row >= row_end) continue;
+                if (whole) {
+                    rg[u] = *reinterpret_cast<const uint4*>(dy + row * ldy + col);
+                } else {
+                    alignas(16) T e[VEC];
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) e[j] = j < valid ? dy[row * ldy + col + j] : Cvt<T>::from_f(0.f);
+                    rg[u] = *reinterpret_cast<const uint4*>(e);
                 }
+                if (ACT != kActNone) rz[u] = *reinterpret_cast<const uint4*>(pre + row * ldp + col);  // whole rows by its pitch
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const long long row = row0 + 8 * u;
-                if (row >= row_end) break;
-                linear_slope<LinearTail<T>::kFast>(g[u], z[u], act);
-                if (dz != nullptr) *reinterpret_cast<uint4*>(dz + row * ldz + col) = rms_pack<T>(g[u]);
+                if (row >= row_end) continue;
+                float g[VEC], z[VEC];
+                rms_unpack<T>(rg[u], g);
+                rms_unpack<T>(rz[u], z);
+                linear_slope<LinearTail<T>::kFast, ACT>(g, z);
+                if (valid < VEC) {  // what the saved rows hold behind their last column is anything
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[j] += g[u][j];
+                    for (int j = 0; j < VEC; ++j) g[j] = j < valid ? g[j] : 0.f;
+                }
+                if (dz != nullptr) *reinterpret_cast<uint4*>(dz + row * ldz + col) = rms_pack<T>(g);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] += g[j];
             }
         }
     }

@@ -221,7 +221,13 @@ def test_extreme_values():
             slope_err = 4e-6 + half * (0.8 * xd.detach().double().abs() * (act not in (None, "relu")) + ref[1].abs())
             slope_err = torch.where(xd.detach().abs() > 80, 1e-6, slope_err)
             _inside(dx, 8 * ref[1], half * 8 * ref[1].abs() + 8 * slope_err, f"{act} {dtype} slope")
-    for act in ACTS:  # a NaN stays in its row, an infinity in its column
+    inf = torch.tensor([[float("inf")], [3e38], [-3e38]], device=DEV)
+    for dtype in (torch.bfloat16, torch.float32):
+        for act in ACTS:
+            y = helion_b200.linear(inf.to(dtype), torch.ones(8, 1, device=DEV, dtype=dtype), activation=act)
+            assert bool((y[0] == float("inf")).all()) and bool((y[1] > 2.9e38).all())
+            assert act is None or bool((y[2] == 0).all())
+    for act in ACTS:  # a NaN stays in its row
         xb = torch.randn(40, 64, device=DEV).bfloat16()
         xb[7, 3] = float("nan")
         y = helion_b200.linear(xb, torch.randn(72, 64, device=DEV).bfloat16(), activation=act)
