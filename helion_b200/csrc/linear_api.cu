@@ -31,6 +31,12 @@ ProductPlan plan_product(long long M, long long N, long long K, int dtype, unsig
     return p;
 }
 
+// Few tokens take the decode kernel. It measured faster than the core's split contraction up to its 64 tokens.
+constexpr long long kDecodeTokens = 64;
+inline bool decodes(long long M, int dtype, unsigned flags) {
+    return dtype != LCE_DTYPE_F32 && !(flags & LCE_FLAG_FORCE_SIMT) && M <= kDecodeTokens;
+}
+
 // An operand [rows, cols] as the caller has it, and whether the kernels need it at another pitch (a copy in scratch).
 struct Operand {
     const void* ptr;
@@ -94,7 +100,7 @@ int product(const DeviceInfo& d, const ProductPlan& p, const Operand& a, const O
     if (p.use_tc) {
         if constexpr (sizeof(T) == 2) {
             // a split contraction leaves as plain sums; linear_reduce_kernel finishes them
-            const bool light = (tail.act == kActNone && tail.residual == nullptr) || p.splits > 1;
+            const bool light = (tail.act == kActNone && tail.residual == nullptr && tail.bias == nullptr) || p.splits > 1;
             if constexpr (A_MN || B_MN) {
                 rc = product_tc<T, A_MN, B_MN, kActNone, false>(d, p, am, bm, M, N, K, tail, scratch, s);
             } else if (light) {
@@ -130,13 +136,67 @@ bool linear_args_ok(long long M, long long N, long long K, long long ldx, long l
 }
 bool linear_too_large(long long M, long long N, long long K) { return M > 0x7fffff00ll || N > 0x7fffff00ll || K > 0x7fffff00ll; }
 
-size_t forward_bytes(const Operand& x, const Operand& w, const ProductPlan& p) { return x.copy_bytes + w.copy_bytes + p.bytes; }
+size_t forward_bytes(const Operand& x, const Operand& w, const ProductPlan& p, bool decode) {
+    return x.copy_bytes + w.copy_bytes + (decode ? 0 : p.bytes);
+}
+
+template <class T, int BN>
+int launch_decode(const DeviceInfo& d, const Operand& x, const Operand& w, long long N, long long K, const LinearTail<T>& tail, cudaStream_t s) {
+    const int dtype = std::is_same<T, __nv_bfloat16>::value ? LCE_DTYPE_BF16 : LCE_DTYPE_F16;
+    CUtensorMap tm_w, tm_x;
+    int rc;
+    if ((rc = make_tmap(&tm_w, w.ptr, dtype, K, N, w.ld * 2, kBK, kBM))) return rc;
+    if ((rc = make_tmap(&tm_x, x.ptr, dtype, K, x.rows, x.ld * 2, kBK, BN))) return rc;
+    // the contraction is cut until the CTAs fill the GPU twice over, as long as a CTA has two blocks of 64 to stream
+    const long long tiles = cdiv(N, kBM), k_blocks = cdiv(K, kBK);
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= 2 * d.sm_count && k_blocks >= 4 * splits) splits *= 2;
+    if (tiles * splits > 0x7fffffffll) return LCE_ERR_TOO_LARGE;
+    auto kern = linear_decode_kernel<T, BN>;
+    constexpr int smem = DecodeSmem<BN>::kTotalBytes;
+    static std::atomic<bool> opted_in[kMaxDevices];  // setting the attribute twice from two threads is harmless
+    if (!opted_in[d.index].load(std::memory_order_acquire)) {
+        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return LCE_ERR_CUDA;
+        opted_in[d.index].store(true, std::memory_order_release);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+    cfg.blockDim = dim3(kGemmThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    int n_attr = 0;
+    if (pdl_enabled()) {
+        attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n_attr].val.programmaticStreamSerializationAllowed = 1;
+        ++n_attr;
+    }
+    if (splits > 1) {
+        attr[n_attr].id = cudaLaunchAttributeClusterDimension;
+        attr[n_attr].val.clusterDim.x = splits;
+        attr[n_attr].val.clusterDim.y = 1;
+        attr[n_attr].val.clusterDim.z = 1;
+        ++n_attr;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n_attr;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, tm_w, tm_x, static_cast<int>(k_blocks), splits, tail, d.status_ptr);
+    LCE_COUNT_LAUNCH();
+    return cuda_failed(err) ? LCE_ERR_CUDA : LCE_OK;
+}
 
 template <class T>
-int forward_impl(const DeviceInfo& d, Operand x, Operand w, const ProductPlan& p, long long M, long long N, long long K,
+int forward_impl(const DeviceInfo& d, Operand x, Operand w, const ProductPlan& p, bool decode, long long M, long long N, long long K,
                  const LinearTail<T>& tail, char* ws, cudaStream_t s) {
     int rc;
     if ((rc = place_operand<T>(x, ws, s)) || (rc = place_operand<T>(w, ws, s))) return rc;
+    if constexpr (sizeof(T) == 2) {
+        if (decode) {
+            if (M <= 16) return launch_decode<T, 16>(d, x, w, N, K, tail, s);
+            if (M <= 32) return launch_decode<T, 32>(d, x, w, N, K, tail, s);
+            return launch_decode<T, 64>(d, x, w, N, K, tail, s);
+        }
+    }
     return product<T, false, false>(d, p, x, w, M, N, K, tail, ws, s);
 }
 
@@ -240,7 +300,7 @@ size_t lce_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void
                                           int64_t K, int dtype, unsigned flags) {
     if (!linear_args_ok(M, N, K, ldx, ldw, LCE_ACT_NONE, dtype) || linear_too_large(M, N, K) || M == 0) return 0;
     return forward_bytes(plan_operand(x, ldx, M, K, dtype, flags), plan_operand(w, ldw, N, K, dtype, flags),
-                         plan_product(M, N, K, dtype, flags));
+                         plan_product(M, N, K, dtype, flags), decodes(M, dtype, flags));
 }
 
 int lce_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, const void* residual,
@@ -253,7 +313,8 @@ int lce_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     if (!x || !w || !out) return LCE_ERR_ARG;
     const Operand xo = plan_operand(x, ldx, M, K, dtype, flags), wo = plan_operand(w, ldw, N, K, dtype, flags);
     const ProductPlan p = plan_product(M, N, K, dtype, flags);
-    const size_t need = forward_bytes(xo, wo, p);
+    const bool decode = decodes(M, dtype, flags);
+    const size_t need = forward_bytes(xo, wo, p, decode);
     if (need > 0 && (!ws || ws_bytes < need)) return LCE_ERR_WS_TOO_SMALL;
     DeviceInfo* d;
     const int rc = device_info(&d);
@@ -261,7 +322,7 @@ int lce_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     char* scratch = static_cast<char*>(ws);
 #define LCE_LINEAR_FORWARD(T)                                                                                              \
-    forward_impl<T>(*d, xo, wo, p, M, N, K,                                                                                \
+    forward_impl<T>(*d, xo, wo, p, decode, M, N, K,                                                                             \
                     LinearTail<T>{static_cast<T*>(out), ldo, act == LCE_ACT_NONE ? nullptr : static_cast<T*>(pre),         \
                                   pre_pitch(N), static_cast<const T*>(bias), static_cast<const T*>(residual), ldr, static_cast<int>(M),  \
                                   static_cast<int>(N), act},                                                               \

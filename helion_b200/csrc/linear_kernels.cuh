@@ -317,8 +317,8 @@ __device__ __forceinline__ void pack32(const float (&v)[32], uint4 (&raw)[4]) {
     }
 }
 
-// ACT: the activation, or kActAny to go by the call's (CUDA-core GEMM, split contractions). HEAVY: for calls with an
-// activation, a residual or saved values.
+// ACT: the activation, or kActAny to go by the call's (CUDA-core GEMM, split contractions). HEAVY: for calls with a
+// bias, an activation or a residual.
 constexpr int kActAny = -1;
 template <class T, int ACT, bool HEAVY>
 struct EpiLinear;
@@ -532,6 +532,207 @@ linear_reduce_kernel(const float* scratch, int slices, long long slab_floats, in
             if (t.residual != nullptr) z[j] += Cvt<T>::to_f(t.residual[row * t.ldr + col + j]);
             t.out[row * t.ldo + col + j] = Cvt<T>::from_f(z[j]);
         }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// A handful of tokens (at most 64): the product is bound by reading W once, so W is the operand with 128 rows and the
+// tokens are the narrow one:
+//   D[n, m] = sum_k W[n, k] x[m, k],  128 x BN tiles, BN = 16, 32 or 64 (tokens beyond M read as zeros)
+// With x as the 128-row operand (the core above) a launch moves the same bytes but needs its partial sums in global
+// memory and a second launch to add them. Here the contraction is split over the CTAs of a cluster: each streams its
+// share of 128 rows of W through a TMA ring, multiplies (tcgen05, one accumulator of BN columns), leaves its partial
+// tile in shared memory, and after one cluster barrier every CTA adds BN / S columns of it over the cluster in rank order
+// and runs the epilogue on them. A ring of about 100 KB lets two CTAs share an SM, so a whole wave of W is in flight.
+// Warp roles: 0 TMA producer, 1 MMA issuer and tensor-memory owner, 2-5 read the accumulator (warp w lanes 32*(w%4)..).
+// ---------------------------------------------------------------------------------------------
+template <int BN>
+struct DecodeSmem {
+    static constexpr int kABytes = kBM * kBK * 2;
+    static constexpr int kStageBytes = kABytes + BN * kBK * 2;
+    static constexpr int kStages = BN == 16 ? 6 : (BN == 32 ? 5 : 4);
+    static constexpr int kTotalBytes = kStages * kStageBytes + 128 + 1024;  // barriers; slack to align the ring by hand
+    static_assert(BN * kBM * 4 <= kStages * kStageBytes, "the partial tile takes the ring's place");
+};
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <class T, int BN>
+__global__ void __launch_bounds__(kGemmThreads, 2)
+linear_decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, int k_blocks, int splits,
+                     const LinearTail<T> t, int* __restrict__ status) {
+    using S = DecodeSmem<BN>;
+    constexpr int kStages = S::kStages;
+    constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
+    constexpr uint32_t kIdesc = ptx::make_idesc_f16(kBM, BN, std::is_same<T, __nv_bfloat16>::value, false, false);
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bars = base + kStages * S::kStageBytes;  // full[kStages] | empty[kStages] | done | tmem ptr | abort
+    uint8_t* gen = smem_raw + (base - ptx::smem_u32(smem_raw));
+    uint8_t* gen_bars = gen + kStages * S::kStageBytes;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (kStages + s); };
+    const uint32_t done = bars + 8u * (2 * kStages);
+    volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(gen_bars + 8 * (2 * kStages + 1));
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gen_bars + 8 * (2 * kStages + 1) + 4);
+    static_assert(8 * (2 * kStages + 2) <= 128, "barrier block");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = splits > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+    const int tile = static_cast<int>(blockIdx.x) / splits;
+    const int kb0 = static_cast<int>(static_cast<long long>(k_blocks) * rank / splits);
+    const int kb1 = static_cast<int>(static_cast<long long>(k_blocks) * (rank + 1) / splits);  // splits <= k_blocks: never empty
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            ptx::mbar_init(full(s), 1);
+            ptx::mbar_init(empty(s), 1);
+        }
+        ptx::mbar_init(done, 1);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&tm_w);
+        ptx::prefetch_tensormap(&tm_x);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(ptx::smem_u32(const_cast<uint32_t*>(tmem_ptr)), kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = *tmem_ptr;
+    ptx::grid_dep_launch();
+    ptx::grid_dep_wait();  // nothing above touched global memory
+
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            const uint64_t keep = ptx::make_l2_policy(ptx::kL2EvictLast), stream = ptx::make_l2_policy(ptx::kL2EvictFirst);
+            int issued = 0;
+            bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+                const int s = issued % kStages;
+                if (!ptx::mbar_wait(empty(s), ((issued / kStages) & 1u) ^ 1u, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t sa = base + s * S::kStageBytes;
+                ptx::mbar_arrive_expect_tx(full(s), S::kStageBytes);
+                ptx::tma_load_2d_hint(sa, &tm_w, full(s), kb * kBK, tile * kBM, stream);   // W: read once
+                ptx::tma_load_2d_hint(sa + S::kABytes, &tm_x, full(s), kb * kBK, 0, keep);  // x: every CTA reads it
+            }
+            if (!ok) {  // let the copies in flight land before the CTA retires
+                atomicCAS(status, 0, kDevErrProducerTimeout);
+                const int back = issued < kStages ? issued : kStages;
+                for (int j = 1; j <= back; ++j)
+                    for (int spin = 0; spin < (1 << 16); ++spin)
+                        if (ptx::mbar_try_wait(full((issued - j) % kStages), ((issued - j) / kStages) & 1u)) break;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (ptx::elect_one()) {
+            bool ok = true;
+            int used = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++used) {
+                const int s = used % kStages;
+                if (!ptx::mbar_wait(full(s), (used / kStages) & 1u, abort_flag)) {
+                    atomicCAS(status, 0, kDevErrMmaTimeout);
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                const uint32_t sa = base + s * S::kStageBytes, sb = sa + S::kABytes;
+#pragma unroll
+                for (int k = 0; k < kBK / kUmmaK; ++k)
+                    ptx::umma_f16(tmem, ptx::make_smem_desc(sa + k * (kUmmaK * 2), 0, 1024),
+                                  ptx::make_smem_desc(sb + k * (kUmmaK * 2), 0, 1024), kIdesc, (kb != kb0 || k != 0) ? 1u : 0u);
+                ptx::umma_commit(empty(s));
+            }
+            ptx::umma_commit(done);  // also on the way out of a timeout: what was issued drains before the memory is freed
+            if (!ok)
+                for (int spin = 0; spin < (1 << 16); ++spin)
+                    if (ptx::mbar_try_wait(done, 0)) break;
+        }
+        __syncwarp();
+    }
+    // The accumulator: thread = one of 128 features, a column a token.
+    float acc[BN < 32 ? 32 : BN];
+    const int feature = (warp & 3) * 32 + lane;
+    if (warp >= 2) {
+        if (!ptx::mbar_wait(done, 0, abort_flag) && lane == 0) atomicCAS(status, 0, kDevErrEpilogueTimeout);
+        __syncwarp();
+        ptx::tc_fence_after_sync();
+        const uint32_t taddr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+#pragma unroll
+        for (int c = 0; c < static_cast<int>(kTmemCols); c += 32) ptx::tmem_ld_32x32(taddr + c, *reinterpret_cast<float(*)[32]>(acc + c));
+        ptx::tmem_ld_wait();
+        ptx::tc_fence_before_sync();
+    }
+    const int n = tile * kBM + feature;
+    // G tokens of feature n from token m0 on (those below m1): everything is read before anything is written.
+    const float bias = warp >= 2 && n < t.cols && t.bias != nullptr ? Cvt<T>::to_f(t.bias[n]) : 0.f;
+    constexpr int G = BN / 8;  // a cluster of 8 leaves this many to each
+    auto finish = [&](float* z, int m0, int m1) {
+        float r[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            r[i] = t.residual != nullptr && m0 + i < m1 ? Cvt<T>::to_f(t.residual[(m0 + i) * t.ldr + n]) : 0.f;
+            z[i] += bias;
+        }
+        float (&v)[G] = *reinterpret_cast<float(*)[G]>(z);
+        if (t.pre != nullptr) {
+            float saved[G];
+            linear_saved(v, t.act, saved);
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+                if (m0 + i < m1) t.pre[(m0 + i) * t.ldp + n] = Cvt<T>::from_f(saved[i]);
+        }
+        linear_act<true>(v, t.act);
+#pragma unroll
+        for (int i = 0; i < G; ++i)
+            if (m0 + i < m1) t.out[(m0 + i) * t.ldo + n] = Cvt<T>::from_f(v[i] + r[i]);
+    };
+    if (splits == 1) {
+        if (warp >= 2 && n < t.cols) {
+#pragma unroll
+            for (int m = 0; m < BN; m += G)
+                if (m < t.rows) finish(acc + m, m, t.rows);
+        }
+        __syncthreads();
+    } else {
+        float* part = reinterpret_cast<float*>(gen);  // [token][feature]: all products that read the ring have finished
+        if (warp >= 2) {
+#pragma unroll
+            for (int m = 0; m < BN; ++m) part[m * kBM + feature] = acc[m];
+        }
+        __syncthreads();
+        ptx::cluster_sync_all();
+        if (warp >= 2 && n < t.cols) {
+            const int per = BN / splits;
+            const int m1 = min((rank + 1) * per, t.rows);
+            for (int m0 = rank * per; m0 < m1; m0 += G) {
+                const uint32_t at = base + static_cast<uint32_t>(m0 * kBM + feature) * 4u;
+                float z[G];
+#pragma unroll
+                for (int i = 0; i < G; ++i) z[i] = m0 + i < m1 ? ld_cluster_f32(ptx::map_to_cta(at + i * kBM * 4, 0)) : 0.f;
+                for (int s = 1; s < splits; ++s) {  // in rank order
+#pragma unroll
+                    for (int i = 0; i < G; ++i) z[i] += m0 + i < m1 ? ld_cluster_f32(ptx::map_to_cta(at + i * kBM * 4, s)) : 0.f;
+                }
+                finish(z, m0, m1);
+            }
+        }
+        __syncthreads();
+        ptx::cluster_sync_all();  // no CTA leaves while another may still read its part
+    }
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem, kTmemCols);
     }
 }
 

@@ -70,8 +70,9 @@ def test_c_abi_checks_and_workspace_sizes():
     need = L.lce_linear_forward_workspace_bytes(p + 2, 64, p, 64, 4, 32, 64, 0, 0)
     assert need >= 4 * 64 * 2 and forward(x=p + 2, ws=p, ws_bytes=need - 1) == 3 and forward(x=p + 2) == 3
     assert L.lce_linear_forward_workspace_bytes(p, 64, p, 64, 4, 32, 64, 0, 0) == 0
-    # a short product is split along its contraction: slabs
-    assert L.lce_linear_forward_workspace_bytes(p, 8192, p, 8192, 16, 4096, 8192, 0, 0) > 0
+    # a short product is split along its contraction: slabs; a handful of tokens needs none
+    assert L.lce_linear_forward_workspace_bytes(p, 8192, p, 8192, 100, 4096, 8192, 0, 0) > 0
+    assert L.lce_linear_forward_workspace_bytes(p, 8192, p, 8192, 16, 4096, 8192, 0, 0) == 0
 
     def backward(dy=p, ldy=32, pre=p, dx=p, dw=p, db=p, m=4, act=2, ws=None, ws_bytes=0):
         return L.lce_linear_backward(dy, ldy, p, 64, p, 64, pre, dx, dw, db, m, 32, 64, act, 0, ws, ws_bytes, 0, None)
