@@ -18,7 +18,7 @@ FLAG_FORCE_SIMT, FLAG_FORCE_TC, FLAG_DX_F32, FLAG_NO_DX, FLAG_NO_DW, FLAG_ONE_CT
 REDUCTIONS = {"none": REDUCTION_NONE, "mean": REDUCTION_MEAN, "sum": REDUCTION_SUM}
 
 class HeadRows(ctypes.Structure):
-    """``lce_head_rows`` of include/helion_lce.h."""
+    """``lce_head_rows`` of include/helion_lce.h; passed by address."""
 
     _fields_ = [("x", c_void_p), ("x_stride", c_int64 * 3), ("out", c_void_p), ("out_stride", c_int64 * 3),
                 ("grad", c_void_p), ("grad_stride", c_int64 * 3), ("weight", c_void_p), ("dweight", c_void_p),
@@ -87,12 +87,12 @@ SIGNATURES = {
     "lce_sample_logits": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p, ctypes.c_float, c_void_p, c_int,
                                   c_int64, c_void_p, ctypes.c_float, c_void_p, ctypes.c_float, c_void_p, c_void_p, c_void_p,
                                   c_size_t, c_void_p]),
-    "lce_rope": (c_int, [ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int,
+    "lce_rope": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int,
                          ctypes.c_float, c_int, c_int, c_void_p]),
-    "lce_qk_norm_rope_forward": (c_int, [ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
+    "lce_qk_norm_rope_forward": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
                                          c_void_p, c_int64, c_int, ctypes.c_float, ctypes.c_float, c_int, c_void_p]),
     "lce_qk_norm_rope_backward_workspace_bytes": (c_size_t, [c_int64]),
-    "lce_qk_norm_rope_backward": (c_int, [ctypes.POINTER(HeadRows), ctypes.POINTER(HeadRows), c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
+    "lce_qk_norm_rope_backward": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64, c_int64,
                                           c_void_p, c_int64, c_int, ctypes.c_float, ctypes.c_float, c_int, c_void_p, c_size_t,
                                           c_void_p]),
     "lce_set_tuning": (None, [c_int, c_int, c_int]),

@@ -36,6 +36,14 @@ int check_head_rows(const lce_head_rows* r, const HeadCall& c) {
     return LCE_OK;
 }
 
+// A dimension of one entry has no stride: whatever the caller's tensor says there must not cost it the vector form.
+lce_head_rows plain_strides(lce_head_rows r, const HeadCall& c) {
+    const int64_t extent[3] = {c.batch, c.seq, r.heads};
+    for (int i = 0; i < 3; ++i)
+        if (extent[i] == 1) r.x_stride[i] = r.out_stride[i] = r.grad_stride[i] = 0;
+    return r;
+}
+
 // Deals `tokens` x `heads` rows to warps: whole tokens per warp (their angles are formed once) as long as that gives
 // every SM `kWarps` warps, pieces of a token otherwise. A step is `per_step` heads.
 template <class T>
@@ -155,13 +163,12 @@ int heads_call(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, in
     HeadCall c{batch, seq, dim, half, interleaved, MODE, dtype, 0};
     int rc = check_head_rows(q, c);
     if (rc) return rc;
-    const lce_head_rows none = {};
-    const lce_head_rows& kr = k ? *k : none;
     if (k && (rc = check_head_rows(k, c))) return rc;
-    const bool work = batch > 0 && seq > 0 && (q->heads > 0 || kr.heads > 0);
-    if (!work && !(MODE == kHeadNormBackward && (q->dweight || kr.dweight))) return LCE_OK;
+    const lce_head_rows qr = plain_strides(*q, c), kr = k ? plain_strides(*k, c) : lce_head_rows{};
+    const bool work = batch > 0 && seq > 0 && (qr.heads > 0 || kr.heads > 0);
+    if (!work && !(MODE == kHeadNormBackward && (qr.dweight || kr.dweight))) return LCE_OK;
     if (work && (!positions || (half > 0 && !freq))) return LCE_ERR_ARG;
-    if (MODE == kHeadNormBackward && (q->dweight || kr.dweight) &&
+    if (MODE == kHeadNormBackward && (qr.dweight || kr.dweight) &&
         (!ws || ws_bytes < lce_qk_norm_rope_backward_workspace_bytes(dim)))
         return LCE_ERR_WS_TOO_SMALL;
     DeviceInfo* d;
@@ -181,7 +188,7 @@ int heads_call(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, in
     p.scale = scale;
     p.sin_sign = inverse ? -1.f : 1.f;
     p.eps = eps;
-    return dispatch_heads<MODE>(c, *q, kr, p, static_cast<float*>(ws), static_cast<cudaStream_t>(stream));
+    return dispatch_heads<MODE>(c, qr, kr, p, static_cast<float*>(ws), static_cast<cudaStream_t>(stream));
 }
 
 // ---------------------------------------------------------------------------------------------

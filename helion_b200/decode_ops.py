@@ -17,8 +17,9 @@ from __future__ import annotations
 import torch
 
 from . import _lib, parallel
-from .ops import FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _need_contiguous, _need_cuda, _need_dtype, _on_device, _path_flags, \
-    _ptr, _stream, _workspace
+from .ops import FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _launch, _need_contiguous, _need_cuda, _need_dtype, _on_device, \
+    _path_flags, _ptr, _stream, _workspace
+
 
 
 def greedy_head(hidden: torch.Tensor, weight: torch.Tensor, *, vocab_start: int | None = None,
@@ -325,16 +326,10 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
     token = torch.empty(shape, dtype=torch.int64, device=dev)
     logprob = torch.empty(shape, dtype=torch.float32, device=dev) if return_logprob else None
     if rows:
-        L = _lib.lib()
         code = _DTYPE_CODE[logits.dtype]
-        need = L.lce_sample_logits_workspace_bytes(rows, vocab, code)
+        need = _lib.lib().lce_sample_logits_workspace_bytes(rows, vocab, code)
         ws = _workspace(need, dev) if need else None
-        with _on_device(dev):
-            _lib.check(
-                L.lce_sample_logits(flat.data_ptr(), flat.stride(0) if rows > 1 else vocab, rows, vocab, code,
-                                    uniforms.contiguous().data_ptr(), _ptr(t), t_all, _ptr(k),
-                                    int(k is not None and k.dtype == torch.int64), int(k_all), _ptr(p), p_all, _ptr(m), m_all,
-                                    token.data_ptr(), _ptr(logprob), _ptr(ws), need, _stream(dev)),
-                "lce_sample_logits",
-            )
+        _launch("lce_sample_logits", dev, flat.data_ptr(), flat.stride(0) if rows > 1 else vocab, rows, vocab, code,
+                uniforms.contiguous().data_ptr(), _ptr(t), t_all, _ptr(k), k is not None and k.dtype is torch.int64, int(k_all),
+                _ptr(p), p_all, _ptr(m), m_all, token.data_ptr(), _ptr(logprob), _ptr(ws), need)
     return (token, logprob) if return_logprob else token

@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import FLOAT_DTYPES, _DTYPE_CODE, _need_cuda, _need_dtype, _on_device, _path_flags, _ptr, _stream, _workspace
+from .ops import FLOAT_DTYPES, _DTYPE_CODE, _launch, _need_cuda, _need_dtype, _path_flags, _ptr, _workspace
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -27,28 +27,31 @@ def _check(x, weight, bias, activation, residual) -> int:
     _need_cuda("x", x)
     _need_cuda("weight", weight)
     _need_dtype("x", x, FLOAT_DTYPES)
-    if x.dim() < 1:
+    shape, dtype, device = x.shape, x.dtype, x.device
+    if not shape:
         raise ValueError("x must have at least 1 dimension shaped (..., in_features).")
     if weight.dim() != 2:
         raise ValueError("weight must be a 2D tensor shaped (out_features, in_features).")
     n, k = weight.shape
-    if x.shape[-1] != k:
-        raise ValueError(f"Shape mismatch: x has last dimension {x.shape[-1]}, weight expects {k}.")
+    if shape[-1] != k:
+        raise ValueError(f"Shape mismatch: x has last dimension {shape[-1]}, weight expects {k}.")
     if n <= 0 or k <= 0:
         raise ValueError("out_features and in_features must be positive.")
-    if bias is not None and tuple(bias.shape) != (n,):
+    if bias is not None and bias.shape != (n,):
         raise ValueError(f"Shape mismatch: bias has shape {tuple(bias.shape)}, expected ({n},).")
-    if residual is not None and residual.shape != (*x.shape[:-1], n):
-        raise ValueError(f"Shape mismatch: residual has shape {tuple(residual.shape)}, expected {(*x.shape[:-1], n)}.")
-    dtype, device = x.dtype, x.device
+    if residual is not None and residual.shape != (*shape[:-1], n):
+        raise ValueError(f"Shape mismatch: residual has shape {tuple(residual.shape)}, expected {(*shape[:-1], n)}.")
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and t.dtype != dtype:
+        if t is None:
+            continue
+        if t.dtype != dtype:
             raise ValueError(f"Dtype mismatch: {name} has dtype {t.dtype}, x has dtype {dtype}.")
-        if t is not None and t.device != device:
+        if t.device != device:
             raise ValueError(f"Device mismatch: {name} is on {t.device}, x is on {device}.")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"activation must be one of None, 'relu', 'gelu', 'gelu_tanh', 'silu'; got {activation!r}.")
-    return ACTIVATIONS[activation]
+    return act
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -76,17 +79,12 @@ def _forward(x, weight, bias, residual, act: int, save: bool):
     pre = torch.empty((m, (n + 7) // 8 * 8), dtype=x.dtype, device=dev) if save and act else None
     if m == 0:
         return out, pre
-    L = _lib.lib()
     flags = _flags(dtype)
     xp, wp = x2.data_ptr(), w2.data_ptr()
-    need = L.lce_linear_forward_workspace_bytes(xp, ldx, wp, ldw, m, n, k, dtype, flags)
+    need = _lib.lib().lce_linear_forward_workspace_bytes(xp, ldx, wp, ldw, m, n, k, dtype, flags)
     ws = _workspace(need, dev) if need else None
-    with _on_device(dev):
-        _lib.check(
-            L.lce_linear_forward(xp, ldx, wp, ldw, _ptr(b), _ptr(r2), ldr, out.data_ptr(), n, _ptr(pre), m, n, k, act, dtype,
-                                 _ptr(ws), need, flags, _stream(dev)),
-            "lce_linear_forward",
-        )
+    _launch("lce_linear_forward", dev, xp, ldx, wp, ldw, _ptr(b), _ptr(r2), ldr, out.data_ptr(), n, _ptr(pre), m, n, k, act,
+            dtype, _ptr(ws), need, flags)
     return out, pre
 
 
@@ -106,17 +104,11 @@ def _backward(dy, x, weight, pre, act: int, need_x: bool, need_w: bool, need_b: 
     dx = torch.empty((m, k), dtype=x.dtype, device=dev) if need_x else None
     dw = torch.empty((n, k), dtype=x.dtype, device=dev) if need_w else None
     db = torch.empty((n,), dtype=x.dtype, device=dev) if need_b else None
-    L = _lib.lib()
     flags = _flags(dtype)
     args = (dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw)
-    need = L.lce_linear_backward_workspace_bytes(*args, m, n, k, act, dtype, flags)
-    ws = _workspace(need, dev)
-    with _on_device(dev):
-        _lib.check(
-            L.lce_linear_backward(*args, _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db), m, n, k, act, dtype, ws.data_ptr(),
-                                  ws.numel(), flags, _stream(dev)),
-            "lce_linear_backward",
-        )
+    ws = _workspace(_lib.lib().lce_linear_backward_workspace_bytes(*args, m, n, k, act, dtype, flags), dev)
+    _launch("lce_linear_backward", dev, *args, _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db), m, n, k, act, dtype, ws.data_ptr(),
+            ws.numel(), flags)
     return dx, dw, db
 
 
@@ -126,7 +118,7 @@ class _Linear(torch.autograd.Function):
         out, pre = _forward(x, weight, bias, residual, act, True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
-        return out.view(*x.shape[:-1], out.shape[-1])
+        return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[1])
 
     @staticmethod
     @once_differentiable
@@ -151,7 +143,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     pitch; inputs whose elements are not contiguous are copied first. fp32 is computed in fp32 throughout. Differentiable
     in ``x``, ``weight``, ``bias`` and ``residual``; sums are formed in a fixed order."""
     act = _check(x, weight, bias, activation, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
-                                    (residual is not None and residual.requires_grad)):
+    if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+            (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         return _Linear.apply(x, weight, bias, residual, act)
-    return _forward(x, weight, bias, residual, act, False)[0].view(*x.shape[:-1], weight.shape[0])
+    out = _forward(x, weight, bias, residual, act, False)[0]
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[1])

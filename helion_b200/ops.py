@@ -164,6 +164,20 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
+def _launch(what: str, device: torch.device, *args) -> None:
+    """The C-ABI call ``what`` with ``args`` and, last, the current stream of ``device``, which is made current for it;
+    the lean form of ``with _on_device(...): check(...)`` for calls that take a few microseconds in all."""
+    fn = getattr(_lib.lib(), what)
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        code = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, _stream(device))
+    if code:
+        _lib.check(code, what)
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

@@ -14,14 +14,16 @@ nothing to them.
 
 from __future__ import annotations
 
+import ctypes
 import math
+from array import array
 from typing import Any
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _need_cuda, _need_dtype, _on_device, _stream, _workspace
+from .ops import FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _launch, _need_cuda, _need_dtype, _workspace
 
 MAX_HEAD_DIM = 1024
 _SCALINGS = (None, "linear", "ntk", "yarn")
@@ -81,23 +83,23 @@ def _check_heads(name: str, x: torch.Tensor) -> None:
         raise ValueError(f"{name} must have a head dimension between 1 and {MAX_HEAD_DIM}; got {x.shape[-1]}.")
 
 
-def _check_positions(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor) -> None:
+def _check_positions(shape: torch.Size, device: torch.device, positions: torch.Tensor, frequencies: torch.Tensor) -> None:
     _need_cuda("positions", positions)
     _need_cuda("frequencies", frequencies)
     _need_dtype("positions", positions, INDEX_DTYPES)
     _need_dtype("frequencies", frequencies, (torch.float64,))
-    lead = x.shape[:-2]
+    lead = shape[:-2]
     if positions.shape != lead and positions.shape != lead[-1:]:
         wanted = f"{tuple(lead)}" + (f" or {tuple(lead[-1:])}" if len(lead) == 2 else "")
         raise ValueError(f"Shape mismatch: positions has shape {tuple(positions.shape)}, expected {wanted}.")
-    if frequencies.dim() != 1 or 2 * frequencies.shape[0] > x.shape[-1]:
+    if frequencies.dim() != 1 or 2 * frequencies.shape[0] > shape[-1]:
         raise ValueError(f"Shape mismatch: frequencies has shape {tuple(frequencies.shape)}, expected 1D with at most "
-                         f"{x.shape[-1] // 2} entries (half the head dimension).")
+                         f"{shape[-1] // 2} entries (half the head dimension).")
     if not frequencies.is_contiguous():
         raise ValueError("frequencies must be contiguous.")
     for name, t in (("positions", positions), ("frequencies", frequencies)):
-        if t.device != x.device:
-            raise ValueError(f"Device mismatch: {name} is on {t.device}, the heads are on {x.device}.")
+        if t.device != device:
+            raise ValueError(f"Device mismatch: {name} is on {t.device}, the heads are on {device}.")
 
 
 def _rows_readable(x: torch.Tensor) -> torch.Tensor:
@@ -105,32 +107,35 @@ def _rows_readable(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _strides(x: torch.Tensor) -> tuple[int, int, int]:
-    """Element strides of (batch, seq, head); a dimension of one entry has none (0)."""
-    shape, stride = x.shape, x.stride()
-    head = stride[-2] if shape[-2] > 1 else 0
-    seq = stride[-3] if shape[-3] > 1 else 0
-    return (stride[0] if len(shape) == 4 and shape[0] > 1 else 0), seq, head
+# ----------------------------------------------------------------------------------------------
+# what crosses the C ABI
+# ----------------------------------------------------------------------------------------------
+_NO_TENSOR = (0, 0, 0, 0)
 
 
-_NO_STRIDES = (0, 0, 0)
+def _placed(x: torch.Tensor) -> tuple[int, int, int, int]:
+    """Pointer and element strides of (batch, seq, head)."""
+    s = x.stride()
+    return (x.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (x.data_ptr(), 0, s[0], s[1])
 
 
-def _rows(x: torch.Tensor, out: torch.Tensor, grad: torch.Tensor | None = None, weight: torch.Tensor | None = None,
-          dweight: torch.Tensor | None = None) -> _lib.HeadRows:
-    return _lib.HeadRows(x.data_ptr(), _strides(x), out.data_ptr(), _strides(out),
-                         None if grad is None else grad.data_ptr(), _NO_STRIDES if grad is None else _strides(grad),
-                         None if weight is None else weight.data_ptr(), None if dweight is None else dweight.data_ptr(),
-                         x.shape[-2])
+def _row_fields(x: torch.Tensor, out: torch.Tensor, grad: torch.Tensor | None = None, weight: torch.Tensor | None = None,
+                dweight: torch.Tensor | None = None) -> tuple[int, ...]:
+    """The fields of ``lce_head_rows``, 64 bits each."""
+    return (*_placed(x), *_placed(out), *(_NO_TENSOR if grad is None else _placed(grad)),
+            0 if weight is None else weight.data_ptr(), 0 if dweight is None else dweight.data_ptr(), x.shape[-2])
+
+
+_ROW_BYTES = ctypes.sizeof(_lib.HeadRows)
 
 
 def _place(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor):
     """(batch, seq, dim, positions pointer, is int64, its batch stride, its seq stride, frequencies pointer, half)."""
     shape = x.shape
-    batch, seq = (1, shape[0]) if len(shape) == 3 else (shape[0], shape[1])
     stride = positions.stride()
-    return (batch, seq, shape[-1], positions.data_ptr(), int(positions.dtype == torch.int64),
-            stride[0] if len(stride) == 2 else 0, stride[-1], frequencies.data_ptr(), frequencies.shape[0])
+    batch, seq, _, dim = shape if len(shape) == 4 else (1, *shape)
+    return (batch, seq, dim, positions.data_ptr(), positions.dtype is torch.int64, stride[0] if len(stride) == 2 else 0,
+            stride[-1], frequencies.data_ptr(), frequencies.shape[0])
 
 
 # ----------------------------------------------------------------------------------------------
@@ -139,13 +144,9 @@ def _place(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor):
 def _rope(x, positions, frequencies, interleaved, scale, inverse):
     x = _rows_readable(x)
     out = torch.empty_like(x)
-    dev = x.device
-    with _on_device(dev):
-        _lib.check(
-            _lib.lib().lce_rope(_rows(x, out), *_place(x, positions, frequencies), int(interleaved), scale, int(inverse),
-                                _DTYPE_CODE[x.dtype], _stream(dev)),
-            "lce_rope",
-        )
+    rows = array("q", _row_fields(x, out))
+    _launch("lce_rope", x.device, rows.buffer_info()[0], *_place(x, positions, frequencies), interleaved, scale, inverse,
+            _DTYPE_CODE[x.dtype])
     return out
 
 
@@ -174,10 +175,10 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
     ``(x[i], x[half + i])``, or ``(x[2i], x[2i + 1])`` with ``interleaved``; ``scale`` multiplies the rotated part.
     Differentiable in ``x``; the backward pass is the same kernel turning the other way."""
     _check_heads("x", x)
-    _check_positions(x, positions, frequencies)
-    if torch.is_grad_enabled() and x.requires_grad:
+    _check_positions(x.shape, x.device, positions, frequencies)
+    if x.requires_grad and torch.is_grad_enabled():
         return _Rope.apply(x, positions, frequencies, bool(interleaved), float(scale), False)
-    return _rope(x, positions, frequencies, interleaved, float(scale), False)
+    return _rope(x, positions, frequencies, bool(interleaved), float(scale), False)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -185,14 +186,10 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
 # ----------------------------------------------------------------------------------------------
 def _qk_forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, scale):
     q_out, k_out = torch.empty_like(q), torch.empty_like(k)
-    dev = q.device
-    with _on_device(dev):
-        _lib.check(
-            _lib.lib().lce_qk_norm_rope_forward(_rows(q, q_out, weight=q_weight), _rows(k, k_out, weight=k_weight),
-                                                *_place(q, positions, frequencies), int(interleaved), scale, eps,
-                                                _DTYPE_CODE[q.dtype], _stream(dev)),
-            "lce_qk_norm_rope_forward",
-        )
+    rows = array("q", _row_fields(q, q_out, None, q_weight) + _row_fields(k, k_out, None, k_weight))
+    at = rows.buffer_info()[0]
+    _launch("lce_qk_norm_rope_forward", q.device, at, at + _ROW_BYTES, *_place(q, positions, frequencies), interleaved, scale,
+            eps, _DTYPE_CODE[q.dtype])
     return q_out, k_out
 
 
@@ -212,16 +209,11 @@ class _QKNormRope(torch.autograd.Function):
         dq, dk = torch.empty_like(q), torch.empty_like(k)
         dqw = torch.empty_like(q_weight) if ctx.needs_input_grad[2] else None
         dkw = torch.empty_like(k_weight) if ctx.needs_input_grad[3] else None
-        dev = q.device
-        L = _lib.lib()
-        ws = _workspace(L.lce_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), dev)
-        with _on_device(dev):
-            _lib.check(
-                L.lce_qk_norm_rope_backward(_rows(q, dq, gq, q_weight, dqw), _rows(k, dk, gk, k_weight, dkw),
-                                            *_place(q, positions, frequencies), int(interleaved), scale, eps,
-                                            _DTYPE_CODE[q.dtype], ws.data_ptr(), ws.numel(), _stream(dev)),
-                "lce_qk_norm_rope_backward",
-            )
+        ws = _workspace(_lib.lib().lce_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
+        rows = array("q", _row_fields(q, dq, gq, q_weight, dqw) + _row_fields(k, dk, gk, k_weight, dkw))
+        at = rows.buffer_info()[0]
+        _launch("lce_qk_norm_rope_backward", q.device, at, at + _ROW_BYTES, *_place(q, positions, frequencies), interleaved,
+                scale, eps, _DTYPE_CODE[q.dtype], ws.data_ptr(), ws.numel())
         need = ctx.needs_input_grad
         return (dq if need[0] else None), (dk if need[1] else None), dqw, dkw, None, None, None, None, None
 
@@ -238,24 +230,25 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     the gradients and the inputs once; the weights' gradients are summed in a fixed order."""
     _check_heads("q", q)
     _check_heads("k", k)
-    if k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
-        raise ValueError(f"Shape mismatch: k has shape {tuple(k.shape)}, q has shape {tuple(q.shape)}; they may differ in "
+    shape, dtype, device = q.shape, q.dtype, q.device
+    dim = shape[-1]
+    if k.shape[:-2] != shape[:-2] or k.shape[-1] != dim:
+        raise ValueError(f"Shape mismatch: k has shape {tuple(k.shape)}, q has shape {tuple(shape)}; they may differ in "
                          "the number of heads only.")
-    dim = q.shape[-1]
     for name, t in (("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
-        if t.device != q.device:
-            raise ValueError(f"Device mismatch: {name} is on {t.device}, q is on {q.device}.")
-        if t.dtype != q.dtype:
-            raise ValueError(f"Dtype mismatch: {name} has dtype {t.dtype}, q has dtype {q.dtype}.")
+        if t.device != device:
+            raise ValueError(f"Device mismatch: {name} is on {t.device}, q is on {device}.")
+        if t.dtype != dtype:
+            raise ValueError(f"Dtype mismatch: {name} has dtype {t.dtype}, q has dtype {dtype}.")
     for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if tuple(t.shape) != (dim,):
+        if t.shape != (dim,):
             raise ValueError(f"Shape mismatch: {name} has shape {tuple(t.shape)}, expected ({dim},).")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous.")
-    _check_positions(q, positions, frequencies)
+    _check_positions(shape, device, positions, frequencies)
     if not eps >= 0:
         raise ValueError("eps must not be negative.")
     q, k = _rows_readable(q), _rows_readable(k)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+    if (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad) and torch.is_grad_enabled():
         return _QKNormRope.apply(q, k, q_weight, k_weight, positions, frequencies, float(eps), bool(interleaved), float(scale))
-    return _qk_forward(q, k, q_weight, k_weight, positions, frequencies, float(eps), interleaved, float(scale))
+    return _qk_forward(q, k, q_weight, k_weight, positions, frequencies, float(eps), bool(interleaved), float(scale))

@@ -11,6 +11,8 @@ two such sums: 1e-5 of the magnitudes that it subtracts. dweight adds at most a 
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -316,7 +318,7 @@ def test_outputs_stay_inside_their_buffers():
         pos = torch.arange(seq, device=DEV)
         freq, _ = helion_b200.rope_frequencies(2 * half)
         rows = _lib.HeadRows(x.data_ptr(), x.stride()[:3], out.data_ptr(), out.stride()[:3], None, (0, 0, 0), None, None, heads)
-        _lib.check(L.lce_rope(rows, batch, seq, dim, pos.data_ptr(), 1, 0, 1, freq.data_ptr(), half, 0, 1.0, 0, code,
+        _lib.check(L.lce_rope(ctypes.byref(rows), batch, seq, dim, pos.data_ptr(), 1, 0, 1, freq.data_ptr(), half, 0, 1.0, 0, code,
                               torch.cuda.current_stream().cuda_stream), "lce_rope")
         torch.cuda.synchronize()
         assert torch.equal(out[:, :, :heads, :dim], helion_b200.rope(x, pos, freq))

@@ -111,7 +111,7 @@ def test_c_abi_refuses_before_it_touches_a_device():
     pos, freq = 16, 16  # never dereferenced: every call here is refused
 
     def rope(r=rows, batch=1, seq=1, dim=8, positions=pos, frequencies=freq, half=4, dtype=0):
-        return L.lce_rope(r, batch, seq, dim, positions, 1, 0, 1, frequencies, half, 0, 1.0, 0, dtype, None)
+        return L.lce_rope(None if r is None else ctypes.byref(r), batch, seq, dim, positions, 1, 0, 1, frequencies, half, 0, 1.0, 0, dtype, None)
 
     assert rope(dtype=9) == 1 and rope(batch=-1) == 1 and rope(half=5) == 1 and rope(dim=0) == 1
     assert rope(dim=1025) == 6 and rope(batch=1 << 40) == 6
@@ -123,7 +123,7 @@ def test_c_abi_refuses_before_it_touches_a_device():
     assert need > 0 and L.lce_qk_norm_rope_backward_workspace_bytes(0) == 0
     back = _lib.HeadRows(16, (64, 32, 8), 16, (64, 32, 8), 16, (64, 32, 8), 16, 16, 4)
     args = (1, 1, 8, pos, 1, 0, 1, freq, 4, 0, 1.0, 1e-6, 0)
-    assert L.lce_qk_norm_rope_backward(back, back, *args, 16, need - 1, None) == 3
-    assert L.lce_qk_norm_rope_backward(back, back, *args, None, need, None) == 3
-    assert L.lce_qk_norm_rope_backward(rows, back, *args, 16, need, None) == 1  # no gradient
-    assert L.lce_qk_norm_rope_forward(rows, None, *args, None) == 1
+    assert L.lce_qk_norm_rope_backward(ctypes.byref(back), ctypes.byref(back), *args, 16, need - 1, None) == 3
+    assert L.lce_qk_norm_rope_backward(ctypes.byref(back), ctypes.byref(back), *args, None, need, None) == 3
+    assert L.lce_qk_norm_rope_backward(ctypes.byref(rows), ctypes.byref(back), *args, 16, need, None) == 1  # no gradient
+    assert L.lce_qk_norm_rope_forward(ctypes.byref(rows), None, *args, None) == 1
