@@ -90,7 +90,8 @@ inline int make_tmap(CUtensorMap* tm, const void* base, int dtype, long long inn
 }
 
 // One operand of a GEMM as the host sees it: a row-major matrix [rows, cols] with a pitch.
-// As a K-major operand its rows are the m (n) index; as an MN-major operand its rows are k.
+// As a K-major operand its rows are the m (n) index; as an MN-major operand its rows are k. Columns beyond the
+// problem's are readable and hold zeros (only the CUDA-core GEMM looks at them).
 struct Mat {
     const void* ptr;
     long long rows, cols, pitch_elems;
@@ -318,28 +319,35 @@ int launch_simt(const DeviceInfo& d, const Mat& a, bool a_mn, const Mat& b, bool
     A.ptr = static_cast<const T*>(a.ptr);
     A.stride_mn = a_mn ? 1 : a.pitch_elems;
     A.stride_k = a_mn ? a.pitch_elems : 1;
-    A.extent_mn = static_cast<int>(M);
+    // fp32 rows that are padded with zeros to whole 16-byte vectors are read as whole vectors
+    auto up4 = [](long long v) { return (v + 3) / 4 * 4; };
+    auto mn_extent = [&](const Mat& x, bool mn, long long v) { return mn && x.cols >= up4(v) ? up4(v) : v; };
+    auto k_extent = [&](const Mat& x, bool mn) { return !mn && x.cols >= up4(K) ? up4(K) : K; };
+    A.extent_mn = static_cast<int>(mn_extent(a, a_mn, M));
+    A.extent_k = static_cast<int>(k_extent(a, a_mn));
     B.ptr = static_cast<const T*>(b.ptr);
     B.stride_mn = b_mn ? 1 : b.pitch_elems;
     B.stride_k = b_mn ? b.pitch_elems : 1;
-    B.extent_mn = static_cast<int>(Nn);
+    B.extent_mn = static_cast<int>(mn_extent(b, b_mn, Nn));
+    B.extent_k = static_cast<int>(k_extent(b, b_mn));
     const long long m_tiles = cdiv(M, kBM), n_tiles = cdiv(Nn, kSimtBN);
     if (m_tiles * n_tiles > 0x7fffffffll) return LCE_ERR_TOO_LARGE;
     if (m_tiles * n_tiles == 0 || K == 0) return LCE_OK;
     const long long cap = static_cast<long long>(d.sm_count) * 4;
     const long long work = m_tiles * n_tiles * k_splits;
     const int grid = static_cast<int>(work < cap ? work : cap);
-    const int k = static_cast<int>(K), mt = static_cast<int>(m_tiles), nt = static_cast<int>(n_tiles);
+    // one operand's zeros make up for what the other does not have
+    const int k = A.extent_k > B.extent_k ? A.extent_k : B.extent_k, mt = static_cast<int>(m_tiles), nt = static_cast<int>(n_tiles);
     bool launched = false;
     if constexpr (std::is_same<T, float>::value) {
         // fp32 operands that allow 16-byte loads along their contiguous direction take the vector loaders
-        const auto mode = [&](const SimtOperand<float>& op, long long extent) {
+        const auto mode = [&](const SimtOperand<float>& op) {
             if ((reinterpret_cast<uintptr_t>(op.ptr) & 15u) != 0) return static_cast<int>(kSimtGeneric);
-            if (op.stride_k == 1 && op.stride_mn % 4 == 0 && K % 4 == 0) return static_cast<int>(kSimtVecK);
-            if (op.stride_mn == 1 && op.stride_k % 4 == 0 && extent % 4 == 0) return static_cast<int>(kSimtVecMN);
+            if (op.stride_k == 1 && op.stride_mn % 4 == 0 && op.extent_k % 4 == 0) return static_cast<int>(kSimtVecK);
+            if (op.stride_mn == 1 && op.stride_k % 4 == 0 && op.extent_mn % 4 == 0) return static_cast<int>(kSimtVecMN);
             return static_cast<int>(kSimtGeneric);
         };
-        const int am = mode(A, M), bm = mode(B, Nn);
+        const int am = mode(A), bm = mode(B);
 #define LCE_SIMT_GO(AM, BM) \
     gemm_simt_kernel<float, Epi, AM, BM><<<grid, kSimtThreads, 0, stream>>>(A, B, k, mt, nt, k_splits, ep), launched = true
         if (am == kSimtVecK && bm == kSimtVecK) LCE_SIMT_GO(kSimtVecK, kSimtVecK);

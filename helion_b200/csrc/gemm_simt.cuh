@@ -36,6 +36,8 @@ struct SimtOperand {
     long long stride_mn;  // elements between consecutive m (resp. n)
     long long stride_k;   // elements between consecutive k
     int extent_mn;        // valid m (resp. n)
+    int extent_k;         // readable k: at or beyond it the operand counts as zero (a contraction may be longer, when the
+                          // other operand has zeros there)
 };
 
 // How a thread fetches its share (4 elements) of a 128 x 8 operand tile:
@@ -57,16 +59,18 @@ struct SimtLoader<T, kSimtGeneric> {
     static constexpr bool kAsync = false;
     const T* p;
     long long step, k_adv;
-    int mn_t, k_t, mn_step, k_step, mn_left;
+    int mn_t, k_t, mn_step, k_step, mn_left, k_limit;
     __device__ __forceinline__ void init(const SimtOperand<T>& op, int mn0, int k_begin, int t) {
         if (op.stride_k == 1) { k_t = t % kSimtBK; mn_t = t / kSimtBK; mn_step = kSimtThreads / kSimtBK; k_step = 0; }
         else { mn_t = t % 128; k_t = t / 128; mn_step = 0; k_step = kSimtThreads / 128; }
         p = op.ptr + static_cast<long long>(mn0 + mn_t) * op.stride_mn + static_cast<long long>(k_begin + k_t) * op.stride_k;
         step = mn_step * op.stride_mn + k_step * op.stride_k;
         k_adv = kSimtBK * op.stride_k;
+        k_limit = op.extent_k;
         mn_left = op.extent_mn - mn0 - mn_t;  // element i is in range iff i * mn_step < mn_left
     }
     __device__ __forceinline__ void fetch(int k0, int k_end, float (&r)[kSimtLoads], float*) {
+        k_end = min(k_end, k_limit);
 #pragma unroll
         for (int i = 0; i < kSimtLoads; ++i) {
             r[i] = 0.f;
@@ -123,11 +127,12 @@ struct SimtLoader<float, kSimtVecMN> {
     static constexpr bool kAsync = true;
     const float* p;
     long long k_adv, k_half;
-    int k, mn4;
+    int k, mn4, k_limit;
     bool valid;
     __device__ __forceinline__ void init(const SimtOperand<float>& op, int mn0, int k_begin, int t) {
         k = t >> 5;
         mn4 = (t & 31) * 4;
+        k_limit = op.extent_k;
         valid = mn0 + mn4 < op.extent_mn;  // extent % 4 == 0: all four or none
         p = op.ptr + (mn0 + mn4) + static_cast<long long>(k_begin + k) * op.stride_k;
         k_adv = kSimtBK * op.stride_k;
@@ -135,6 +140,7 @@ struct SimtLoader<float, kSimtVecMN> {
         if (!valid) p = op.ptr;  // never dereferenced (source size 0), but keep the address inside the tensor
     }
     __device__ __forceinline__ void fetch(int k0, int k_end, float (&)[kSimtLoads], float* tile) {
+        k_end = min(k_end, k_limit);
 #pragma unroll
         for (int i = 0; i < kSimtVecs; ++i) {
             const bool in = valid && k0 + k + i * (kSimtThreads / 32) < k_end;

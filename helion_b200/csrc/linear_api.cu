@@ -47,9 +47,10 @@ struct Operand {
 
 Operand plan_operand(const void* ptr, long long ld, long long rows, long long cols, int dtype, unsigned flags) {
     Operand o{ptr, ld, rows, cols, 0, 0};
-    const bool tc = dtype != LCE_DTYPE_F32 && !(flags & LCE_FLAG_FORCE_SIMT);
-    if (tc && !(aligned16(ptr) && ld % 8 == 0)) {  // TMA reads rows that start on 16-byte boundaries only
-        o.copy_ld = cdiv(cols, 8) * 8;
+    const long long vec = 16 / static_cast<long long>(elem_size(dtype));
+    const bool vectors = dtype == LCE_DTYPE_F32 || !(flags & LCE_FLAG_FORCE_SIMT);  // forced: element by element anyway
+    if (vectors && !(aligned16(ptr) && ld % vec == 0)) {
+        o.copy_ld = cdiv(cols, vec) * vec;
         o.copy_bytes = align_up(static_cast<size_t>(rows) * o.copy_ld * elem_size(dtype), 256);
     }
     return o;
@@ -65,7 +66,7 @@ int place_operand(Operand& o, char*& ws, cudaStream_t s) {
         static_cast<const T*>(o.ptr), o.ld, dst, o.copy_ld, o.rows, static_cast<int>(o.cols));
     LCE_COUNT_LAUNCH();
     o.ptr = dst;
-    o.ld = o.copy_ld;
+    o.ld = o.cols = o.copy_ld;
     return cuda_failed(cudaGetLastError()) ? LCE_ERR_CUDA : LCE_OK;
 }
 
@@ -121,7 +122,7 @@ int product(const DeviceInfo& d, const ProductPlan& p, const Operand& a, const O
         rc = launch_simt<T, Epi>(d, am, A_MN, bm, B_MN, M, N, K, epilogue_params<Epi>(p, tail, scratch), s, p.splits);
     }
     if (rc == LCE_OK && p.splits > 1) {
-        const long long quads = cdiv(N, 4) * M;
+        const long long quads = cdiv(N, 16) * cdiv(M, 16) * 64;
         const int blocks = static_cast<int>(cdiv(quads, 256) < 4096 ? cdiv(quads, 256) : 4096);
         const cudaError_t err = launch_dependent(linear_reduce_kernel<T>, blocks, 256, s, static_cast<const float*>(scratch),
                                                  p.splits, p.slab_floats, static_cast<int>(cdiv(N, p.bn)), p.bn, tail);
@@ -270,7 +271,7 @@ int linear_backward_impl(const DeviceInfo& d, BackwardPlan& b, const void* dy, l
             if (cuda_failed(err)) return LCE_ERR_CUDA;
         }
     }
-    const Operand z{b.copy_dz ? dz : dy, b.copy_dz ? b.ldz : ldy, M, N, 0, 0};
+    const Operand z{b.copy_dz ? dz : dy, b.copy_dz ? b.ldz : ldy, M, b.copy_dz ? b.ldz : N, 0, 0};
     LinearTail<T> tail = {};
     if (dx) {  // [M, K] = dz [M, N] W [N, K]
         tail.out = static_cast<T*>(dx);

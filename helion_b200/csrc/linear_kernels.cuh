@@ -490,18 +490,22 @@ struct EpiLinear {
     static __device__ __forceinline__ void end(State&, const Params&, const TileCtx&) {}
 };
 
-// Adds the slices of a split contraction in slice order and finishes the values. One thread = four columns of a row.
+// Adds the slices of a split contraction in slice order and finishes the values. One thread = four columns of a row; 64
+// threads take 16 rows (which lie side by side in a slab) of 4 such quads (side by side in the output).
 template <class T>
 __global__ void __launch_bounds__(256)
 linear_reduce_kernel(const float* scratch, int slices, long long slab_floats, int n_tiles, int bn, const LinearTail<T> t) {
     ptx::grid_dep_launch();
     ptx::grid_dep_wait();  // `scratch` holds the slices of the preceding GEMM
-    const long long quads_per_row = (static_cast<long long>(t.cols) + 3) / 4;
-    const long long total = quads_per_row * t.rows;
+    const long long groups_per_row = (static_cast<long long>(t.cols) + 15) / 16;
+    const long long total = groups_per_row * ((t.rows + 15ll) / 16) * 64;
     for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
          i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const int row = static_cast<int>(i / quads_per_row);
-        const int col = static_cast<int>(i - row * quads_per_row) * 4;
+        const long long group = i / 64, row_group = group / groups_per_row;
+        const int in_group = static_cast<int>(i & 63);
+        const int row = static_cast<int>(row_group) * 16 + (in_group & 15);
+        const int col = static_cast<int>(group - row_group * groups_per_row) * 16 + (in_group >> 4) * 4;
+        if (row >= t.rows || col >= t.cols) continue;
         const int n_tile = col / bn, c4 = (col - n_tile * bn) / 4, m_tile = row / kBM;
         const float4* sp = reinterpret_cast<const float4*>(scratch) +
                            ((static_cast<long long>(m_tile) * n_tiles + n_tile) * (bn / 4) + c4) * kBM + (row - m_tile * kBM);
@@ -736,13 +740,14 @@ linear_decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     }
 }
 
-// Rows copied to a pitch that TMA can read (a multiple of 16 bytes): operands whose rows start off 16-byte boundaries.
+// Rows copied to a pitch of whole 16-byte vectors, zeros behind the last column: operands whose rows start off 16-byte
+// boundaries, which TMA cannot read and the CUDA-core GEMM only element by element.
 template <class T>
 __global__ void __launch_bounds__(256)
 repitch_kernel(const T* __restrict__ src, long long lds, T* __restrict__ dst, long long ldd, long long rows, int cols) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (long long r = blockIdx.x * 8ll + warp; r < rows; r += gridDim.x * 8ll)
-        for (int c = lane; c < cols; c += 32) dst[r * ldd + c] = src[r * lds + c];
+        for (int c = lane; c < ldd; c += 32) dst[r * ldd + c] = c < cols ? src[r * lds + c] : Cvt<T>::from_f(0.f);
 }
 
 // dz = dy * act'(pre), rounded, and the column sums of the unrounded dz over this CTA's rows.
