@@ -26,6 +26,15 @@ bool head_rows_vectors(const lce_head_rows& r, const HeadCall& c, long long vec,
     return c.mode == kHeadRope || reinterpret_cast<uintptr_t>(r.weight) % bytes == 0;
 }
 
+// Whether the offsets within one token fit 32 bits.
+bool head_offsets_32(const lce_head_rows& r, const HeadCall& c) {
+    auto fits = [&](const int64_t* stride) {
+        const long long s = stride[2] < 0 ? -stride[2] : stride[2];
+        return s < (1ll << 31) && s * r.heads + c.dim < (1ll << 31);
+    };
+    return fits(r.x_stride) && fits(r.out_stride) && fits(r.grad_stride);
+}
+
 int check_head_rows(const lce_head_rows* r, const HeadCall& c) {
     if (!r || r->heads < 0) return LCE_ERR_ARG;
     if (r->heads > 0x7fffffll / 32) return LCE_ERR_TOO_LARGE;
@@ -83,32 +92,34 @@ int launch_heads(const HeadCall& c, const lce_head_rows& q, const lce_head_rows&
     const long long np = c.half / VEC, nv = c.dim / VEC;
     const int items = static_cast<int>(INTERLEAVED ? cdiv(nv, 2) : np + cdiv(nv - 2 * np, 2));
     const bool vector = c.dim % VEC == 0 && pair % VEC == 0 && items <= 32 && head_rows_vectors(q, c, VEC, 16) &&
-                        head_rows_vectors(k, c, VEC, 16);
+                        head_rows_vectors(k, c, VEC, 16) && head_offsets_32(q, c) && head_offsets_32(k, c);
     p.items = items;
     p.lanes = 1;
     while (p.lanes < items) p.lanes <<= 1;
     p.pairs2 = c.dim % 2 == 0 && head_rows_vectors(q, c, 2, 2 * sizeof(T)) && head_rows_vectors(k, c, 2, 2 * sizeof(T));
     const int per_step = vector ? 32 / p.lanes : 1;
-    const int warps = vector ? kHeadWarps : kRowFormWarps;
-    // The backward keeps sums over everything a warp walks, so its grid is what fits the GPU at once, shared between
-    // q and k by their numbers of heads; the others launch one warp per unit.
-    const long long all = q.heads + k.heads;
-    auto share = [&](long long heads) {
-        if (MODE != kHeadNormBackward) return 1ll << 20;
-        const long long fit = c.sm_count * (vector ? 2ll : 3ll);
-        const long long cap = (fit < kHeadMaxCtas ? fit : kHeadMaxCtas) * heads / (all > 0 ? all : 1);
+    using Shape = HeadShape<T, MODE>;
+    const int warps = vector ? Shape::kWarps : kRowFormWarps;
+    // The grid is what fits the GPU at once: a warp then walks many tokens, which spreads its set-up, and in the backward
+    // its sums. q and k share it by their steps, a token's angles counting as two (they take as many instructions).
+    const long long steps_q = q.heads > 0 ? cdiv(q.heads, per_step) + 2 : 0, steps_k = k.heads > 0 ? cdiv(k.heads, per_step) + 2 : 0;
+    auto share = [&](long long steps) {
+        // rotations alone, and fp32 norms, keep up without and are 4 % faster dealt out by the hardware, a token to a warp
+        if (MODE == kHeadRope || (MODE == kHeadNorm && sizeof(T) == 4)) return 1ll << 20;
+        const long long fit = c.sm_count * (vector ? static_cast<long long>(Shape::kCtas) : 3ll);
+        const long long cap = (fit < kHeadMaxCtas ? fit : kHeadMaxCtas) * steps / (steps_q + steps_k > 0 ? steps_q + steps_k : 1);
         return cap < 1 ? 1ll : cap;
     };
-    HeadRows<T> hq = deal_heads<T>(q, c, per_step, warps, share(q.heads));
-    HeadRows<T> hk = deal_heads<T>(k, c, per_step, warps, share(k.heads));
+    HeadRows<T> hq = deal_heads<T>(q, c, per_step, warps, share(steps_q));
+    HeadRows<T> hk = deal_heads<T>(k, c, per_step, warps, share(steps_k));
     if (MODE == kHeadNormBackward) {
         if (q.dweight) hq.partial = partial;
         if (k.dweight) hk.partial = partial + static_cast<long long>(hq.ctas) * c.dim;
     }
     if (hq.ctas + hk.ctas > 0) {
         if (vector) {
-            const int smem = kHeadWarps * items * VEC * static_cast<int>(sizeof(float2));
-            heads_vector_kernel<T, INTERLEAVED, MODE><<<hq.ctas + hk.ctas, kHeadThreads, smem, s>>>(hq, hk, p);
+            const int smem = Shape::kWarps * items * VEC * static_cast<int>(sizeof(float2));
+            heads_vector_kernel<T, INTERLEAVED, MODE><<<hq.ctas + hk.ctas, Shape::kThreads, smem, s>>>(hq, hk, p);
         } else {
             const int smem = kRowFormWarps * row_form_floats(p.dim, p.half, MODE) * 4;
             auto kern = heads_row_kernel<T, INTERLEAVED, MODE>;
@@ -159,7 +170,8 @@ int heads_call(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, in
                int pos_i64, int64_t pos_b, int64_t pos_s, const double* freq, int64_t half, int interleaved, float scale,
                int inverse, float eps, int dtype, void* ws, size_t ws_bytes, void* stream) {
     if (!known_dtype(dtype) || batch < 0 || seq < 0 || dim < 1 || half < 0 || 2 * half > dim) return LCE_ERR_ARG;
-    if (dim > kHeadMaxDim || batch > 0x7fffffffll || seq > 0x7fffffffll || batch * seq > (1ll << 40)) return LCE_ERR_TOO_LARGE;
+    // a grid's stride over 2^31 units must not wrap 32 bits
+    if (dim > kHeadMaxDim || batch > 0x7fffffffll || seq > 0x7fffffffll || batch * seq > 0x70000000ll) return LCE_ERR_TOO_LARGE;
     HeadCall c{batch, seq, dim, half, interleaved, MODE, dtype, 0};
     int rc = check_head_rows(q, c);
     if (rc) return rc;

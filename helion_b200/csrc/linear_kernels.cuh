@@ -32,26 +32,6 @@ constexpr float kGeluA = 0.044715f;
 // has to be done in 8000 cycles of its four schedulers. The normal distribution is
 //   F(-a) = exp(-a^2 / 2) g(a),  g a polynomial in 1 / (1 + 0.26 a)
 // fitted here by reweighted least squares to 3.4e-7 of g for a up to 14 (with the exponential 2e-6 up to a = 6).
-struct Pair {
-    unsigned long long v;
-};
-__device__ __forceinline__ Pair pair(float lo, float hi) {
-    Pair p;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
-    return p;
-}
-__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
-__device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v)); }
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return d;
-}
 __device__ __forceinline__ float fast_reciprocal(float x) {
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

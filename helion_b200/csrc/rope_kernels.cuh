@@ -30,8 +30,6 @@
 
 namespace lce {
 
-constexpr int kHeadThreads = 256;
-constexpr int kHeadWarps = kHeadThreads / 32;
 constexpr int kHeadMaxCtas = 592;   // backward CTAs in all = partial dweight rows (4 per SM on 148 SMs)
 constexpr int kHeadMaxDim = 1024;
 constexpr int kRowFormWarps = 4;
@@ -53,7 +51,7 @@ struct HeadRows {
     int heads;
     int chunks;       // warps that share one token
     int steps;        // steps (of 32 / lanes heads; one head in the row form) per warp
-    long long units;  // tokens * chunks
+    long long units;  // tokens * chunks, below 2^31
     int ctas;
 };
 
@@ -95,47 +93,73 @@ __device__ __forceinline__ float head_rstd(float sum, float inv_dim, float eps) 
     return (a > 0.f && a < INFINITY) ? y * fmaf(-0.5f * a * y, y, 1.5f) : y;
 }
 
-// A lane's two vectors turned by the angles cs / sn (VEC of them). rot0 / rot1: whether the vector is inside the
-// rotated part at all (the half layout pairs vectors that are both inside or both outside).
-template <class T, bool INTERLEAVED, int VEC = RmsTile<T>::kVec>
-__device__ __forceinline__ void rope_turn(float (&a)[VEC], float (&b)[VEC], const float (&cs)[VEC], const float (&sn)[VEC],
-                                          bool rot0, bool rot1) {
+// A lane's two vectors, rotated. The half layout pairs element j of the first with element j of the second; interleaved,
+// neighbours of one vector pair up. Coefficients come in the same places either way:
+//   half          y0 = x0 c0 + x1 s0,           y1 = x1 c1 + x0 s1
+//   interleaved   y0 = x0 c0 + swapped(x0) s0,  y1 = x1 c1 + swapped(x1) s1
+// rot0 / rot1: whether the vector is inside the rotated part at all; outside, y = x c, and the other vector, whatever it
+// holds, has no say.
+// SAME (half layout): s0 is -s1 and not read.
+template <bool INTERLEAVED, bool SAME, int N>
+__device__ __forceinline__ void rope_turn(Pair (&x0)[N], Pair (&x1)[N], const Pair (&c0)[N], const Pair (&s0)[N],
+                                          const Pair (&c1)[N], const Pair (&s1)[N], bool rot0, bool rot1) {
     if constexpr (INTERLEAVED) {
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
-            if (rot0) {
-                const float x = a[2 * j], y = a[2 * j + 1];
-                a[2 * j] = x * cs[j] - y * sn[j];
-                a[2 * j + 1] = y * cs[j] + x * sn[j];
-            }
-            if (rot1) {
-                const float x = b[2 * j], y = b[2 * j + 1];
-                b[2 * j] = x * cs[VEC / 2 + j] - y * sn[VEC / 2 + j];
-                b[2 * j + 1] = y * cs[VEC / 2 + j] + x * sn[VEC / 2 + j];
-            }
+        for (int j = 0; j < N; ++j) {
+            x0[j] = rot0 ? fma2(swapped(x0[j]), s0[j], x0[j] * c0[j]) : x0[j] * c0[j];
+            x1[j] = rot1 ? fma2(swapped(x1[j]), s1[j], x1[j] * c1[j]) : x1[j] * c1[j];
         }
     } else if (rot0) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float x = a[j], y = b[j];
-            a[j] = x * cs[j] - y * sn[j];
-            b[j] = y * cs[j] + x * sn[j];
+        for (int j = 0; j < N; ++j) {
+            const Pair a = x0[j], b = x1[j];
+            const Pair ac = a * c0[j];
+            x1[j] = fma2(a, s1[j], b * c1[j]);
+            if constexpr (SAME) {  // two instructions, but no registers for -s
+                float b0, b1, n0, n1, t0, t1;
+                split(b, b0, b1);
+                split(s1[j], n0, n1);
+                split(ac, t0, t1);
+                x0[j] = pair(fmaf(-b0, n0, t0), fmaf(-b1, n1, t1));
+            } else {
+                x0[j] = fma2(b, s0[j], ac);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            x0[j] = x0[j] * c0[j];
+            x1[j] = x1[j] * c1[j];
         }
     }
 }
 
+// Threads of a CTA, CTAs per SM and steps whose loads are in flight while one is worked on. Registers are what limits
+// them (a 16-bit step works on 16 elements a lane, an fp32 one on 8); measured at 16384 tokens of 32 + 8 heads of 128:
+// the 16-bit norm 71 us on 2 x 256 threads, 76 on 3 (the registers spill); its backward 111 us on 384, 122 on 2 x 256;
+// fp32 at 8192 tokens 62 us on 3 x 256, 68 on 2, the backward 93 on 2 x 256, 101 on 384.
+template <class T, int MODE>
+struct HeadShape {
+    static constexpr bool kWide = sizeof(T) == 2;
+    static constexpr int kThreads = MODE == kHeadNormBackward && kWide ? 384 : 256;
+    static constexpr int kWarps = kThreads / 32;
+    static constexpr int kCtas = MODE == kHeadNormBackward ? (kWide ? 1 : 2) : (MODE == kHeadNorm && kWide ? 2 : 3);
+    static constexpr int kAhead = 2;
+};
+
 template <class T, bool INTERLEAVED, int MODE>
-__global__ void __launch_bounds__(kHeadThreads, MODE == kHeadNormBackward ? 2 : 3)
+__global__ void __launch_bounds__(HeadShape<T, MODE>::kThreads, HeadShape<T, MODE>::kCtas)
 heads_vector_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const RopePlan p) {
-    constexpr int VEC = RmsTile<T>::kVec;
-    constexpr int U = 2;  // steps whose loads are in flight together
+    constexpr int VEC = RmsTile<T>::kVec, N = VEC / 2;
+    constexpr int U = HeadShape<T, MODE>::kAhead, kWarps = HeadShape<T, MODE>::kWarps;
     extern __shared__ __align__(16) unsigned char head_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool second = static_cast<int>(blockIdx.x) >= rows_q.ctas;
     const HeadRows<T>& h = second ? rows_k : rows_q;
     const int cta = static_cast<int>(blockIdx.x) - (second ? rows_q.ctas : 0);
     const int table_len = p.items * VEC;
-    float2* table = reinterpret_cast<float2*>(head_smem) + warp * table_len;
+    float* cos_table = reinterpret_cast<float*>(head_smem) + warp * 2 * table_len;
+    float* sin_table = cos_table + table_len;
 
     const int it = lane & (p.lanes - 1), sub = lane / p.lanes, per_step = 32 / p.lanes;
     const bool on = it < p.items;
@@ -161,110 +185,151 @@ heads_vector_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const Ro
         if (on0) w0 = *reinterpret_cast<const uint4*>(h.weight + col0);
         if (on1) w1 = *reinterpret_cast<const uint4*>(h.weight + col1);
     }
-    float acc0[VEC], acc1[VEC];  // dweight of this lane's columns
+    Pair acc0[N], acc1[N];  // dweight of this lane's columns
     if constexpr (MODE == kHeadNormBackward) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc0[j] = acc1[j] = 0.f;
+        for (int j = 0; j < N; ++j) acc0[j] = acc1[j] = both(0.f);
     }
 
+    // Within a token offsets take 32 bits (the host sees to it), and so do the units.
     const int total_steps = (h.heads + per_step - 1) / per_step;
-    const long long unit_step = static_cast<long long>(h.ctas) * kHeadWarps;
-    for (long long u = static_cast<long long>(cta) * kHeadWarps + warp; u < h.units; u += unit_step) {
-        const long long token = u / h.chunks;
-        const int step0 = static_cast<int>(u - token * h.chunks) * h.steps;
+    const int x_h = static_cast<int>(h.x_h), dy_h = static_cast<int>(h.dy_h), o_h = static_cast<int>(h.o_h);
+    const unsigned units = static_cast<unsigned>(h.units), seq = static_cast<unsigned>(p.seq), chunks = h.chunks;
+    const unsigned unit_step = static_cast<unsigned>(h.ctas) * kWarps;
+    uint4 x0[U], x1[U], d0[U], d1[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) x0[i] = x1[i] = d0[i] = d1[i] = zero;  // and so they stay in lanes without columns
+    for (unsigned u = cta * kWarps + warp; u < units; u += unit_step) {
+        const unsigned token = chunks == 1 ? u : u / chunks;
+        const int step0 = static_cast<int>(u - token * chunks) * h.steps;
         const int step1 = min(step0 + h.steps, total_steps);
-        const long long b = token / p.seq, s = token - b * p.seq;
+        const unsigned b = token / seq, s = token - b * seq;
         const T* x = h.x + b * h.x_b + s * h.x_s;
         const T* dy = MODE == kHeadNormBackward ? h.dy + b * h.dy_b + s * h.dy_s : nullptr;
         T* out = h.out + b * h.o_b + s * h.o_s;
 
-        uint4 x0[U], x1[U], d0[U], d1[U];
-        auto fetch = [&](int step) {
-#pragma unroll
-            for (int i = 0; i < U; ++i) {
-                const int head = (step + i) * per_step + sub;
-                const bool in = step + i < step1 && head < h.heads;
-                x0[i] = in && on0 ? *reinterpret_cast<const uint4*>(x + head * h.x_h + col0) : zero;
-                x1[i] = in && on1 ? *reinterpret_cast<const uint4*>(x + head * h.x_h + col1) : zero;
-                if constexpr (MODE == kHeadNormBackward) {
-                    d0[i] = in && on0 ? *reinterpret_cast<const uint4*>(dy + head * h.dy_h + col0) : zero;
-                    d1[i] = in && on1 ? *reinterpret_cast<const uint4*>(dy + head * h.dy_h + col1) : zero;
-                }
+        auto fetch = [&](int i, int step) {
+            if (step >= step1) return;  // the same for the warp
+            const int head = min(step * per_step + sub, h.heads - 1);  // a row that is not there: the last, and not stored
+            const int at = head * x_h;
+            if (on0) x0[i] = *reinterpret_cast<const uint4*>(x + (at + col0));
+            if (on1) x1[i] = *reinterpret_cast<const uint4*>(x + (at + col1));
+            if constexpr (MODE == kHeadNormBackward) {
+                const int dat = head * dy_h;
+                if (on0) d0[i] = *reinterpret_cast<const uint4*>(dy + (dat + col0));
+                if (on1) d1[i] = *reinterpret_cast<const uint4*>(dy + (dat + col1));
             }
         };
-        fetch(step0);  // in flight while the angles are formed
+#pragma unroll
+        for (int i = 0; i < U; ++i) fetch(i, step0 + i);  // in flight while the angles are formed
 
         const double pos = rope_position(p, b, s);
         __syncwarp();  // the previous token's table has been read
-        for (int i = lane; i < table_len; i += 32)
-            table[i] = i < p.half ? rope_angle(pos, p.freq[i], p.scale, p.sin_sign) : make_float2(1.f, 0.f);
+        for (int i = lane; i < table_len; i += 32) {
+            const float2 t = i < p.half ? rope_angle(pos, p.freq[i], p.scale, p.sin_sign) : make_float2(1.f, 0.f);
+            cos_table[i] = t.x;
+            sin_table[i] = t.y;
+        }
         __syncwarp();
-        float cs[VEC], sn[VEC];
+        Pair c0[N], s0[N], c1[N], s1[N];
+        {
+            float c[VEC], n[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float2 t = table[on ? it * VEC + j : j];
-            cs[j] = t.x;
-            sn[j] = t.y;
+            for (int j = 0; j < VEC; j += 4) {  // 16-byte aligned: table_len and it * VEC are whole vectors
+                *reinterpret_cast<float4*>(c + j) = *reinterpret_cast<const float4*>(cos_table + (on ? it * VEC : 0) + j);
+                *reinterpret_cast<float4*>(n + j) = *reinterpret_cast<const float4*>(sin_table + (on ? it * VEC : 0) + j);
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if constexpr (INTERLEAVED) {
+                    c0[j] = both(c[j]);
+                    c1[j] = both(c[N + j]);
+                    s0[j] = pair(-n[j], n[j]);
+                    s1[j] = pair(-n[N + j], n[N + j]);
+                } else {
+                    c0[j] = c1[j] = pair(c[2 * j], c[2 * j + 1]);
+                    s0[j] = pair(-n[2 * j], -n[2 * j + 1]);
+                    s1[j] = pair(n[2 * j], n[2 * j + 1]);
+                }
+            }
+        }
+        if constexpr (MODE == kHeadNorm) {  // the weights ride on the coefficients
+            Pair v0[N], v1[N];
+            unpack_pairs<T>(w0, v0);
+            unpack_pairs<T>(w1, v1);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                c0[j] = c0[j] * v0[j];
+                c1[j] = c1[j] * v1[j];
+                s0[j] = s0[j] * (INTERLEAVED ? swapped(v0[j]) : v1[j]);
+                s1[j] = s1[j] * (INTERLEAVED ? swapped(v1[j]) : v0[j]);
+            }
         }
 
         for (int step = step0; step < step1; step += U) {
-            if (step != step0) fetch(step);
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 const int head = (step + i) * per_step + sub;
                 const bool in = step + i < step1 && head < h.heads;
-                float a[VEC], c[VEC];
-                rms_unpack<T>(x0[i], a);
-                rms_unpack<T>(x1[i], c);
+                Pair a[N], c[N], g0[N], g1[N];
+                unpack_pairs<T>(x0[i], a);
+                unpack_pairs<T>(x1[i], c);
+                if constexpr (MODE == kHeadNormBackward) {
+                    unpack_pairs<T>(d0[i], g0);
+                    unpack_pairs<T>(d1[i], g1);
+                }
+                fetch(i, step + i + U);
                 if constexpr (MODE == kHeadRope) {
-                    rope_turn<T, INTERLEAVED>(a, c, cs, sn, rot0, rot1);
+                    rope_turn<INTERLEAVED, MODE == kHeadRope>(a, c, c0, s0, c1, s1, rot0, rot1);
                 } else {
-                    float v0[VEC], v1[VEC];
-                    rms_unpack<T>(w0, v0);
-                    rms_unpack<T>(w1, v1);
-                    float ss = 0.f;
+                    Pair squares = both(0.f);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) ss = fmaf(a[j], a[j], fmaf(c[j], c[j], ss));
+                    for (int j = 0; j < N; ++j) squares = fma2(a[j], a[j], fma2(c[j], c[j], squares));
+                    float ss = sum(squares);
                     if constexpr (MODE == kHeadNorm) {
                         for (int o = p.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                        const float rstd = head_rstd(ss, inv_dim, p.eps);
+                        const Pair rstd = both(head_rstd(ss, inv_dim, p.eps));
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            a[j] = a[j] * rstd * v0[j];
-                            c[j] = c[j] * rstd * v1[j];
+                        for (int j = 0; j < N; ++j) {
+                            a[j] = a[j] * rstd;
+                            c[j] = c[j] * rstd;
                         }
-                        rope_turn<T, INTERLEAVED>(a, c, cs, sn, rot0, rot1);
+                        rope_turn<INTERLEAVED, MODE == kHeadRope>(a, c, c0, s0, c1, s1, rot0, rot1);
                     } else {
-                        float g0[VEC], g1[VEC];
-                        rms_unpack<T>(d0[i], g0);
-                        rms_unpack<T>(d1[i], g1);
-                        rope_turn<T, INTERLEAVED>(g0, g1, cs, sn, rot0, rot1);
-                        float dot = 0.f;
+                        Pair v0[N], v1[N];
+                        rope_turn<INTERLEAVED, true>(g0, g1, c0, s0, c1, s1, rot0, rot1);
+                        unpack_pairs<T>(w0, v0);
+                        unpack_pairs<T>(w1, v1);
+                        Pair dots = both(0.f);
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            v0[j] *= g0[j];
-                            v1[j] *= g1[j];
-                            dot = fmaf(v0[j], a[j], fmaf(v1[j], c[j], dot));
+                        for (int j = 0; j < N; ++j) {
+                            v0[j] = v0[j] * g0[j];
+                            v1[j] = v1[j] * g1[j];
+                            dots = fma2(v0[j], a[j], fma2(v1[j], c[j], dots));
                         }
+                        float dot = sum(dots);
                         for (int o = p.lanes >> 1; o > 0; o >>= 1) {
                             ss += __shfl_xor_sync(0xffffffffu, ss, o);
                             dot += __shfl_xor_sync(0xffffffffu, dot, o);
                         }
-                        const float rstd = head_rstd(ss, inv_dim, p.eps);
-                        const float k = rstd * rstd * dot * inv_dim;
+                        const float r = head_rstd(ss, inv_dim, p.eps);
+                        const Pair rstd = both(r), k = both(-r * r * dot * inv_dim);  // dx = rstd (g w + k x^)
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            if (in) {  // a row that is not there adds nothing, whatever 1 / sqrt(eps) is
-                                acc0[j] = fmaf(g0[j], a[j] * rstd, acc0[j]);
-                                acc1[j] = fmaf(g1[j], c[j] * rstd, acc1[j]);
+                        for (int j = 0; j < N; ++j) {
+                            a[j] = a[j] * rstd;
+                            c[j] = c[j] * rstd;
+                            if (in) {
+                                acc0[j] = fma2(g0[j], a[j], acc0[j]);
+                                acc1[j] = fma2(g1[j], c[j], acc1[j]);
                             }
-                            a[j] = rstd * (v0[j] - a[j] * k);
-                            c[j] = rstd * (v1[j] - c[j] * k);
+                            a[j] = fma2(a[j], k, v0[j] * rstd);
+                            c[j] = fma2(c[j], k, v1[j] * rstd);
                         }
                     }
                 }
-                if (in && on0) *reinterpret_cast<uint4*>(out + head * h.o_h + col0) = rms_pack<T>(a);
-                if (in && on1) *reinterpret_cast<uint4*>(out + head * h.o_h + col1) = rms_pack<T>(c);
+                const int oat = head * o_h;
+                if (in && on0) *reinterpret_cast<uint4*>(out + (oat + col0)) = pack_pairs<T>(a);
+                if (in && on1) *reinterpret_cast<uint4*>(out + (oat + col1)) = pack_pairs<T>(c);
             }
         }
     }
@@ -272,11 +337,17 @@ heads_vector_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const Ro
     if constexpr (MODE == kHeadNormBackward) {
         if (h.partial == nullptr) return;  // the same for the whole CTA
         // lanes that hold the same columns first (a fixed butterfly), then the warps in order
+        float sum0[VEC], sum1[VEC];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            split(acc0[j], sum0[2 * j], sum0[2 * j + 1]);
+            split(acc1[j], sum1[2 * j], sum1[2 * j + 1]);
+        }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             for (int o = p.lanes; o < 32; o <<= 1) {
-                acc0[j] += __shfl_xor_sync(0xffffffffu, acc0[j], o);
-                acc1[j] += __shfl_xor_sync(0xffffffffu, acc1[j], o);
+                sum0[j] += __shfl_xor_sync(0xffffffffu, sum0[j], o);
+                sum1[j] += __shfl_xor_sync(0xffffffffu, sum1[j], o);
             }
         }
         __syncthreads();  // the tables are no longer needed: their space holds the warps' sums, [warps][dim]
@@ -284,15 +355,15 @@ heads_vector_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const Ro
         if (sub == 0) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                if (on0) sums[warp * p.dim + col0 + j] = acc0[j];
-                if (on1) sums[warp * p.dim + col1 + j] = acc1[j];
+                if (on0) sums[warp * p.dim + col0 + j] = sum0[j];
+                if (on1) sums[warp * p.dim + col1 + j] = sum1[j];
             }
         }
         __syncthreads();
-        for (int d = threadIdx.x; d < p.dim; d += kHeadThreads) {
+        for (int d = threadIdx.x; d < p.dim; d += kWarps * 32) {
             float t = 0.f;
 #pragma unroll
-            for (int k = 0; k < kHeadWarps; ++k) t += sums[k * p.dim + d];
+            for (int k = 0; k < kWarps; ++k) t += sums[k * p.dim + d];
             h.partial[static_cast<long long>(cta) * p.dim + d] = t;
         }
     }
@@ -357,12 +428,13 @@ heads_row_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const RopeP
         }
     };
 
-    const long long unit_step = static_cast<long long>(h.ctas) * kRowFormWarps;
-    for (long long u = static_cast<long long>(cta) * kRowFormWarps + warp; u < h.units; u += unit_step) {
-        const long long token = u / h.chunks;
-        const int head0 = static_cast<int>(u - token * h.chunks) * h.steps;
+    const unsigned units = static_cast<unsigned>(h.units), seq = static_cast<unsigned>(p.seq), chunks = h.chunks;
+    const unsigned unit_step = static_cast<unsigned>(h.ctas) * kRowFormWarps;
+    for (unsigned u = cta * kRowFormWarps + warp; u < units; u += unit_step) {
+        const unsigned token = u / chunks;
+        const int head0 = static_cast<int>(u - token * chunks) * h.steps;
         const int head1 = min(head0 + h.steps, h.heads);
-        const long long b = token / p.seq, s = token - b * p.seq;
+        const unsigned b = token / seq, s = token - b * seq;
         const T* x = h.x + b * h.x_b + s * h.x_s;
         const T* dy = MODE == kHeadNormBackward ? h.dy + b * h.dy_b + s * h.dy_s : nullptr;
         T* out = h.out + b * h.o_b + s * h.o_s;

@@ -103,4 +103,56 @@ __device__ __forceinline__ void rms_store(T* __restrict__ row, int c, int H, con
     }
 }
 
+// Two fp32 values that share an instruction where the hardware has one (multiply, add and fused multiply-add).
+struct Pair {
+    unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+__device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v)); }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ Pair swapped(Pair p) {
+    float lo, hi;
+    split(p, lo, hi);
+    return pair(hi, lo);
+}
+__device__ __forceinline__ float sum(Pair p) {
+    float lo, hi;
+    split(p, lo, hi);
+    return lo + hi;
+}
+
+template <class T>
+__device__ __forceinline__ void unpack_pairs(const uint4& raw, Pair (&v)[RmsTile<T>::kVec / 2]) {
+    float f[RmsTile<T>::kVec];
+    rms_unpack<T>(raw, f);
+#pragma unroll
+    for (int j = 0; j < RmsTile<T>::kVec / 2; ++j) v[j] = pair(f[2 * j], f[2 * j + 1]);
+}
+template <class T>
+__device__ __forceinline__ uint4 pack_pairs(const Pair (&v)[RmsTile<T>::kVec / 2]) {
+    float f[RmsTile<T>::kVec];
+#pragma unroll
+    for (int j = 0; j < RmsTile<T>::kVec / 2; ++j) split(v[j], f[2 * j], f[2 * j + 1]);
+    return rms_pack<T>(f);
+}
+
 }  // namespace lce
