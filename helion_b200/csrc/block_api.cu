@@ -54,9 +54,9 @@ lce_head_rows plain_strides(lce_head_rows r, const HeadCall& c) {
 }
 
 // Deals `tokens` x `heads` rows to warps: whole tokens per warp (their angles are formed once) as long as that gives
-// every SM `kWarps` warps, pieces of a token otherwise. A step is `per_step` heads.
+// every SM `kWarps` warps, pieces of a token otherwise. `total_steps`: of a token.
 template <class T>
-HeadRows<T> deal_heads(const lce_head_rows& r, const HeadCall& c, int per_step, int warps_per_cta, long long max_ctas) {
+HeadRows<T> deal_heads(const lce_head_rows& r, const HeadCall& c, long long total_steps, int warps_per_cta, long long max_ctas) {
     HeadRows<T> h;
     h.x = static_cast<const T*>(r.x);
     h.x_b = r.x_stride[0], h.x_s = r.x_stride[1], h.x_h = r.x_stride[2];
@@ -67,7 +67,7 @@ HeadRows<T> deal_heads(const lce_head_rows& r, const HeadCall& c, int per_step, 
     h.weight = static_cast<const T*>(r.weight);
     h.partial = nullptr;
     h.heads = static_cast<int>(r.heads);
-    const long long tokens = c.batch * c.seq, total_steps = cdiv(r.heads, per_step);
+    const long long tokens = c.batch * c.seq;
     if (tokens == 0 || total_steps == 0) {
         h.chunks = h.steps = 1;
         h.units = 0;
@@ -101,18 +101,23 @@ int launch_heads(const HeadCall& c, const lce_head_rows& q, const lce_head_rows&
     using Shape = HeadShape<T, MODE>;
     const int warps = vector ? Shape::kWarps : kRowFormWarps;
     // The grid is what fits the GPU at once: a warp then walks many tokens, which spreads its set-up, and in the backward
-    // its sums. q and k share it by their steps, a token's angles counting as two (they take as many instructions).
-    const long long steps_q = q.heads > 0 ? cdiv(q.heads, per_step) + 2 : 0, steps_k = k.heads > 0 ? cdiv(k.heads, per_step) + 2 : 0;
-    auto share = [&](long long steps) {
+    // its sums. Where q and k have CTAs of their own they share the grid by their steps, a token's set-up counting as two.
+    const long long steps_q = cdiv(q.heads, per_step), steps_k = cdiv(k.heads, per_step);
+    const long long cost_q = steps_q > 0 ? steps_q + 2 : 0, cost_k = steps_k > 0 ? steps_k + 2 : 0;
+    const bool together = vector && MODE != kHeadNormBackward;
+    auto share = [&](long long cost) {
         // rotations alone, and fp32 norms, keep up without and are 4 % faster dealt out by the hardware, a token to a warp
         if (MODE == kHeadRope || (MODE == kHeadNorm && sizeof(T) == 4)) return 1ll << 20;
         const long long fit = c.sm_count * (vector ? static_cast<long long>(Shape::kCtas) : 3ll);
-        const long long cap = (fit < kHeadMaxCtas ? fit : kHeadMaxCtas) * steps / (steps_q + steps_k > 0 ? steps_q + steps_k : 1);
+        if (together) return fit;
+        const long long cap = (fit < kHeadMaxCtas ? fit : kHeadMaxCtas) * cost / (cost_q + cost_k > 0 ? cost_q + cost_k : 1);
         return cap < 1 ? 1ll : cap;
     };
-    HeadRows<T> hq = deal_heads<T>(q, c, per_step, warps, share(steps_q));
-    HeadRows<T> hk = deal_heads<T>(k, c, per_step, warps, share(steps_k));
+    HeadRows<T> hq = deal_heads<T>(q, c, together ? steps_q + steps_k : steps_q, warps, share(cost_q));
+    HeadRows<T> hk = deal_heads<T>(k, c, together ? 0 : steps_k, warps, share(cost_k));
     if (MODE == kHeadNormBackward) {
+        // the partial rows have to fit the workspace, whatever the split above comes to
+        if (hq.ctas + hk.ctas > kHeadMaxCtas + 1) return LCE_ERR_WS_TOO_SMALL;
         if (q.dweight) hq.partial = partial;
         if (k.dweight) hk.partial = partial + static_cast<long long>(hq.ctas) * c.dim;
     }

@@ -71,14 +71,24 @@ struct RopePlan {
     float eps;
 };
 
-// cos and sin of position * frequency, times scale: the product in turns and its fraction in 64 bits.
-__device__ __forceinline__ float2 rope_angle(double pos, double freq, float scale, float sin_sign) {
-    double turns = pos * (freq * 0.15915494309189533577);  // 1 / (2 pi)
+// cos and sin of an angle given as position x turns per position, times scale: the product and its fraction in 64 bits.
+// For 16-bit results the hardware's sine and cosine do (within 4e-7 for an angle in [-pi, pi]); they save most of a
+// token's set-up.
+template <bool FAST>
+__device__ __forceinline__ float2 rope_angle(double pos, double turns_per_position, float scale, float sin_sign) {
+    double turns = pos * turns_per_position;
     turns -= rint(turns);
     float s, c;
-    sincospif(2.f * static_cast<float>(turns), &s, &c);
+    if constexpr (FAST) {
+        const float radians = 6.283185307179586f * static_cast<float>(turns);
+        s = __sinf(radians);
+        c = __cosf(radians);
+    } else {
+        sincospif(2.f * static_cast<float>(turns), &s, &c);
+    }
     return make_float2(c * scale, s * scale * sin_sign);
 }
+constexpr double kTurnsPerRadian = 0.15915494309189533577;  // 1 / (2 pi)
 
 __device__ __forceinline__ double rope_position(const RopePlan& p, long long b, long long s) {
     const long long i = b * p.pos_b + s * p.pos_s;
@@ -93,43 +103,33 @@ __device__ __forceinline__ float head_rstd(float sum, float inv_dim, float eps) 
     return (a > 0.f && a < INFINITY) ? y * fmaf(-0.5f * a * y, y, 1.5f) : y;
 }
 
-// A lane's two vectors, rotated. The half layout pairs element j of the first with element j of the second; interleaved,
-// neighbours of one vector pair up. Coefficients come in the same places either way:
-//   half          y0 = x0 c0 + x1 s0,           y1 = x1 c1 + x0 s1
-//   interleaved   y0 = x0 c0 + swapped(x0) s0,  y1 = x1 c1 + swapped(x1) s1
-// rot0 / rot1: whether the vector is inside the rotated part at all; outside, y = x c, and the other vector, whatever it
-// holds, has no say.
-// SAME (half layout): s0 is -s1 and not read.
-template <bool INTERLEAVED, bool SAME, int N>
-__device__ __forceinline__ void rope_turn(Pair (&x0)[N], Pair (&x1)[N], const Pair (&c0)[N], const Pair (&s0)[N],
-                                          const Pair (&c1)[N], const Pair (&s1)[N], bool rot0, bool rot1) {
+// A lane's two vectors, rotated by the angles whose cosines and sines are c and n. The half layout pairs element j of the
+// first with element j of the second; interleaved, neighbours of one vector pair up (the first vector takes the first half
+// of the angles). rot0 / rot1: whether the vector is inside the rotated part at all; outside it stays as it is.
+template <bool INTERLEAVED, int N>
+__device__ __forceinline__ void rope_turn(Pair (&x0)[N], Pair (&x1)[N], const float (&c)[2 * N], const float (&n)[2 * N], bool rot0, bool rot1) {
     if constexpr (INTERLEAVED) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            x0[j] = rot0 ? fma2(swapped(x0[j]), s0[j], x0[j] * c0[j]) : x0[j] * c0[j];
-            x1[j] = rot1 ? fma2(swapped(x1[j]), s1[j], x1[j] * c1[j]) : x1[j] * c1[j];
+            float x, y;
+            if (rot0) {
+                split(x0[j], x, y);
+                x0[j] = pair(fmaf(-y, n[j], x * c[j]), fmaf(x, n[j], y * c[j]));
+            }
+            if (rot1) {
+                split(x1[j], x, y);
+                x1[j] = pair(fmaf(-y, n[N + j], x * c[N + j]), fmaf(x, n[N + j], y * c[N + j]));
+            }
         }
     } else if (rot0) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const Pair a = x0[j], b = x1[j];
-            const Pair ac = a * c0[j];
-            x1[j] = fma2(a, s1[j], b * c1[j]);
-            if constexpr (SAME) {  // two instructions, but no registers for -s
-                float b0, b1, n0, n1, t0, t1;
-                split(b, b0, b1);
-                split(s1[j], n0, n1);
-                split(ac, t0, t1);
-                x0[j] = pair(fmaf(-b0, n0, t0), fmaf(-b1, n1, t1));
-            } else {
-                x0[j] = fma2(b, s0[j], ac);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            x0[j] = x0[j] * c0[j];
-            x1[j] = x1[j] * c1[j];
+            const Pair a = x0[j], cs = pair(c[2 * j], c[2 * j + 1]), sn = pair(n[2 * j], n[2 * j + 1]);
+            float b0, b1, t0, t1;
+            split(x1[j], b0, b1);
+            split(a * cs, t0, t1);
+            x1[j] = fma2(a, sn, x1[j] * cs);
+            x0[j] = pair(fmaf(-b0, n[2 * j], t0), fmaf(-b1, n[2 * j + 1], t1));  // a pair would need registers for -n
         }
     }
 }
@@ -147,14 +147,17 @@ struct HeadShape {
     static constexpr int kAhead = 2;
 };
 
+// The backward's CTAs belong to q or to k, whose sums they keep; otherwise a unit of work is a token, or a piece of one,
+// with its query heads first and then its key heads.
 template <class T, bool INTERLEAVED, int MODE>
 __global__ void __launch_bounds__(HeadShape<T, MODE>::kThreads, HeadShape<T, MODE>::kCtas)
 heads_vector_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const RopePlan p) {
     constexpr int VEC = RmsTile<T>::kVec, N = VEC / 2;
     constexpr int U = HeadShape<T, MODE>::kAhead, kWarps = HeadShape<T, MODE>::kWarps;
+    constexpr bool kBackward = MODE == kHeadNormBackward;
     extern __shared__ __align__(16) unsigned char head_smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool second = static_cast<int>(blockIdx.x) >= rows_q.ctas;
+    const bool second = kBackward && static_cast<int>(blockIdx.x) >= rows_q.ctas;
     const HeadRows<T>& h = second ? rows_k : rows_q;
     const int cta = static_cast<int>(blockIdx.x) - (second ? rows_q.ctas : 0);
     const int table_len = p.items * VEC;
@@ -179,133 +182,77 @@ heads_vector_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const Ro
     const bool on0 = on && col0 < p.dim, on1 = on && col1 < p.dim;
     const float inv_dim = 1.0f / static_cast<float>(p.dim);
 
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    uint4 w0 = zero, w1 = zero;
-    if constexpr (MODE != kHeadRope) {
-        if (on0) w0 = *reinterpret_cast<const uint4*>(h.weight + col0);
-        if (on1) w1 = *reinterpret_cast<const uint4*>(h.weight + col1);
-    }
     Pair acc0[N], acc1[N];  // dweight of this lane's columns
-    if constexpr (MODE == kHeadNormBackward) {
+    if constexpr (kBackward) {
 #pragma unroll
         for (int j = 0; j < N; ++j) acc0[j] = acc1[j] = both(0.f);
     }
-
-    // Within a token offsets take 32 bits (the host sees to it), and so do the units.
-    const int total_steps = (h.heads + per_step - 1) / per_step;
-    const int x_h = static_cast<int>(h.x_h), dy_h = static_cast<int>(h.dy_h), o_h = static_cast<int>(h.o_h);
-    const unsigned units = static_cast<unsigned>(h.units), seq = static_cast<unsigned>(p.seq), chunks = h.chunks;
-    const unsigned unit_step = static_cast<unsigned>(h.ctas) * kWarps;
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+    uint4 w0 = zero, w1 = zero;
+    auto load_weights = [&](const HeadRows<T>& rows) {
+        if (MODE != kHeadRope && on0) w0 = *reinterpret_cast<const uint4*>(rows.weight + col0);
+        if (MODE != kHeadRope && on1) w1 = *reinterpret_cast<const uint4*>(rows.weight + col1);
+    };
+    if constexpr (kBackward) load_weights(h);
     uint4 x0[U], x1[U], d0[U], d1[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) x0[i] = x1[i] = d0[i] = d1[i] = zero;  // and so they stay in lanes without columns
-    for (unsigned u = cta * kWarps + warp; u < units; u += unit_step) {
-        const unsigned token = chunks == 1 ? u : u / chunks;
-        const int step0 = static_cast<int>(u - token * chunks) * h.steps;
-        const int step1 = min(step0 + h.steps, total_steps);
-        const unsigned b = token / seq, s = token - b * seq;
-        const T* x = h.x + b * h.x_b + s * h.x_s;
-        const T* dy = MODE == kHeadNormBackward ? h.dy + b * h.dy_b + s * h.dy_s : nullptr;
-        T* out = h.out + b * h.o_b + s * h.o_s;
 
-        auto fetch = [&](int i, int step) {
-            if (step >= step1) return;  // the same for the warp
-            const int head = min(step * per_step + sub, h.heads - 1);  // a row that is not there: the last, and not stored
-            const int at = head * x_h;
-            if (on0) x0[i] = *reinterpret_cast<const uint4*>(x + (at + col0));
-            if (on1) x1[i] = *reinterpret_cast<const uint4*>(x + (at + col1));
-            if constexpr (MODE == kHeadNormBackward) {
-                const int dat = head * dy_h;
-                if (on0) d0[i] = *reinterpret_cast<const uint4*>(dy + (dat + col0));
-                if (on1) d1[i] = *reinterpret_cast<const uint4*>(dy + (dat + col1));
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < U; ++i) fetch(i, step0 + i);  // in flight while the angles are formed
-
-        const double pos = rope_position(p, b, s);
-        __syncwarp();  // the previous token's table has been read
-        for (int i = lane; i < table_len; i += 32) {
-            const float2 t = i < p.half ? rope_angle(pos, p.freq[i], p.scale, p.sin_sign) : make_float2(1.f, 0.f);
-            cos_table[i] = t.x;
-            sin_table[i] = t.y;
+    float c[VEC], n[VEC];  // this token's angles, for this lane's columns
+    // Within a token offsets take 32 bits (the host sees to it).
+    auto fetch = [&](const HeadRows<T>& rows, const T* x, const T* dy, int i, int step, int end) {
+        if (step >= end) return;  // the same for the warp
+        const int head = min(step * per_step + sub, rows.heads - 1);  // a row that is not there: the last, and not stored
+        const int at = head * static_cast<int>(rows.x_h);
+        if (on0) x0[i] = *reinterpret_cast<const uint4*>(x + (at + col0));
+        if (on1) x1[i] = *reinterpret_cast<const uint4*>(x + (at + col1));
+        if constexpr (kBackward) {
+            const int dat = head * static_cast<int>(rows.dy_h);
+            if (on0) d0[i] = *reinterpret_cast<const uint4*>(dy + (dat + col0));
+            if (on1) d1[i] = *reinterpret_cast<const uint4*>(dy + (dat + col1));
         }
-        __syncwarp();
-        Pair c0[N], s0[N], c1[N], s1[N];
-        {
-            float c[VEC], n[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; j += 4) {  // 16-byte aligned: table_len and it * VEC are whole vectors
-                *reinterpret_cast<float4*>(c + j) = *reinterpret_cast<const float4*>(cos_table + (on ? it * VEC : 0) + j);
-                *reinterpret_cast<float4*>(n + j) = *reinterpret_cast<const float4*>(sin_table + (on ? it * VEC : 0) + j);
-            }
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                if constexpr (INTERLEAVED) {
-                    c0[j] = both(c[j]);
-                    c1[j] = both(c[N + j]);
-                    s0[j] = pair(-n[j], n[j]);
-                    s1[j] = pair(-n[N + j], n[N + j]);
-                } else {
-                    c0[j] = c1[j] = pair(c[2 * j], c[2 * j + 1]);
-                    s0[j] = pair(-n[2 * j], -n[2 * j + 1]);
-                    s1[j] = pair(n[2 * j], n[2 * j + 1]);
-                }
-            }
-        }
-        if constexpr (MODE == kHeadNorm) {  // the weights ride on the coefficients
-            Pair v0[N], v1[N];
-            unpack_pairs<T>(w0, v0);
-            unpack_pairs<T>(w1, v1);
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                c0[j] = c0[j] * v0[j];
-                c1[j] = c1[j] * v1[j];
-                s0[j] = s0[j] * (INTERLEAVED ? swapped(v0[j]) : v1[j]);
-                s1[j] = s1[j] * (INTERLEAVED ? swapped(v1[j]) : v0[j]);
-            }
-        }
-
-        for (int step = step0; step < step1; step += U) {
+    };
+    // Steps begin .. end of one tensor's heads; the first U are on their way.
+    auto walk = [&](const HeadRows<T>& rows, const T* x, const T* dy, T* out, int begin, int end) {
+        for (int step = begin; step < end; step += U) {
 #pragma unroll
             for (int i = 0; i < U; ++i) {
                 const int head = (step + i) * per_step + sub;
-                const bool in = step + i < step1 && head < h.heads;
-                Pair a[N], c[N], g0[N], g1[N];
+                const bool in = step + i < end && head < rows.heads;
+                Pair a[N], b[N], g0[N], g1[N];
                 unpack_pairs<T>(x0[i], a);
-                unpack_pairs<T>(x1[i], c);
-                if constexpr (MODE == kHeadNormBackward) {
+                unpack_pairs<T>(x1[i], b);
+                if constexpr (kBackward) {
                     unpack_pairs<T>(d0[i], g0);
                     unpack_pairs<T>(d1[i], g1);
                 }
-                fetch(i, step + i + U);
+                fetch(rows, x, dy, i, step + i + U, end);
                 if constexpr (MODE == kHeadRope) {
-                    rope_turn<INTERLEAVED, MODE == kHeadRope>(a, c, c0, s0, c1, s1, rot0, rot1);
+                    rope_turn<INTERLEAVED>(a, b, c, n, rot0, rot1);
                 } else {
-                    Pair squares = both(0.f);
+                    Pair v0[N], v1[N], squares = both(0.f);
+                    unpack_pairs<T>(w0, v0);
+                    unpack_pairs<T>(w1, v1);
 #pragma unroll
-                    for (int j = 0; j < N; ++j) squares = fma2(a[j], a[j], fma2(c[j], c[j], squares));
+                    for (int j = 0; j < N; ++j) squares = fma2(a[j], a[j], fma2(b[j], b[j], squares));
                     float ss = sum(squares);
                     if constexpr (MODE == kHeadNorm) {
                         for (int o = p.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                         const Pair rstd = both(head_rstd(ss, inv_dim, p.eps));
 #pragma unroll
                         for (int j = 0; j < N; ++j) {
-                            a[j] = a[j] * rstd;
-                            c[j] = c[j] * rstd;
+                            a[j] = a[j] * rstd * v0[j];
+                            b[j] = b[j] * rstd * v1[j];
                         }
-                        rope_turn<INTERLEAVED, MODE == kHeadRope>(a, c, c0, s0, c1, s1, rot0, rot1);
+                        rope_turn<INTERLEAVED>(a, b, c, n, rot0, rot1);
                     } else {
-                        Pair v0[N], v1[N];
-                        rope_turn<INTERLEAVED, true>(g0, g1, c0, s0, c1, s1, rot0, rot1);
-                        unpack_pairs<T>(w0, v0);
-                        unpack_pairs<T>(w1, v1);
+                        rope_turn<INTERLEAVED>(g0, g1, c, n, rot0, rot1);
                         Pair dots = both(0.f);
 #pragma unroll
                         for (int j = 0; j < N; ++j) {
                             v0[j] = v0[j] * g0[j];
                             v1[j] = v1[j] * g1[j];
-                            dots = fma2(v0[j], a[j], fma2(v1[j], c[j], dots));
+                            dots = fma2(v0[j], a[j], fma2(v1[j], b[j], dots));
                         }
                         float dot = sum(dots);
                         for (int o = p.lanes >> 1; o > 0; o >>= 1) {
@@ -317,19 +264,64 @@ heads_vector_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const Ro
 #pragma unroll
                         for (int j = 0; j < N; ++j) {
                             a[j] = a[j] * rstd;
-                            c[j] = c[j] * rstd;
+                            b[j] = b[j] * rstd;
                             if (in) {
                                 acc0[j] = fma2(g0[j], a[j], acc0[j]);
-                                acc1[j] = fma2(g1[j], c[j], acc1[j]);
+                                acc1[j] = fma2(g1[j], b[j], acc1[j]);
                             }
                             a[j] = fma2(a[j], k, v0[j] * rstd);
-                            c[j] = fma2(c[j], k, v1[j] * rstd);
+                            b[j] = fma2(b[j], k, v1[j] * rstd);
                         }
                     }
                 }
-                const int oat = head * o_h;
+                const int oat = head * static_cast<int>(rows.o_h);
                 if (in && on0) *reinterpret_cast<uint4*>(out + (oat + col0)) = pack_pairs<T>(a);
-                if (in && on1) *reinterpret_cast<uint4*>(out + (oat + col1)) = pack_pairs<T>(c);
+                if (in && on1) *reinterpret_cast<uint4*>(out + (oat + col1)) = pack_pairs<T>(b);
+            }
+        }
+    };
+    auto start = [&](const HeadRows<T>& rows, const T* x, const T* dy, int begin, int end) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) fetch(rows, x, dy, i, begin + i, end);
+    };
+
+    const int steps_q = (h.heads + per_step - 1) / per_step, steps_k = kBackward ? 0 : (rows_k.heads + per_step - 1) / per_step;
+    const unsigned units = static_cast<unsigned>(h.units), seq = static_cast<unsigned>(p.seq), chunks = h.chunks;
+    const unsigned unit_step = static_cast<unsigned>(h.ctas) * kWarps;
+    for (unsigned u = cta * kWarps + warp; u < units; u += unit_step) {
+        const unsigned token = chunks == 1 ? u : u / chunks;
+        const int begin = static_cast<int>(u - token * chunks) * h.steps, end = min(begin + h.steps, steps_q + steps_k);
+        const int end_q = min(end, steps_q), begin_k = max(begin, steps_q) - steps_q, end_k = end - steps_q;
+        const unsigned b = token / seq, s = token - b * seq;
+        const T* x = h.x + b * h.x_b + s * h.x_s;
+        const T* dy = kBackward ? h.dy + b * h.dy_b + s * h.dy_s : nullptr;
+        const T* xk = kBackward ? nullptr : rows_k.x + b * rows_k.x_b + s * rows_k.x_s;
+        // the first loads are in flight while the angles are formed
+        if (begin < end_q) start(h, x, dy, begin, end_q);
+        else if (!kBackward) start(rows_k, xk, dy, begin_k, end_k);
+
+        const double pos = rope_position(p, b, s);
+        __syncwarp();  // the previous token's table has been read
+        for (int i = lane; i < table_len; i += 32) {
+            const float2 t = i < p.half ? rope_angle<sizeof(T) == 2>(pos, p.freq[i] * kTurnsPerRadian, p.scale, p.sin_sign) : make_float2(1.f, 0.f);
+            cos_table[i] = t.x;
+            sin_table[i] = t.y;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {  // 16-byte aligned: table_len and it * VEC are whole vectors
+            *reinterpret_cast<float4*>(c + j) = *reinterpret_cast<const float4*>(cos_table + (on ? it * VEC : 0) + j);
+            *reinterpret_cast<float4*>(n + j) = *reinterpret_cast<const float4*>(sin_table + (on ? it * VEC : 0) + j);
+        }
+        if (begin < end_q) {
+            if constexpr (MODE == kHeadNorm) load_weights(h);
+            walk(h, x, dy, h.out + b * h.o_b + s * h.o_s, begin, end_q);
+        }
+        if constexpr (!kBackward) {
+            if (begin_k < end_k) {
+                if (begin < end_q) start(rows_k, xk, dy, begin_k, end_k);
+                load_weights(rows_k);
+                walk(rows_k, xk, dy, rows_k.out + b * rows_k.o_b + s * rows_k.o_s, begin_k, end_k);
             }
         }
     }
@@ -440,7 +432,7 @@ heads_row_kernel(const HeadRows<T> rows_q, const HeadRows<T> rows_k, const RopeP
         T* out = h.out + b * h.o_b + s * h.o_s;
         const double pos = rope_position(p, b, s);
         __syncwarp();
-        for (int i = lane; i < p.half; i += 32) table[i] = rope_angle(pos, p.freq[i], p.scale, p.sin_sign);
+        for (int i = lane; i < p.half; i += 32) table[i] = rope_angle<sizeof(T) == 2>(pos, p.freq[i] * kTurnsPerRadian, p.scale, p.sin_sign);
         for (int head = head0; head < head1; head += kRowFormRows) {
             const int n = min(kRowFormRows, head1 - head);
             __syncwarp();  // the rows of the previous step have been stored

@@ -129,11 +129,6 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return d;
 }
-__device__ __forceinline__ Pair swapped(Pair p) {
-    float lo, hi;
-    split(p, lo, hi);
-    return pair(hi, lo);
-}
 __device__ __forceinline__ float sum(Pair p) {
     float lo, hi;
     split(p, lo, hi);
