@@ -161,7 +161,8 @@ class _Rope(torch.autograd.Function):
     def backward(ctx: Any, *grad_outputs):
         interleaved, scale, inverse = ctx.how
         # the rotation's transpose is the rotation by the negative angle, which is differentiable in turn
-        dx = _Rope.apply(grad_outputs[0], *ctx.saved_tensors, interleaved, scale, not inverse)
+        turn = _Rope.apply if torch.is_grad_enabled() else _rope
+        dx = turn(grad_outputs[0], *ctx.saved_tensors, interleaved, scale, not inverse)
         return dx, None, None, None, None, None
 
 
