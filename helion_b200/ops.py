@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from threading import get_ident
 from typing import Any
 
 import torch
@@ -183,20 +184,21 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 _WS_CACHE_MAX = 32 << 20
-_ws_cache: dict[tuple[int, int], torch.Tensor] = {}
+_ws_cache: dict[tuple[int, int, int], torch.Tensor] = {}
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """Scratch for one C-ABI call. Small requests (latency-bound problems, where an allocation is a visible
-    share of the call) reuse one buffer per (device, stream): calls on one stream run in order, so they may
-    share scratch; calls on different streams get different buffers. Large requests are allocated per call and
+    share of the call) reuse one buffer per (device, stream, thread): the calls that a thread makes on one stream run
+    in order, so they may share scratch; the launches of two threads' calls may interleave on a stream, and calls on
+    different streams run together, so those get different buffers. Large requests are allocated per call and
     go back to torch's caching allocator afterwards. So are all requests while the stream is being captured: a
     graph keeps using its scratch whenever it is replayed, possibly beside other work of any stream, so its
     scratch has to come from the graph's own pool."""
     nbytes = max(int(nbytes), 256)
     if nbytes > _WS_CACHE_MAX or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index if device.index is not None else torch.cuda.current_device(), _stream(device))
+    key = (device.index if device.index is not None else torch.cuda.current_device(), _stream(device), get_ident())
     buf = _ws_cache.get(key)
     if buf is None or buf.numel() < nbytes:
         if len(_ws_cache) >= 64:  # streams come and go: do not let the cache grow without bound
