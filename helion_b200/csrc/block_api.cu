@@ -216,11 +216,39 @@ constexpr long long kSampleMaxSliceBytes = 160 << 10;   // beyond it a CTA re-re
 
 // CTAs per row: enough that a share fits shared memory well and, for few rows, that the GPU is busy - as long as a share
 // is worth the cluster's barriers.
+// bf16 batches that take sample_values_kernel, a CTA per row. top_p 0.95, sample_kernel against it, us, at 128256 logits:
+// 24 rows 52 / 72, 48 rows 84 / 72, 148 rows 160 / 74, 256 rows 250 / 94; at 50257: 24 rows 37 / 49, 48 rows 61 / 49; at
+// 8003: 148 rows 27 / 32, 256 rows 47 / 35. Rows without filters, of which sample_kernel only needs the maximum and the
+// weights: 48 rows of 128256 43 / 63, 256 rows 125 / 88.
+constexpr long long kSampleValueRows = 40, kSampleValueRowsUnfiltered = 128;
+constexpr long long kSampleValueLogits = 2000000;
+
+// A CTA per row, for batches of bf16 rows.
+int launch_sample_values(const DeviceInfo& d, const __nv_bfloat16* logits, long long ld, long long rows, long long vocab,
+                         int groups, const SampleParams& p, cudaStream_t s) {
+    auto kern = sample_values_kernel;
+    static std::atomic<bool> opted_in[kMaxDevices];
+    if (!opted_in[d.index].load(std::memory_order_acquire)) {
+        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kValueBytes))) return LCE_ERR_CUDA;
+        opted_in[d.index].store(true, std::memory_order_release);
+    }
+    kern<<<static_cast<unsigned>(rows), kSampleThreads, kValueBytes, s>>>(logits, ld, static_cast<int>(vocab), groups, p);
+    LCE_COUNT_LAUNCH();
+    return cuda_failed(cudaGetLastError()) ? LCE_ERR_CUDA : LCE_OK;
+}
+
 template <class T>
 int launch_sample(const DeviceInfo& d, const void* logits, long long ld, long long rows, long long vocab, const SampleParams& p,
                   cudaStream_t s) {
     constexpr int VEC = RmsTile<T>::kVec;
     const long long n_vec = cdiv(vocab + VEC - 1, VEC);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const long long groups = cdiv(n_vec, static_cast<long long>(kSampleWarps) * kValueChunk);
+        const bool filtered = p.top_k || p.top_p || (p.top_k_all > 0 && p.top_k_all < vocab) || p.top_p_all < 1.f;
+        if (rows >= (filtered ? kSampleValueRows : kSampleValueRowsUnfiltered) && rows * vocab >= kSampleValueLogits &&
+            groups * kSampleWarps <= kValueMaxChunks)
+            return launch_sample_values(d, static_cast<const T*>(logits), ld, rows, vocab, static_cast<int>(groups), p, s);
+    }
     int ctas = 1;
     while (ctas < kSampleMaxCluster &&
            (cdiv(n_vec, ctas) * 16 > kSampleSliceBytes || (rows * ctas < 2 * d.sm_count && vocab / (2 * ctas) >= 2048)))

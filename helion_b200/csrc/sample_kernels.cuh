@@ -174,18 +174,86 @@ __device__ __forceinline__ void sample_block_before(V (&v)[N], V (*tmp)[kSampleW
     }
 }
 
+// The index, by one warp: the first kept element of vectors begin .. end - 1 with whose weight the sum passes `target`;
+// where rounding left the target behind the last of them (or u is 1), that one. fetch(v, x) gives a vector's VEC values,
+// `tie_start` ties lie before `begin`.
+template <int VEC, class Fetch, class Weight>
+__device__ __forceinline__ void sample_find(int begin, int end, int head, Fetch&& fetch, Weight&& kept_weight, float bound,
+                                            double w_tie, long long ties, long long tie_start, double target,
+                                            double everything, long long row, const SampleParams& p) {
+    const int lane = threadIdx.x & 31;
+    // 32 vectors at a time
+    double passed = 0;
+    long long ties_passed = tie_start;
+    long long last = -1;  // of this lane's kept elements
+    double last_w = 0;
+    for (int base = begin; base < end; base += 32) {
+        const int v = base + lane;
+        float x[VEC];
+        int n_equal = 0;
+        if (v < end) {
+            fetch(v, x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) x[j] = -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) n_equal += x[j] == bound && v < end;
+        const int equal_incl = sample_warp_scan(n_equal);
+        long long tie = ties_passed + equal_incl - n_equal;
+        double w[VEC], lane_sum = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            w[j] = 0;
+            if (x[j] > bound) w[j] = kept_weight(x[j]);
+            else if (x[j] == bound && v < end && tie++ < ties) w[j] = w_tie;
+            lane_sum += w[j];
+            if (w[j] > 0) {
+                last = static_cast<long long>(v) * VEC + j - head;
+                last_w = w[j];
+            }
+        }
+        const double incl = sample_warp_scan(lane_sum);
+        const unsigned hit = __ballot_sync(0xffffffffu, lane_sum > 0 && passed + incl > target);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) {
+                double r = passed + (incl - lane_sum);
+                bool done = false;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    r += w[j];
+                    if (!done && w[j] > 0 && r > target) {
+                        done = true;
+                        last = static_cast<long long>(v) * VEC + j - head;
+                        last_w = w[j];
+                    }
+                }
+                p.token[row] = last;
+                if (p.logprob) p.logprob[row] = static_cast<float>(log(last_w / everything));
+            }
+            return;
+        }
+        passed += __shfl_sync(0xffffffffu, incl, 31);
+        ties_passed += __shfl_sync(0xffffffffu, equal_incl, 31);
+    }
+    // rounding left the target behind the last kept element, or u is 1: that element
+    const uint32_t best = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(last + 1));
+    if (static_cast<uint32_t>(last + 1) == best) {
+        p.token[row] = last;
+        if (p.logprob) p.logprob[row] = static_cast<float>(log(last_w / everything));
+    }
+}
+
+// One row, by the CTAs of a cluster.
 template <class T>
-__global__ void __launch_bounds__(kSampleThreads, 2)
-sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas, int vectors_per_warp, int in_smem,
-              const SampleParams p) {
+__device__ __forceinline__ void sample_row(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
+                                           int vectors_per_warp, int in_smem, const SampleParams& p, SampleShared& sh,
+                                           unsigned char* sample_slice, long long row) {
     constexpr int VEC = RmsTile<T>::kVec;
     using Key = SampleKey<T>;
     constexpr int kBins = kSampleBins, PER = kSampleBinsPerThread;
-    extern __shared__ __align__(16) unsigned char sample_slice[];
-    __shared__ SampleShared sh;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int rank = static_cast<int>(ptx::cluster_ctarank());
-    const long long row = blockIdx.x / n_ctas;
 
     // The row in 16-byte vectors that start on 16-byte boundaries: the first and the last may reach past it.
     const T* l = logits + row * ld;
@@ -762,66 +830,351 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
     }
     if (warp != owner) return;
     target -= start;
-    // the index: 32 vectors at a time
-    double passed = 0;
-    long long ties_passed = tie_start;
-    long long last = -1;  // of this lane's kept elements
-    double last_w = 0;
-    for (int base = v0; base < v1; base += 32) {
-        const int v = base + lane;
-        float x[VEC];
-        int n_equal = 0;
-        if (v < v1) {
-            fetch(v, x);
-        } else {
+    sample_find<VEC>(v0, v1, head, fetch, kept_weight, bound, w_tie, ties, tie_start, target, everything, row, p);
+}
+
+template <class T>
+__global__ void __launch_bounds__(kSampleThreads, 2)
+sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas, int vectors_per_warp, int in_smem,
+              const SampleParams p) {
+    extern __shared__ __align__(16) unsigned char sample_slice[];
+    __shared__ SampleShared sh;
+    sample_row<T>(logits, ld, vocab, n_ctas, vectors_per_warp, in_smem, p, sh, sample_slice, blockIdx.x / n_ctas);
+}
+
+// Batches of bf16 rows, a CTA per row: a histogram with one bin per VALUE. A bin's weights are then known from its count,
+// so thresholds cost an exponential per value that occurs, nothing has to be narrowed, and the weights of the kept logits
+// are looked up. Two passes over the row: counts, then the kept weights by chunks of 1024 logits, of which one holds the
+// token. Values of a magnitude of 2^-32 and more below 2^10 have bins, and zero; a row with any other but -inf and NaN
+// (one in 100000 of rounded normal values) is drawn by sample_row. 256 x 128256 with top_p 0.95: 94 us where a cluster a
+// row takes 250; 1024 rows 303 against 880. What bounds it is shared memory: one atomic per logit, and one 8-byte lookup
+// per kept logit; a lone CTA on an SM (up to 148 rows: 74 us) also waits for its own loads and 64-bit chains. Four vectors of
+// a lane in flight: two took 98, eight spilled and took 109. A cluster of 2 for a row, each adding up both's counts,
+// took 66 us against 74 at 64 rows and lost from 100 rows on.
+constexpr int kValueLow = (127 - 32) << 7;  // the bits of 2^-32
+constexpr int kValueSpan = 5375;            // magnitudes with bins: all below 2^10 but the last
+constexpr int kValueBins = 2 * kValueSpan + 1;  // larger values first: positive ones, zero, negative ones
+constexpr int kValuePerThread = 21;
+constexpr int kValuePadded = kValuePerThread * kSampleThreads;
+static_assert(kValuePadded >= kValueBins, "every bin has a thread");
+constexpr int kValueUnroll = 4;                      // vectors of a lane in flight
+constexpr int kValueChunk = 32 * kValueUnroll;       // vectors that are summed together
+constexpr int kValueMaxChunks = 1024;                // of a row: a sum and a number of ties each
+constexpr int kValueBytes = kValuePadded * 8 + kValueMaxChunks * 12;
+
+__device__ __forceinline__ float value_of_bin(int bin) {
+    const int d = bin - kValueSpan;
+    if (d == 0) return 0.f;
+    const uint32_t m = kValueLow + (d < 0 ? -d : d) - 1;
+    return __uint_as_float((m << 16) | (d > 0 ? 0x80000000u : 0u));
+}
+
+// The index of the bin of a value that has one and is not zero, by its bits.
+__device__ __forceinline__ int bin_of_value(uint32_t bits) {
+    const int off = static_cast<int>(bits & 0x7fffu) - kValueLow + 1;
+    return kValueSpan + (bits & 0x8000u ? off : -off);
+}
+
+// sample_row from global memory, out of line.
+__device__ __noinline__ void sample_row_alone(const __nv_bfloat16* logits, long long ld, int vocab, int vectors_per_warp,
+                                              const SampleParams& p, SampleShared& sh, long long row) {
+    sample_row<__nv_bfloat16>(logits, ld, vocab, 1, vectors_per_warp, 0, p, sh, nullptr, row);
+}
+
+__global__ void __launch_bounds__(kSampleThreads, 2)
+sample_values_kernel(const __nv_bfloat16* __restrict__ logits, long long ld, int vocab, int groups, const SampleParams p) {
+    using T = __nv_bfloat16;
+    using Key = SampleKey<T>;
+    constexpr int VEC = RmsTile<T>::kVec, PER = kValuePerThread, U = kValueUnroll;
+    extern __shared__ __align__(16) unsigned char sample_slice[];
+    __shared__ SampleShared sh;
+    uint32_t* hist = reinterpret_cast<uint32_t*>(sample_slice);
+    double* table = reinterpret_cast<double*>(sample_slice);  // in its place, later: the kept weight of every value
+    double* chunk_sum = table + kValuePadded;
+    uint32_t* chunk_equal = reinterpret_cast<uint32_t*>(chunk_sum + kValueMaxChunks);
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const long long row = blockIdx.x;
+
+    const T* l = logits + row * ld;
+    const int head = static_cast<int>((reinterpret_cast<uintptr_t>(l) & 15u) / sizeof(T));
+    const T* aligned = l - head;
+    const int n_vec = static_cast<int>((static_cast<long long>(vocab) + head + VEC - 1) / VEC);
+    const long long share = static_cast<long long>(groups) * kValueChunk;  // vectors of a warp
+    const int v0 = static_cast<int>(min(static_cast<long long>(n_vec), warp * share));
+    const int v1 = static_cast<int>(min(static_cast<long long>(n_vec), (warp + 1) * share));
+    constexpr uint32_t kNothing = 0xff80ff80u;  // -inf twice
+    auto read = [&](int v, int end) {  // outside the row, and from `end` on, -inf
+        if (v >= end) return make_uint4(kNothing, kNothing, kNothing, kNothing);
+        const long long i0 = static_cast<long long>(v) * VEC - head;
+        if (i0 >= 0 && i0 + VEC <= vocab) return __ldg(reinterpret_cast<const uint4*>(aligned + static_cast<long long>(v) * VEC));
+        alignas(16) T tmp[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) x[j] = -INFINITY;
-        }
+        for (int j = 0; j < VEC; ++j) tmp[j] = i0 + j >= 0 && i0 + j < vocab ? l[i0 + j] : Cvt<T>::from_f(-INFINITY);
+        return *reinterpret_cast<const uint4*>(tmp);
+    };
+
+    float temp = p.temperature ? p.temperature[row] : p.temperature_all;
+    long long k = p.top_k ? (p.top_k_i64 ? static_cast<const long long*>(p.top_k)[row] : static_cast<const int*>(p.top_k)[row]) : p.top_k_all;
+    float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
+    float min_row = p.min_p ? p.min_p[row] : p.min_p_all;
+    if (!(temp > 0.f)) {  // the first maximum: the top_k of 1
+        temp = 1.f;
+        k = 1;
+        min_row = 0.f;
+    }
+    const bool counted = k != 1;  // else only the maximum is asked for
+
+    if (t < kSampleTable) sh.table[t] = exp2(t / static_cast<double>(kSampleTable));
+    if (t == 0) {
+        sh.first_u = kValuePadded;
+        sh.first_l = kSampleThreads;
+        sh.bin = kValuePadded;
+    }
+    // ---- the counts, or the maximum
+    bool other = false;  // a value without a bin
+    float top = -INFINITY;
+    if (counted) {
+        for (int i = t; i < kValuePadded; i += kSampleThreads) hist[i] = 0;
+        __syncthreads();
+        for (int base = v0 + lane; base < v1; base += kValueChunk) {
+            uint4 raw[U];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) n_equal += x[j] == bound && v < v1;
-        const int equal_incl = sample_warp_scan(n_equal);
-        long long tie = ties_passed + equal_incl - n_equal;
-        double w[VEC], lane_sum = 0;
+            for (int i = 0; i < U; ++i) raw[i] = read(base + 32 * i, v1);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            w[j] = 0;
-            if (x[j] > bound) w[j] = kept_weight(x[j]);
-            else if (x[j] == bound && v < v1 && tie++ < ties) w[j] = w_tie;
-            lane_sum += w[j];
-            if (w[j] > 0) {
-                last = static_cast<long long>(v) * VEC + j - head;
-                last_w = w[j];
-            }
-        }
-        const double incl = sample_warp_scan(lane_sum);
-        const unsigned hit = __ballot_sync(0xffffffffu, lane_sum > 0 && passed + incl > target);
-        if (hit) {
-            if (lane == __ffs(hit) - 1) {
-                double r = passed + (incl - lane_sum);
-                bool done = false;
+            for (int i = 0; i < U; ++i) {
+                const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    r += w[j];
-                    if (!done && w[j] > 0 && r > target) {
-                        done = true;
-                        last = static_cast<long long>(v) * VEC + j - head;
-                        last_w = w[j];
-                    }
+                    const uint32_t h = j & 1 ? words[j >> 1] >> 16 : words[j >> 1] & 0xffffu;
+                    const uint32_t m = h & 0x7fffu;
+                    if (m - kValueLow < kValueSpan) atomicAdd(&hist[bin_of_value(h)], 1u);
+                    else if (m == 0) atomicAdd(&hist[kValueSpan], 1u);
+                    else if (h != 0xff80u && m <= 0x7f80u) other = true;
                 }
-                p.token[row] = last;
-                if (p.logprob) p.logprob[row] = static_cast<float>(log(last_w / everything));
             }
+        }
+    } else {
+        for (int base = v0 + lane; base < v1; base += kValueChunk) {
+            uint4 raw[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) raw[i] = read(base + 32 * i, v1);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                float x[VEC];
+                rms_unpack<T>(raw[i], x);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) top = fmaxf(top, x[j]);
+            }
+        }
+        const uint32_t key = __reduce_max_sync(0xffffffffu, Key::of(top));
+        if (lane == 0) sh.wu[warp] = key;
+    }
+    if (__syncthreads_or(other)) {
+        sample_row_alone(logits, ld, vocab, static_cast<int>(share), p, sh, row);
+        return;
+    }
+    long long members = 0;  // of this thread's bins
+    if (counted) {
+        unsigned first = kValuePadded;
+#pragma unroll
+        for (int j = PER - 1; j >= 0; --j) {
+            const uint32_t c = hist[PER * t + j];
+            members += c;
+            if (c > 0) first = PER * t + j;
+        }
+        first = __reduce_min_sync(0xffffffffu, first);
+        if (lane == 0 && first < kValuePadded) atomicMin(&sh.first_u, first);
+        __syncthreads();
+        if (sh.first_u < kValuePadded) top = value_of_bin(sh.first_u);
+    } else {
+        uint32_t key = 0;
+        for (int i = 0; i < kSampleWarps; ++i) key = max(key, sh.wu[i]);
+        top = Key::value(key);
+        if (top == INFINITY) {
+            __syncthreads();  // all have read sh.wu
+            sample_row_alone(logits, ld, vocab, static_cast<int>(share), p, sh, row);
             return;
         }
-        passed += __shfl_sync(0xffffffffu, incl, 31);
-        ties_passed += __shfl_sync(0xffffffffu, equal_incl, 31);
     }
-    // rounding left the target behind the last kept element, or u is 1: that element
-    const uint32_t best = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(last + 1));
-    if (static_cast<uint32_t>(last + 1) == best) {
-        p.token[row] = last;
-        if (p.logprob) p.logprob[row] = static_cast<float>(log(last_w / everything));
+    if (top == -INFINITY) {
+        if (t == 0) {
+            p.token[row] = -1;
+            if (p.logprob) p.logprob[row] = -INFINITY;
+        }
+        return;
     }
+    SampleWeights weight;
+    weight.top = top;
+    weight.top_d = top;
+    weight.inv_t = 1.0 / static_cast<double>(temp);
+    weight.inv_t32 = 0;
+    weight.table = sh.table;
+
+    // ---- what is kept: values above `bound`, and `ties` of those equal to it
+    float bound = -INFINITY;
+    long long ties = 0;
+    if (k == 1) {
+        bound = top;
+        ties = 1;
+    } else if (counted) {
+        int last_bin = kValuePadded;  // of the top_k
+        if (k > 0 && k < vocab) {
+            long long before[1] = {members};
+            sample_block_before<1>(before, sh.wn);
+            if (before[0] < k && k <= before[0] + members) {
+                long long run = before[0];
+                for (int j = 0; j < PER; ++j) {
+                    const long long c = hist[PER * t + j];
+                    if (run < k && k <= run + c) {
+                        sh.bin = PER * t + j;
+                        sh.count = k - run;
+                    }
+                    run += c;
+                }
+            }
+            __syncthreads();
+            if (sh.bin < kValuePadded) {  // else fewer than k values are above -inf
+                last_bin = static_cast<int>(sh.bin);
+                bound = value_of_bin(last_bin);
+                ties = sh.count;
+            }
+            __syncthreads();
+        }
+        if (top_p < 1.f) {
+            auto kept = [&](int bin) -> long long {  // the top_k's members in a bin
+                const long long c = hist[bin];
+                return bin < last_bin ? c : (bin == last_bin ? min(c, ties) : 0);
+            };
+            double sum = 0;
+            for (int j = 0; j < PER; ++j) {
+                const long long c = kept(PER * t + j);
+                if (c > 0) sum += static_cast<double>(c) * weight(value_of_bin(PER * t + j));
+            }
+            double before[1] = {sum};
+            sample_block_before<1>(before, sh.wd);
+            if (t == kSampleThreads - 1) sh.total_d[0] = before[0] + sum;
+            __syncthreads();
+            const double limit = (top_p > 0.f ? static_cast<double>(top_p) : 0.0) * sh.total_d[0];
+            if (sum > 0 && before[0] + sum > limit) atomicMin(&sh.first_l, static_cast<unsigned>(t));
+            __syncthreads();
+            if (sh.first_l == t) {
+                // the first bin whose weights pass the limit; by the rounding of the scan, the last one
+                double run = before[0], w = 0, ahead = 0;
+                long long n = 0;
+                for (int j = 0; j < PER; ++j) {
+                    const long long c = kept(PER * t + j);
+                    if (c == 0) continue;
+                    n = c;
+                    w = weight(value_of_bin(PER * t + j));
+                    ahead = run;
+                    sh.bin = PER * t + j;
+                    run += static_cast<double>(c) * w;
+                    if (run > limit) break;
+                }
+                // tie number i (from 0) is kept while ahead + i w <= limit; the very first value always
+                const double room = w > 0 ? (limit - ahead) / w : 4e9;
+                long long most = room < 0 ? 0 : static_cast<long long>(fmin(room, 4e9)) + 1;
+                if (sh.bin == sh.first_u && most < 1) most = 1;
+                sh.count = min(most, n);
+            }
+            __syncthreads();
+            if (sh.first_l < kSampleThreads) {
+                bound = value_of_bin(static_cast<int>(sh.bin));
+                ties = sh.count;
+            }
+        }
+    }
+    const double min_p = min_row > 0.f ? fminf(min_row, 1.f) : 0.0;
+    auto kept_weight = [&](float v) {
+        const double w = weight(v);
+        return w >= min_p ? w : 0.0;
+    };
+    const double w_tie = ties > 0 ? kept_weight(bound) : 0.0;
+
+    // ---- the kept weights by chunk
+    const int n_chunks = groups * kSampleWarps;
+    if (counted) {
+        __syncthreads();  // all have read the counts
+        for (int i = t; i < kValueBins; i += kSampleThreads) {
+            const float v = value_of_bin(i);
+            table[i] = v > bound && v <= top ? kept_weight(v) : 0.0;
+        }
+        __syncthreads();
+    }
+    for (int g = 0; g < groups; ++g) {
+        const int base = static_cast<int>(min(static_cast<long long>(v1), v0 + static_cast<long long>(g) * kValueChunk)) + lane;
+        uint4 raw[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) raw[i] = read(base + 32 * i, v1);
+        double sum = 0;
+        uint32_t equal = 0;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            float x[VEC];
+            rms_unpack<T>(raw[i], x);
+            float m = x[0];
+#pragma unroll
+            for (int j = 1; j < VEC; ++j) m = fmaxf(m, x[j]);
+            if (m >= bound) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const uint32_t h = j & 1 ? words[j >> 1] >> 16 : words[j >> 1] & 0xffffu;
+                    if (x[j] > bound) sum += table[x[j] == 0.f ? kValueSpan : bin_of_value(h)];
+                    else if (x[j] == bound) ++equal;
+                }
+            }
+        }
+        sum = sample_warp_sum(sum);
+        equal = __reduce_add_sync(0xffffffffu, equal);
+        if (lane == 0) {
+            chunk_sum[warp * groups + g] = sum;
+            chunk_equal[warp * groups + g] = equal;
+        }
+    }
+    __syncthreads();
+    if (warp != 0) return;
+
+    // ---- the chunk, 32 at a time
+    auto chunk = [&](int c, long long& before, long long& n_incl, long long& n) -> double {  // its kept weight
+        n = c < n_chunks ? chunk_equal[c] : 0;
+        n_incl = sample_warp_scan(n);
+        const long long left = ties - (before + n_incl - n);
+        const long long tied = left <= 0 ? 0 : min(left, n);
+        return c < n_chunks ? chunk_sum[c] + static_cast<double>(tied) * w_tie : 0.0;
+    };
+    double everything = 0;
+    long long before = 0, n_incl, n;
+    for (int c = lane; c - lane < n_chunks; c += 32) {
+        everything += sample_warp_sum(chunk(c, before, n_incl, n));
+        before += __shfl_sync(0xffffffffu, n_incl, 31);
+    }
+    float u = p.uniform[row];
+    u = u > 0.f ? u : 0.f;
+    const double target = static_cast<double>(u) * everything;
+    double run = 0, start = 0;
+    long long tie_start = 0;
+    int owner = -1;  // the chunk whose weights pass the target, or the last one that holds any
+    before = 0;
+    for (int c = lane; c - lane < n_chunks; c += 32) {
+        const double s = chunk(c, before, n_incl, n);
+        const double incl = sample_warp_scan(s);
+        const unsigned any = __ballot_sync(0xffffffffu, s > 0), hit = __ballot_sync(0xffffffffu, s > 0 && run + incl > target);
+        if (any) {
+            const int at = hit ? __ffs(hit) - 1 : 31 - __clz(any);
+            owner = c - lane + at;
+            start = run + __shfl_sync(0xffffffffu, incl - s, at);
+            tie_start = before + __shfl_sync(0xffffffffu, n_incl - n, at);
+            if (hit) break;
+        }
+        run += __shfl_sync(0xffffffffu, incl, 31);
+        before += __shfl_sync(0xffffffffu, n_incl, 31);
+    }
+    if (owner < 0) return;  // not reached: the maximum is kept
+    const int begin = static_cast<int>(min(static_cast<long long>(n_vec), owner / groups * share + static_cast<long long>(owner % groups) * kValueChunk));
+    const int end = min(n_vec, begin + kValueChunk);
+    auto fetch = [&](int v, float (&x)[VEC]) { rms_unpack<T>(read(v, end), x); };
+    sample_find<VEC>(begin, end, head, fetch, kept_weight, bound, w_tie, ties, tie_start, target - start, everything, row, p);
 }
 
 }  // namespace lce

@@ -170,6 +170,41 @@ def test_batches(rows):
     assert torch.equal(token, again)
 
 
+@pytest.mark.parametrize("layout", ["rows", "view"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_large_batches_with_rows_of_every_kind(dtype, layout):
+    """A batch that large bf16 calls take in another form, each row with filters of its own: ordinary rows, masked ones,
+    ties, zeros of both signs, rows of values that have no bin of their own (tiny, huge, infinite), nothing kept, NaN."""
+    rows, vocab = 72, 32771
+    wide = _logits(rows, vocab + 13, dtype, 31)
+    logits = wide[:, 5:5 + vocab] if layout == "view" else wide[:, :vocab].contiguous()
+    g = _gen(32)
+    largest = torch.finfo(dtype).max
+    for i in range(8):  # every kind meets eight of the filters
+        at = 9 * i
+        logits[at + 1].masked_fill_(torch.rand(vocab, generator=g, device=DEV) < 0.9, -INF)
+        logits[at + 2, ::7] = 3e-7 if dtype == torch.float16 else 1e-12
+        logits[at + 3, 5::1001] = largest / 2
+        logits[at + 4, 17 * (i + 1)::9001] = INF
+        logits[at + 5] = torch.randint(-4, 5, (vocab,), generator=g, device=DEV).to(dtype)
+        logits[at + 6] = torch.where(torch.rand(vocab, generator=g, device=DEV) < 0.5, 0.0, -0.0).to(dtype)
+        logits[at + 7, ::3] = float("nan")
+        logits[at + 8] = -INF if i % 2 else -2.75
+    u = torch.rand(rows, generator=_gen(33), device=DEV)
+    u[3], u[4] = 0.0, 1.0
+    params = {"temperature": 1.0, "top_k": 0, "top_p": 1.0, "min_p": 0.0}
+    lists = {name: [FILTERS[(5 * i + i // 9) % len(FILTERS)].get(name, off) for i in range(rows)] for name, off in params.items()}
+    first = _check(logits, u, **lists)
+    second = _check(logits.clone(), u, **lists)
+    assert torch.equal(first[0], second[0]) and torch.equal(first[1], second[1])
+
+
+@pytest.mark.parametrize("filters", FILTERS)
+def test_large_batches_of_one_kind(filters):
+    logits = _logits(64, 31253, torch.bfloat16, 41)
+    _check(logits, torch.rand(64, generator=_gen(42), device=DEV), **filters)
+
+
 def test_peaked_flat_and_wide_spread_logits():
     vocab = 70000
     u = torch.tensor([0.0, 0.2, 0.7, 0.999999], device=DEV)
