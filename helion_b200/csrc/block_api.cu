@@ -260,14 +260,15 @@ int launch_sample(const DeviceInfo& d, const void* logits, long long ld, long lo
     auto kern = sample_kernel<T>;
     static std::atomic<bool> opted_in[kMaxDevices];  // setting the attribute twice from two threads is harmless
     if (!opted_in[d.index].load(std::memory_order_acquire)) {
-        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSampleMaxSliceBytes))))
+        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(kSampleList * 8 + kSampleMaxSliceBytes))))
             return LCE_ERR_CUDA;
         opted_in[d.index].store(true, std::memory_order_release);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
     cfg.blockDim = dim3(kSampleThreads);
-    cfg.dynamicSmemBytes = in_smem ? static_cast<size_t>(slice) : 0;
+    cfg.dynamicSmemBytes = kSampleList * 8 + (in_smem ? static_cast<size_t>(slice) : 0);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;

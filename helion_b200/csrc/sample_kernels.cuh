@@ -12,16 +12,25 @@
 // - one in a hundred rows - would go to the wrong one. A NaN counts as -inf; a row with nothing above -inf gives
 // token -1; among +inf all weight is shared equally; a temperature that is not positive takes the first maximum.
 //
-// No sort. A prefix of the order is a threshold on the logit and a number of ties, and both are found by counting:
+// A prefix of the order is a threshold on the logit and a number of ties, and both are found by counting:
 //   1. a cluster of 1..8 CTAs takes a row; each keeps its slice in shared memory, so the logits are read once;
 //   2. a histogram of (max - l) / temperature brackets the threshold: exactly for top_k, and for top_p between bounds,
 //      since a bin's weights are known to the bin's width from its count;
-//   3. for top_p one pass sums all weights, and those above the bracket, in 64 bits;
+//   3. where the top_k's bracket and all above it hold at most 1024 logits, the first CTA collects and sorts those and
+//      draws from the list (sample_listed); else, for top_p, one pass sums all weights, and those above the bracket, in
+//      64 bits;
 //   4. histograms over the ordered bits of the logits inside the bracket narrow it to a single value;
 //      only elements inside the bracket need their weight for that;
 //   5. one pass sums the kept weights by warp, the sums find the warp that holds u times the total, and that warp
 //      finds the index.
-// Histograms are counts (integer atomics in shared memory) and sums have a fixed order: the same tokens on every run.
+// Histograms are counts (integer atomics in shared memory), lists are sorted and sums have a fixed order: the same tokens
+// on every run. Large batches of bf16 rows are drawn by sample_values_kernel, below.
+//
+// The bytes are nothing: 64 x 128256 fp32 is 33 MB, 5 us. What bounds a row is the chain of its steps, each a scan, a block
+// scan and a barrier of the cluster with every CTA reading the others' 4 KB of bins: 3 to 5 us, 33 us in all for one row
+// with filters of every kind (51 without the list), 25 with a top_k alone. 64 such rows take 93 us (117 without the list):
+// about 200 of the 296 CTAs that would fit are resident, since clusters of 8 do not fill every GPC. CTAs of 1024 threads
+// in clusters of 4 took the same; slices re-read from L2 instead of kept in shared memory 13 to 40 % more.
 #pragma once
 
 #include "ptx.cuh"
@@ -93,8 +102,12 @@ struct SampleShared {
     double total_d[2];
     unsigned first_u, first_l;
     unsigned bin;
+    unsigned listed;  // entries of the list, in the first CTA
     long long before, count;
 };
+
+constexpr int kSampleList = 1024;
+static_assert(kSampleList == 2 * kSampleThreads, "two entries a thread");
 
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
     asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
@@ -104,6 +117,12 @@ __device__ __forceinline__ void st_cluster_s64(uint32_t addr, long long v) {
 }
 __device__ __forceinline__ void ld_cluster(uint32_t addr, uint32_t (&v)[2]) {
     asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ uint32_t atom_cluster_add(uint32_t addr, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(addr), "r"(v) : "memory");
+    return old;
 }
 
 // The weights of one row (whose maximum is finite).
@@ -244,11 +263,96 @@ __device__ __forceinline__ void sample_find(int begin, int end, int head, Fetch&
     }
 }
 
-// One row, by the CTAs of a cluster.
+// Sorts 2^log2 entries, larger first.
+__device__ __forceinline__ void sample_sort(unsigned long long* list, int log2) {
+    const int t = threadIdx.x;
+    for (int size = 1; size <= log2; ++size)
+        for (int step = size - 1; step >= 0; --step) {
+            __syncthreads();
+            if (t < 1 << (log2 - 1)) {
+                const int i = ((t >> step) << (step + 1)) | (t & ((1 << step) - 1)), j = i | (1 << step);
+                const unsigned long long a = list[i], b = list[j];
+                if ((a < b) == (((i >> size) & 1) == 0)) {
+                    list[i] = b;
+                    list[j] = a;
+                }
+            }
+        }
+    __syncthreads();
+}
+
+// The draw from the top_k alone, by one CTA: `list` holds the n largest logits in any order, as key and inverted index,
+// the k first of which are kept by the top_k.
+template <class T>
+__device__ __noinline__ void sample_listed(unsigned long long* list, int n, int k, const SampleWeights& weight, float top_p,
+                                           double min_p, const SampleParams& p, SampleShared& sh, long long row) {
+    using Key = SampleKey<T>;
+    const int t = threadIdx.x;
+    int log2 = 1;
+    while (1 << log2 < n) ++log2;
+    for (int i = n + t; i < 1 << log2; i += kSampleThreads) list[i] = 0;
+    sample_sort(list, log2);
+    unsigned long long entry[2];
+    double w[2], before[1] = {0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        entry[j] = 2 * t + j < k ? list[2 * t + j] : 0;
+        w[j] = entry[j] ? weight(Key::value(static_cast<uint32_t>(entry[j] >> 32))) : 0.0;
+        before[0] += w[j];
+    }
+    double sum = before[0];
+    sample_block_before<1>(before, sh.wd);
+    if (t == kSampleThreads - 1) sh.total_d[0] = before[0] + sum;
+    if (t == 0) sh.bin = 0xffffffffu;
+    __syncthreads();
+    // predecessors within top_p of the sum, the first always; what is left is sorted by index
+    const double limit = top_p < 1.f ? (top_p > 0.f ? static_cast<double>(top_p) : 0.0) * sh.total_d[0] : INFINITY;
+    double ahead = before[0];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const bool kept = entry[j] != 0 && w[j] > 0 && w[j] >= min_p && (ahead <= limit || 2 * t + j == 0);
+        ahead += w[j];
+        if (2 * t + j < 1 << log2)
+            list[2 * t + j] = kept ? (entry[j] << 32) | (entry[j] >> 32) : 0;  // the inverted index leads
+    }
+    sample_sort(list, log2);
+    double sums[1] = {0};
+    int entries = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        entry[j] = 2 * t + j < 1 << log2 ? list[2 * t + j] : 0;
+        entries += entry[j] != 0;
+        w[j] = entry[j] ? weight(Key::value(static_cast<uint32_t>(entry[j]))) : 0.0;
+        sums[0] += w[j];
+    }
+    sum = sums[0];
+    sample_block_before<1>(sums, sh.wd);
+    if (t == kSampleThreads - 1) sh.total_d[0] = sums[0] + sum;
+    const int last = __syncthreads_count(entries > 0) + __syncthreads_count(entries > 1) - 1;
+    const double everything = sh.total_d[0];
+    float u = p.uniform[row];
+    u = u > 0.f ? u : 0.f;
+    const double target = static_cast<double>(u) * everything;
+    double run = sums[0];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        run += w[j];
+        if (entry[j] && (run > target || 2 * t + j == last)) atomicMin(&sh.bin, static_cast<unsigned>(2 * t + j));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        if (entry[j] && sh.bin == 2 * t + j) {
+            p.token[row] = 0xffffffffu - static_cast<uint32_t>(entry[j] >> 32);
+            if (p.logprob) p.logprob[row] = static_cast<float>(log(w[j] / everything));
+        }
+}
+
+// One row, by the CTAs of a cluster. `list` is room for kSampleList entries in shared memory.
 template <class T>
 __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
                                            int vectors_per_warp, int in_smem, const SampleParams& p, SampleShared& sh,
-                                           unsigned char* sample_slice, long long row) {
+                                           unsigned long long* list, unsigned char* sample_slice, long long row) {
     constexpr int VEC = RmsTile<T>::kVec;
     using Key = SampleKey<T>;
     constexpr int kBins = kSampleBins, PER = kSampleBinsPerThread;
@@ -343,6 +447,7 @@ __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long lo
         for (int j = 0; j < VEC; ++j) top = fmaxf(top, x[j]);
     }
     if (t < kSampleTable) sh.table[t] = exp2(t / static_cast<double>(kSampleTable));
+    if (t == 0) sh.listed = 0;
     for (int i = t; i < kBins; i += kSampleThreads) sh.hist[0][i] = sh.hist[1][i] = 0;
     {
         uint32_t k = __reduce_max_sync(0xffffffffu, Key::of(top));
@@ -452,6 +557,10 @@ __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long lo
     long long ties = 0;
     long long k = p.top_k ? (p.top_k_i64 ? static_cast<const long long*>(p.top_k)[row] : static_cast<const int*>(p.top_k)[row]) : p.top_k_all;
 
+    const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
+    const float min_row = p.min_p ? p.min_p[row] : p.min_p_all;
+    const double min_p = min_row > 0.f ? fminf(min_row, 1.f) : 0.0;
+
     // ---- 2., 4. top_k: the k-th value
     if (k > 0 && k < vocab) {
         uint32_t lo = 0, hi = 0;
@@ -475,12 +584,14 @@ __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long lo
                 if (run < k && k <= run + cs[j]) {
                     sh.bin = PER * t + j;
                     sh.before = run;
+                    sh.count = cs[j];
                 }
                 run += cs[j];
             }
             __syncthreads();
             const uint32_t b = sh.bin;
             above = sh.before;
+            const long long reached = above + sh.count;  // values down to the bracket's lowest
             if (b == kBins) break;
             all = false;
             if (shift == 0) {
@@ -489,6 +600,28 @@ __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long lo
             }
             if (shift < 0) {
                 bracket_of_bins(static_cast<int>(b), static_cast<int>(b), lo, hi);
+                if (reached <= kSampleList) {
+                    // few enough to be listed: the first CTA collects them and draws from the list
+                    const float low_end = Key::at_least(lo);
+                    const uint32_t listed = ptx::map_to_cta(ptx::smem_u32(&sh.listed), 0);
+                    for (int v = v0 + lane; v < v1; v += 32) {
+                        float x[VEC];
+                        fetch(v, x);
+                        if (largest(x) < low_end) continue;
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j)
+                            if (x[j] >= low_end) {
+                                const uint32_t index = static_cast<uint32_t>(static_cast<long long>(v) * VEC + j - head);
+                                const uint32_t n = atom_cluster_add(listed, 1);  // below `reached`: the histogram has counted them
+                                const unsigned long long entry = (static_cast<unsigned long long>(Key::of(x[j])) << 32) | (0xffffffffu - index);
+                                if (n < kSampleList) st_cluster_s64(ptx::map_to_cta(ptx::smem_u32(&list[n]), 0), static_cast<long long>(entry));
+                            }
+                    }
+                    __syncthreads();
+                    ptx::cluster_sync_all();
+                    if (rank == 0) sample_listed<T>(list, static_cast<int>(reached), static_cast<int>(k), weight, top_p, min_p, p, sh, row);
+                    return;
+                }
             } else {
                 hi -= b << shift;
                 lo = max(lo, hi - ((1u << shift) - 1u));
@@ -503,7 +636,6 @@ __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long lo
     }
 
     // ---- 2., 3., 4. top_p: the smallest value whose predecessors' weights stay within the limit
-    const float top_p = p.top_p ? p.top_p[row] : p.top_p_all;
     bool carry = false;  // whether this thread's weights above the bracket are summed already, as `carried`
     double carried = 0;
     float carry_low = 0, carry_high = 0;  // the bracket
@@ -734,9 +866,6 @@ __device__ __forceinline__ void sample_row(const T* __restrict__ logits, long lo
             }
         }
     }
-    const float min_row = p.min_p ? p.min_p[row] : p.min_p_all;
-    const double min_p = min_row > 0.f ? fminf(min_row, 1.f) : 0.0;
-
     // ---- 5. the kept weights by warp
     auto kept_weight = [&](float v) {
         const double w = weight(v);
@@ -839,7 +968,8 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
               const SampleParams p) {
     extern __shared__ __align__(16) unsigned char sample_slice[];
     __shared__ SampleShared sh;
-    sample_row<T>(logits, ld, vocab, n_ctas, vectors_per_warp, in_smem, p, sh, sample_slice, blockIdx.x / n_ctas);
+    sample_row<T>(logits, ld, vocab, n_ctas, vectors_per_warp, in_smem, p, sh, reinterpret_cast<unsigned long long*>(sample_slice),
+                  sample_slice + kSampleList * 8, blockIdx.x / n_ctas);
 }
 
 // Batches of bf16 rows, a CTA per row: a histogram with one bin per VALUE. A bin's weights are then known from its count,
@@ -877,8 +1007,8 @@ __device__ __forceinline__ int bin_of_value(uint32_t bits) {
 
 // sample_row from global memory, out of line.
 __device__ __noinline__ void sample_row_alone(const __nv_bfloat16* logits, long long ld, int vocab, int vectors_per_warp,
-                                              const SampleParams& p, SampleShared& sh, long long row) {
-    sample_row<__nv_bfloat16>(logits, ld, vocab, 1, vectors_per_warp, 0, p, sh, nullptr, row);
+                                              const SampleParams& p, SampleShared& sh, void* list, long long row) {
+    sample_row<__nv_bfloat16>(logits, ld, vocab, 1, vectors_per_warp, 0, p, sh, static_cast<unsigned long long*>(list), nullptr, row);
 }
 
 __global__ void __launch_bounds__(kSampleThreads, 2)
@@ -970,7 +1100,7 @@ sample_values_kernel(const __nv_bfloat16* __restrict__ logits, long long ld, int
         if (lane == 0) sh.wu[warp] = key;
     }
     if (__syncthreads_or(other)) {
-        sample_row_alone(logits, ld, vocab, static_cast<int>(share), p, sh, row);
+        sample_row_alone(logits, ld, vocab, static_cast<int>(share), p, sh, sample_slice, row);
         return;
     }
     long long members = 0;  // of this thread's bins
@@ -992,7 +1122,7 @@ sample_values_kernel(const __nv_bfloat16* __restrict__ logits, long long ld, int
         top = Key::value(key);
         if (top == INFINITY) {
             __syncthreads();  // all have read sh.wu
-            sample_row_alone(logits, ld, vocab, static_cast<int>(share), p, sh, row);
+            sample_row_alone(logits, ld, vocab, static_cast<int>(share), p, sh, sample_slice, row);
             return;
         }
     }
