@@ -129,6 +129,9 @@ def lib() -> ctypes.CDLL:
     return handle
 
 
+ERR_WS_TOO_SMALL = 3
+
+
 def check(code: int, what: str) -> None:
     if code != 0:
         msg = lib().lce_strerror(code).decode()

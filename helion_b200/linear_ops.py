@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import FLOAT_DTYPES, _DTYPE_CODE, _launch, _need_cuda, _need_dtype, _path_flags, _ptr, _workspace
+from .ops import FLOAT_DTYPES, _DTYPE_CODE, _launch_scratch, _need_cuda, _need_dtype, _path_flags, _ptr
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -81,10 +81,9 @@ def _forward(x, weight, bias, residual, act: int, save: bool):
         return out, pre
     flags = _flags(dtype)
     xp, wp = x2.data_ptr(), w2.data_ptr()
-    need = _lib.lib().lce_linear_forward_workspace_bytes(xp, ldx, wp, ldw, m, n, k, dtype, flags)
-    ws = _workspace(need, dev) if need else None
-    _launch("lce_linear_forward", dev, xp, ldx, wp, ldw, _ptr(b), _ptr(r2), ldr, out.data_ptr(), n, _ptr(pre), m, n, k, act,
-            dtype, _ptr(ws), need, flags)
+    _launch_scratch("lce_linear_forward",
+                    lambda: _lib.lib().lce_linear_forward_workspace_bytes(xp, ldx, wp, ldw, m, n, k, dtype, flags),
+                    dev, xp, ldx, wp, ldw, _ptr(b), _ptr(r2), ldr, out.data_ptr(), n, _ptr(pre), m, n, k, act, dtype, flags=flags)
     return out, pre
 
 
@@ -106,9 +105,9 @@ def _backward(dy, x, weight, pre, act: int, need_x: bool, need_w: bool, need_b: 
     db = torch.empty((n,), dtype=x.dtype, device=dev) if need_b else None
     flags = _flags(dtype)
     args = (dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw)
-    ws = _workspace(_lib.lib().lce_linear_backward_workspace_bytes(*args, m, n, k, act, dtype, flags), dev)
-    _launch("lce_linear_backward", dev, *args, _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db), m, n, k, act, dtype, ws.data_ptr(),
-            ws.numel(), flags)
+    _launch_scratch("lce_linear_backward",
+                    lambda: _lib.lib().lce_linear_backward_workspace_bytes(*args, m, n, k, act, dtype, flags),
+                    dev, *args, _ptr(pre), _ptr(dx), _ptr(dw), _ptr(db), m, n, k, act, dtype, flags=flags)
     return dx, dw, db
 
 

@@ -19,7 +19,7 @@ from __future__ import annotations
 import ctypes
 import os
 from threading import get_ident
-from typing import Any
+from typing import Any, Callable
 
 import torch
 
@@ -165,16 +165,31 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
-def _launch(what: str, device: torch.device, *args) -> None:
-    """The C-ABI call ``what`` with ``args`` and, last, the current stream of ``device``, which is made current for it;
-    the lean form of ``with _on_device(...): check(...)`` for calls that take a few microseconds in all."""
+def _call(what: str, device: torch.device, *args) -> int:
+    """The status of the C-ABI call ``what`` with ``args`` and, last, the current stream of ``device``, which is made
+    current for it; the lean form of ``with _on_device(...)`` for calls that take a few microseconds in all."""
     fn = getattr(_lib.lib(), what)
     index = device.index
     if index is None or index == torch.cuda.current_device():
-        code = fn(*args, _stream(device))
-    else:
-        with torch.cuda.device(device):
-            code = fn(*args, _stream(device))
+        return fn(*args, _stream(device))
+    with torch.cuda.device(device):
+        return fn(*args, _stream(device))
+
+
+def _launch(what: str, device: torch.device, *args) -> None:
+    code = _call(what, device, *args)
+    if code:
+        _lib.check(code, what)
+
+
+def _launch_scratch(what: str, size: Callable[[], int], device: torch.device, *args, flags: int) -> None:
+    """``what(*args, ws, ws_bytes, flags, stream)`` with the scratch that is there already; ``size()`` bytes are asked for
+    only where the call finds it too small, which it does before it launches anything."""
+    ws = None if torch.cuda.is_current_stream_capturing() else _ws_cache.get(_ws_key(device))
+    code = _call(what, device, *args, _ptr(ws), 0 if ws is None else ws.numel(), flags)
+    if code == _lib.ERR_WS_TOO_SMALL:
+        ws = _workspace(size(), device)
+        code = _call(what, device, *args, ws.data_ptr(), ws.numel(), flags)
     if code:
         _lib.check(code, what)
 
@@ -185,6 +200,10 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 _WS_CACHE_MAX = 32 << 20
 _ws_cache: dict[tuple[int, int, int], torch.Tensor] = {}
+
+
+def _ws_key(device: torch.device) -> tuple[int, int, int]:
+    return (device.index if device.index is not None else torch.cuda.current_device(), _stream(device), get_ident())
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
@@ -198,7 +217,7 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     nbytes = max(int(nbytes), 256)
     if nbytes > _WS_CACHE_MAX or torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index if device.index is not None else torch.cuda.current_device(), _stream(device), get_ident())
+    key = _ws_key(device)
     buf = _ws_cache.get(key)
     if buf is None or buf.numel() < nbytes:
         if len(_ws_cache) >= 64:  # streams come and go: do not let the cache grow without bound

@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes
 import math
 from array import array
+from functools import lru_cache
 from typing import Any
 
 import torch
@@ -194,6 +195,11 @@ def _qk_forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleav
     return q_out, k_out
 
 
+@lru_cache(maxsize=None)
+def _backward_bytes(dim: int) -> int:
+    return _lib.lib().lce_qk_norm_rope_backward_workspace_bytes(dim)
+
+
 class _QKNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, scale):
@@ -210,7 +216,7 @@ class _QKNormRope(torch.autograd.Function):
         dq, dk = torch.empty_like(q), torch.empty_like(k)
         dqw = torch.empty_like(q_weight) if ctx.needs_input_grad[2] else None
         dkw = torch.empty_like(k_weight) if ctx.needs_input_grad[3] else None
-        ws = _workspace(_lib.lib().lce_qk_norm_rope_backward_workspace_bytes(q.shape[-1]), q.device)
+        ws = _workspace(_backward_bytes(q.shape[-1]), q.device)
         rows = array("q", _row_fields(q, dq, gq, q_weight, dqw) + _row_fields(k, dk, gk, k_weight, dkw))
         at = rows.buffer_info()[0]
         _launch("lce_qk_norm_rope_backward", q.device, at, at + _ROW_BYTES, *_place(q, positions, frequencies), interleaved,
