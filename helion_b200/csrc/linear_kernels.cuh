@@ -732,7 +732,8 @@ repitch_kernel(const T* __restrict__ src, long long lds, T* __restrict__ dst, lo
 
 // dz = dy * act'(pre), rounded, and the column sums of the unrounded dz over this CTA's rows.
 // A CTA of 256 threads owns 32 x VEC columns and the row slab [slab * rows_per_slab, ...): 32 column groups x 8 rows
-// at a time, four of them in flight. Bound by the bytes: dy and pre in, dz out. partial: [slabs][cols] (nullptr: no sums);
+// at a time, four of them in flight. Bytes: dy and pre in, dz out; 8192 x 4096 bf16 with gelu takes 46 us for 201 MB, 0.67 of the
+// copy bandwidth (0.57 instructions a cycle and scheduler, the slope's), 3 CTAs an SM by registers. partial: [slabs][cols] (nullptr: no sums);
 // dz nullptr: sums only (no activation, dz = dy). Columns of dz up to its pitch, behind the last, are set to zero.
 template <class T, int ACT>
 __global__ void __launch_bounds__(256, 3)

@@ -23,6 +23,10 @@
 // dweight: every warp keeps sums for its columns in registers (vector form) or shared memory (row form) over all the
 // rows that it walks, each CTA adds its warps' sums in a fixed order and writes one partial row, and
 // head_dweight_kernel adds the partial rows in a fixed order. No atomics: the same bits on every run.
+//
+// Measured at 16384 tokens, heads of 128, bf16: rope of 40 heads 54 us a direction for 336 MB (0.95 of the copy bandwidth);
+// qk_norm_rope of 32 + 8 heads 65 us forward (0.79) and 103 us backward for 503 MB (0.75), where registers leave too few
+// warps for more loads in flight (24 % and 19 % of the warps), and 6 us for dweight.
 #pragma once
 
 #include "ptx.cuh"
@@ -72,7 +76,7 @@ struct RopePlan {
 };
 
 // cos and sin of an angle given as position x turns per position, times scale: the product and its fraction in 64 bits.
-// For 16-bit results the hardware's sine and cosine do (within 4e-7 for an angle in [-pi, pi]); they save most of a
+// For 16-bit results the hardware's sine and cosine do (within 4.2e-7 for an angle in [-pi, pi]); they save most of a
 // token's set-up.
 template <bool FAST>
 __device__ __forceinline__ float2 rope_angle(double pos, double turns_per_position, float scale, float sin_sign) {

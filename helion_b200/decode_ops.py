@@ -189,7 +189,7 @@ def sampling_distribution(hidden: torch.Tensor, weight: torch.Tensor, *, tempera
     """``(indices, probs)``, each ``[..., m]``: the tokens that can be drawn for every row and their probabilities
     (0 for masked ones; ``-1`` indices only carry probability 0) under the reference's
     sampling rule - repetition penalty, temperature, top-k, nucleus (top-p), multinomial draw
-    (``sample_next_token``, examples/common.py:263-306) - computed from at most ``max_candidates`` (<= 64)
+    (``sample_next_token``, examples/common.py:263-306; on logits that exist, ``sample_logits``) - computed from at most ``max_candidates`` (<= 64)
     candidates per row that ``topk_head`` selects, instead of from ``V`` materialised logits.
 
     What makes that exact: with ``top_k`` in 1..64 only the ``top_k`` best survive the reference's mask, so

@@ -3,7 +3,7 @@ GPU only.
 
 Tolerances, from arithmetic. A result is rounded once: half a unit, eps / 2 relative. Before that, in 32 bits:
 an angle's fraction of a turn is rounded to 24 bits (2 pi x 0.5 x 2^-25 < 1e-7 in angle), cos and sin are good to a few
-2^-24, and the rotation adds three roundings: below 6e-7 of the pair's magnitudes (|a| + |b|, at most twice the row's
+2^-24 (the hardware's, for 16-bit types, to 2^-21.2 = 4.2e-7), and the rotation adds three roundings: below 6e-7 of the pair's magnitudes (|a| + |b|, at most twice the row's
 largest). A row's sum of squares of up to 1024 terms passes through at most 37 additions per lane and butterfly, 2.2e-6
 relative, half of that in rstd, which adds 2e-7 of its own: 2e-6 of a normalised element. The backward combines
 two such sums: 1e-5 of the magnitudes that it subtracts. dweight adds at most a few hundred terms in sequence:
