@@ -406,3 +406,46 @@ def test_threads_that_share_a_stream():
     for t in threads:
         t.join(120)
     assert not any(t.is_alive() for t in threads) and not wrong, wrong
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "on_cpu"])
+def test_saved_tensors_that_move(how):
+    """Activation checkpointing and saved tensors kept on the host: the backward pass sees other tensors than the forward
+    saved, at other addresses, and must give the same bits."""
+    from torch.utils.checkpoint import checkpoint
+
+    dtype = torch.bfloat16
+    w, _, x, _, positions = _train_inputs(dtype, 2, 24, HIDDEN, HEADS, KV, DIM, FFN, 60)
+    freq, _ = helion_b200.rope_frequencies(DIM, theta=10000.0)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w["qkv"], w["qkv_bias"], w["qn"], w["kn"])]
+
+    def block(x, weight, bias, qn, kn):
+        heads = helion_b200.linear(x, weight, bias, activation="gelu").unflatten(-1, (HEADS + 2 * KV, DIM))
+        q, k = helion_b200.qk_norm_rope(heads[:, :, :HEADS], heads[:, :, HEADS:HEADS + KV], qn, kn, positions.clone(), freq.clone())
+        return q, k, helion_b200.rope(heads[:, :, HEADS + KV:], positions.clone(), freq.clone())
+
+    plain = block(*leaves)
+    dys = [torch.randn(t.shape, generator=_gen(61), device=DEV).to(dtype) for t in plain]
+    expected = torch.autograd.grad(plain, leaves, dys)
+    if how == "checkpoint":
+        outs = checkpoint(block, *leaves, use_reentrant=False)
+    else:
+        with torch.autograd.graph.save_on_cpu():
+            outs = block(*leaves)
+    noise = [torch.randn(1 << 16, device=DEV) for _ in range(8)]  # takes the addresses that were freed
+    got = torch.autograd.grad(outs, leaves, dys)
+    assert len(noise) == 8
+    for a, b in zip([*outs, *got], [*plain, *expected]):
+        assert torch.equal(a, b)
+
+
+def test_inference_mode():
+    w = _weights(torch.bfloat16, 70)
+    head, x, position, keys, values, u = _decode_inputs(4, 16, torch.bfloat16, 71)
+    freq, _ = helion_b200.rope_frequencies(DIM, theta=10000.0)
+    results = []
+    for guard in (torch.no_grad, torch.inference_mode):
+        with guard():
+            at = _decode_step(w, head, x.clone(), position, freq, keys.clone(), values.clone(), u)
+            results.append([at["token"].clone(), at["logprob"].clone(), at["logits"].clone()])
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -311,3 +311,24 @@ def test_agrees_with_the_sampling_head_on_its_candidates():
         for i in range(6):
             at = (idx[i] == token[i]).nonzero()[0, 0]
             assert abs(float(lp[i].exp()) - float(probs[i, at])) <= 1e-4
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("equal", [1, 2, 3, 511, 1023, 1024, 1025])
+def test_lists_of_candidates(dtype, equal):
+    """A top_k whose candidates are few enough to be listed, up to and past the list's 1024: `equal` logits share the
+    k-th value, so the lower indices are kept; some lie above, some far below."""
+    vocab = 6007
+    g = _gen(90 + equal)
+    order = torch.randperm(vocab, generator=g, device=DEV)
+    row = torch.full((vocab,), -3.0, device=DEV)
+    row[order[:equal]] = 2.0
+    above = [] if equal >= 1023 else [2.5, 3.0, 3.0, 4.0]
+    for i, v in enumerate(above):
+        row[order[equal + i]] = v
+    row[order[equal + 10:equal + 500]] = -INF
+    ks = sorted({1, 2, max(1, equal // 2), equal, equal + len(above), equal + len(above) + 1})
+    u = torch.linspace(0, 1, len(ks), device=DEV)
+    logits = row.to(dtype).expand(len(ks), vocab).contiguous()
+    _check(logits, u, top_k=ks)
+    _check(logits, u, temperature=0.6, top_k=ks, top_p=[0.3 + 0.1 * (i % 6) for i in range(len(ks))], min_p=0.1)
