@@ -67,7 +67,7 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 
 def _forward(x, weight, bias, residual, act: int, save: bool):
-    """(out [M, N], pre or None) for x [..., K]."""
+    """(out [..., N], pre [M, N padded] or None) for x [..., K]."""
     dtype, dev = _DTYPE_CODE[x.dtype], x.device
     x2, ldx = _rows(x)
     w2, ldw = _rows(weight)
@@ -75,7 +75,7 @@ def _forward(x, weight, bias, residual, act: int, save: bool):
     m, k = x2.shape
     n = w2.shape[0]
     b = bias.contiguous() if bias is not None else None
-    out = torch.empty((m, n), dtype=x.dtype, device=dev)
+    out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
     pre = torch.empty((m, (n + 7) // 8 * 8), dtype=x.dtype, device=dev) if save and act else None
     if m == 0:
         return out, pre
@@ -87,22 +87,26 @@ def _forward(x, weight, bias, residual, act: int, save: bool):
     return out, pre
 
 
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _flags(dtype: int) -> int:
     flags = _path_flags()
     return flags & ~_lib.FLAG_FORCE_TC if dtype == _lib.DTYPE_F32 else flags  # fp32 has no tensor-core path
 
 
 def _backward(dy, x, weight, pre, act: int, need_x: bool, need_w: bool, need_b: bool):
-    """(dx [M, K], dw [N, K], dbias [N]), each or None."""
+    """(dx, dw, dbias), each or None. Few calls of torch: in autograd's thread each takes several microseconds."""
     dtype, dev = _DTYPE_CODE[x.dtype], x.device
     dy2, ldy = _rows(dy)
     x2, ldx = _rows(x)
     w2, ldw = _rows(weight)
     m, n = dy2.shape
     k = w2.shape[1]
-    dx = torch.empty((m, k), dtype=x.dtype, device=dev) if need_x else None
-    dw = torch.empty((n, k), dtype=x.dtype, device=dev) if need_w else None
-    db = torch.empty((n,), dtype=x.dtype, device=dev) if need_b else None
+    dx = _empty_like(x) if need_x else None
+    dw = _empty_like(weight) if need_w else None
+    db = x.new_empty(n) if need_b else None
     flags = _flags(dtype)
     args = (dy2.data_ptr(), ldy, x2.data_ptr(), ldx, w2.data_ptr(), ldw)
     _launch_scratch("lce_linear_backward",
@@ -117,7 +121,7 @@ class _Linear(torch.autograd.Function):
         out, pre = _forward(x, weight, bias, residual, act, True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
-        return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[1])
+        return out
 
     @staticmethod
     @once_differentiable
@@ -128,7 +132,6 @@ class _Linear(torch.autograd.Function):
         dx = dw = db = None
         if need[0] or need[1] or need[2]:
             dx, dw, db = _backward(dy, x, weight, pre, ctx.act, need[0], need[1], need[2])
-            dx = dx.view(x.shape) if dx is not None else None
         return dx, dw, db, (dy if need[3] else None), None
 
 
@@ -145,5 +148,4 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
             (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         return _Linear.apply(x, weight, bias, residual, act)
-    out = _forward(x, weight, bias, residual, act, False)[0]
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[1])
+    return _forward(x, weight, bias, residual, act, False)[0]
