@@ -10,7 +10,7 @@ namespace {
 // The row pitch of what a forward saves for its backward: whole 16-byte vectors whatever the type.
 inline long long pre_pitch(long long N) { return cdiv(N, 8) * 8; }
 
-constexpr long long kDzCtas = 444;  // CTAs that the column sums of the backward aim for (3 per SM on 148 SMs, one wave)
+constexpr long long kDzCtas = 592;  // CTAs that the column sums of the backward aim for (4 per SM on 148 SMs, one wave)
 
 // Scratch of one product C[M, N] = A[M, K] B[N, K]^T: slabs of a split contraction.
 struct ProductPlan {

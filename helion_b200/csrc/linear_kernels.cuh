@@ -732,14 +732,15 @@ repitch_kernel(const T* __restrict__ src, long long lds, T* __restrict__ dst, lo
 
 // dz = dy * act'(pre), rounded, and the column sums of the unrounded dz over this CTA's rows.
 // A CTA of 256 threads owns 32 x VEC columns and the row slab [slab * rows_per_slab, ...): 32 column groups x 8 rows
-// at a time, four of them in flight. Bytes: dy and pre in, dz out; 8192 x 4096 bf16 with gelu takes 46 us for 201 MB, 0.67 of the
-// copy bandwidth (0.57 instructions a cycle and scheduler, the slope's), 3 CTAs an SM by registers. partial: [slabs][cols] (nullptr: no sums);
+// at a time, two of them in flight. Bytes: dy and pre in, dz out; 8192 x 4096 bf16, 201 MB, with the bias gradient and on a
+// cold cache: 47 us with gelu, 40 with relu (0.77 of the copy bandwidth). Three CTAs an SM with four rows in flight took 52
+// and 45, two with four 48 and 42, two with eight (which spill) 69 and 54, five with two (likewise) 56 and 50. partial: [slabs][cols] (nullptr: no sums);
 // dz nullptr: sums only (no activation, dz = dy). Columns of dz up to its pitch, behind the last, are set to zero.
 template <class T, int ACT>
-__global__ void __launch_bounds__(256, 3)
+__global__ void __launch_bounds__(256, 4)
 linear_dz_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ pre, long long ldp, T* __restrict__ dz, long long ldz,
                  float* __restrict__ partial, long long rows, int cols, long long rows_per_slab) {
-    constexpr int U = 4, VEC = 16 / sizeof(T);
+    constexpr int U = 2, VEC = 16 / sizeof(T);
     __shared__ float sums[8][32 * VEC + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = (blockIdx.x * 32 + lane) * VEC;
