@@ -449,3 +449,52 @@ def test_inference_mode():
             at = _decode_step(w, head, x.clone(), position, freq, keys.clone(), values.clone(), u)
             results.append([at["token"].clone(), at["logprob"].clone(), at["logits"].clone()])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_offsets_beyond_32_bits():
+    """Tensors of more than 2^31 elements: the last rows, whose offsets pass 32 bits, are those of a small call."""
+    g = _gen(80)
+    m, k, n = 70001, 64, 32768
+    x = torch.randn(m, k, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    w = (torch.randn(n, k, generator=g, device=DEV) / 8).bfloat16().requires_grad_(True)
+    b = torch.randn(n, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    y = helion_b200.linear(x, w, b, activation="relu")
+    assert y.numel() > 2 ** 31
+    dy = torch.empty_like(y).normal_(generator=g)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    rows, cols = slice(m - 300, m), [0, 1, 777, n - 1]
+    tail = helion_b200.linear(x.detach()[rows].clone(), w.detach(), b.detach(), activation="relu")
+    assert torch.equal(y.detach()[rows], tail)
+    xd, wd, bd = (t.detach().double() for t in (x, w, b))
+
+    def slopes(xs, ws, bs, dys):  # dz, and how far it may be off where z is within its rounding of 0
+        z = xs @ ws.t() + bs
+        unsure = z.abs() <= (k + 1) * U * (xs.abs() @ ws.abs().t() + bs.abs())
+        return dys.double() * (z > 0), dys.double().abs() * unsure
+
+    dz, off = slopes(xd[rows], wd, bd, dy[rows])
+    _inside(dx[rows], dz @ wd, (n + 1) * U * (dz.abs() @ wd.abs()) + off @ wd.abs(), "dx")
+    dz, off = slopes(xd, wd[cols], bd[cols], dy[:, cols])
+    _inside(dw[cols], dz.t() @ xd, (m + 1) * U * (dz.abs().t() @ xd.abs()) + off.t() @ xd.abs(), "dw")
+    _inside(db[cols], dz.sum(0), (m + 1) * U * dz.abs().sum(0) + off.sum(0), "dbias")
+    del y, dy, dx, dw, db, dz, off, tail
+
+    heads = torch.empty(1, 66000, 256, 128, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    assert heads.numel() > 2 ** 31
+    positions = torch.arange(66000, device=DEV)[None]
+    freq, _ = helion_b200.rope_frequencies(128)
+    out = helion_b200.rope(heads, positions, freq)
+    part = slice(65900, 66000)
+    assert torch.equal(out[:, part], helion_b200.rope(heads[:, part].clone(), positions[:, part], freq))
+    weight = torch.ones(128, dtype=torch.bfloat16, device=DEV)
+    q, kk = helion_b200.qk_norm_rope(heads, heads[:, :, :2], weight, weight, positions, freq)
+    small = helion_b200.qk_norm_rope(heads[:, part].clone(), heads[:, part, :2].clone(), weight, weight, positions[:, part], freq)
+    assert torch.equal(q[:, part], small[0]) and torch.equal(kk[:, part], small[1])
+    del out, q, kk, small
+
+    for dtype in (torch.bfloat16, torch.float16):
+        logits = heads.view(16896, -1).to(dtype)  # 128000 tokens
+        u = torch.rand(16896, generator=g, device=DEV)
+        token, logprob = helion_b200.sample_logits(logits, u, top_p=0.9, return_logprob=True)
+        last, last_logprob = helion_b200.sample_logits(logits[-70:].clone(), u[-70:], top_p=0.9, return_logprob=True)
+        assert torch.equal(token[-70:], last) and torch.equal(logprob[-70:], last_logprob)
