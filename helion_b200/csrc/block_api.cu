@@ -218,10 +218,12 @@ constexpr long long kSampleMaxSliceBytes = 160 << 10;   // beyond it a CTA re-re
 // is worth the cluster's barriers.
 // bf16 batches that take sample_values_kernel, a CTA per row. top_p 0.95, sample_kernel against it, us, at 128256 logits:
 // 24 rows 52 / 72, 48 rows 84 / 72, 148 rows 160 / 74, 256 rows 250 / 94; at 50257: 24 rows 37 / 49, 48 rows 61 / 49; at
-// 8003: 148 rows 27 / 32, 256 rows 47 / 35. Rows without filters, of which sample_kernel only needs the maximum and the
-// weights: 48 rows of 128256 43 / 63, 256 rows 125 / 88.
-constexpr long long kSampleValueRows = 40, kSampleValueRowsUnfiltered = 128;
-constexpr long long kSampleValueLogits = 2000000;
+// 8003: 148 rows 27 / 32, 256 rows 47 / 35, 16384 rows 1323 / 1186; below that a row's bins cost as much as they save (4000:
+// 1055 / 1110). Rows without filters, of which sample_kernel only needs the maximum and the weights: 48 rows of 128256
+// 43 / 63, 256 rows 125 / 88, 256 rows of 50257 64 / 53, 1024 rows of 8000 57 / 84.
+inline bool takes_values(long long rows, long long vocab, bool filtered) {
+    return filtered ? rows >= 40 && vocab >= 8000 && rows * vocab >= 2000000 : rows >= 128 && vocab >= 32768;
+}
 
 // A CTA per row, for batches of bf16 rows.
 int launch_sample_values(const DeviceInfo& d, const __nv_bfloat16* logits, long long ld, long long rows, long long vocab,
@@ -245,8 +247,7 @@ int launch_sample(const DeviceInfo& d, const void* logits, long long ld, long lo
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         const long long groups = cdiv(n_vec, static_cast<long long>(kSampleWarps) * kValueChunk);
         const bool filtered = p.top_k || p.top_p || (p.top_k_all > 0 && p.top_k_all < vocab) || p.top_p_all < 1.f;
-        if (rows >= (filtered ? kSampleValueRows : kSampleValueRowsUnfiltered) && rows * vocab >= kSampleValueLogits &&
-            groups * kSampleWarps <= kValueMaxChunks)
+        if (takes_values(rows, vocab, filtered) && groups * kSampleWarps <= kValueMaxChunks)
             return launch_sample_values(d, static_cast<const T*>(logits), ld, rows, vocab, static_cast<int>(groups), p, s);
     }
     int ctas = 1;
