@@ -312,7 +312,7 @@ inline int choose_k_splits(long long M, long long Nn, long long K, int cg) {
     return static_cast<int>(s);
 }
 
-template <class T, class Epi>
+template <class T, class Epi, int TS = 128>
 int launch_simt(const DeviceInfo& d, const Mat& a, bool a_mn, const Mat& b, bool b_mn, long long M,
                 long long Nn, long long K, const typename Epi::Params& ep, cudaStream_t stream, int k_splits = 1) {
     SimtOperand<T> A, B;
@@ -330,10 +330,11 @@ int launch_simt(const DeviceInfo& d, const Mat& a, bool a_mn, const Mat& b, bool
     B.stride_k = b_mn ? b.pitch_elems : 1;
     B.extent_mn = static_cast<int>(mn_extent(b, b_mn, Nn));
     B.extent_k = static_cast<int>(k_extent(b, b_mn));
-    const long long m_tiles = cdiv(M, kBM), n_tiles = cdiv(Nn, kSimtBN);
+    const long long m_tiles = cdiv(M, TS), n_tiles = cdiv(Nn, TS);
     if (m_tiles * n_tiles > 0x7fffffffll) return LCE_ERR_TOO_LARGE;
     if (m_tiles * n_tiles == 0 || K == 0) return LCE_OK;
-    const long long cap = static_cast<long long>(d.sm_count) * 4;
+    constexpr int kThreads = SimtTile<TS>::kThreads;
+    const long long cap = static_cast<long long>(d.sm_count) * (4 * 128 / TS);
     const long long work = m_tiles * n_tiles * k_splits;
     const int grid = static_cast<int>(work < cap ? work : cap);
     // one operand's zeros make up for what the other does not have
@@ -349,14 +350,14 @@ int launch_simt(const DeviceInfo& d, const Mat& a, bool a_mn, const Mat& b, bool
         };
         const int am = mode(A), bm = mode(B);
 #define LCE_SIMT_GO(AM, BM) \
-    gemm_simt_kernel<float, Epi, AM, BM><<<grid, kSimtThreads, 0, stream>>>(A, B, k, mt, nt, k_splits, ep), launched = true
+    gemm_simt_kernel<float, Epi, AM, BM, TS><<<grid, kThreads, 0, stream>>>(A, B, k, mt, nt, k_splits, ep), launched = true
         if (am == kSimtVecK && bm == kSimtVecK) LCE_SIMT_GO(kSimtVecK, kSimtVecK);
         else if (am == kSimtVecK && bm == kSimtVecMN) LCE_SIMT_GO(kSimtVecK, kSimtVecMN);
         else if (am == kSimtVecMN && bm == kSimtVecK) LCE_SIMT_GO(kSimtVecMN, kSimtVecK);
         else if (am == kSimtVecMN && bm == kSimtVecMN) LCE_SIMT_GO(kSimtVecMN, kSimtVecMN);
 #undef LCE_SIMT_GO
     }
-    if (!launched) gemm_simt_kernel<T, Epi><<<grid, kSimtThreads, 0, stream>>>(A, B, k, mt, nt, k_splits, ep);
+    if (!launched) gemm_simt_kernel<T, Epi, kSimtGeneric, kSimtGeneric, TS><<<grid, kThreads, 0, stream>>>(A, B, k, mt, nt, k_splits, ep);
     LCE_COUNT_LAUNCH();
     return (cuda_failed(cudaGetLastError()) ? LCE_ERR_CUDA : LCE_OK);
 }

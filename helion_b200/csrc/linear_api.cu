@@ -18,6 +18,7 @@ struct ProductPlan {
     int cg, splits, bn;
     long long slab_floats;
     size_t bytes;
+    bool small_tiles;  // CUDA-core GEMM: 64 x 64 tiles
 };
 
 ProductPlan plan_product(long long M, long long N, long long K, int dtype, unsigned flags) {
@@ -28,6 +29,23 @@ ProductPlan plan_product(long long M, long long N, long long K, int dtype, unsig
     p.splits = p.use_tc ? choose_k_splits(M, N, K, p.cg) : choose_k_splits_simt(M, N, K);
     p.slab_floats = cdiv(M, 2 * kBM) * 2 * cdiv(N, p.bn) * kBM * p.bn;
     p.bytes = p.splits > 1 ? align_up(static_cast<size_t>(p.splits) * p.slab_floats * sizeof(float), 256) : 0;
+    p.small_tiles = false;
+    return p;
+}
+
+// The forward of a call whose relu slopes are saved. A slope is the sign of z, and at a z within its rounding of 0 the order
+// of the sum decides it: one such element in 777 x 1003 shifts fp32 gradients by 6e-4 of their norm, thirty times what
+// rounding does. So an fp32 z whose sign is saved is one chain of fused multiply-adds over the contraction, whatever the number of
+// tokens: a row gets the same slopes in every batch, and those of an unsplit fp32 product elsewhere. Where the contraction would be
+// split, tiles of 64 x 64 fill the GPU instead: 777 x 520 x 1003 46 us (split 35, unsplit tiles of 128 x 128 82); a long
+// contraction with few tiles pays most, 128 x 4096 x 128 167 us against 26.
+ProductPlan plan_forward(long long M, long long N, long long K, int act, const void* pre, int dtype, unsigned flags) {
+    ProductPlan p = plan_product(M, N, K, dtype, flags);
+    if (p.splits > 1 && act == LCE_ACT_RELU && pre && dtype == LCE_DTYPE_F32) {
+        p.splits = 1;
+        p.bytes = 0;
+        p.small_tiles = true;
+    }
     return p;
 }
 
@@ -120,7 +138,13 @@ int product(const DeviceInfo& d, const ProductPlan& p, const Operand& a, const O
         }
     } else {
         using Epi = EpiLinear<T, kActAny, false>;
-        rc = launch_simt<T, Epi>(d, am, A_MN, bm, B_MN, M, N, K, epilogue_params<Epi>(p, tail, scratch), s, p.splits);
+        const typename Epi::Params ep = epilogue_params<Epi>(p, tail, scratch);
+        if constexpr (std::is_same<T, float>::value && !A_MN && !B_MN) {
+            rc = p.small_tiles ? launch_simt<T, Epi, 64>(d, am, A_MN, bm, B_MN, M, N, K, ep, s)
+                               : launch_simt<T, Epi>(d, am, A_MN, bm, B_MN, M, N, K, ep, s, p.splits);
+        } else {
+            rc = launch_simt<T, Epi>(d, am, A_MN, bm, B_MN, M, N, K, ep, s, p.splits);
+        }
     }
     if (rc == LCE_OK && p.splits > 1) {
         const long long quads = cdiv(N, 16) * cdiv(M, 16) * 64;
@@ -314,7 +338,7 @@ int lce_linear_forward(const void* x, int64_t ldx, const void* w, int64_t ldw, c
     if (M == 0) return LCE_OK;
     if (!x || !w || !out) return LCE_ERR_ARG;
     const Operand xo = plan_operand(x, ldx, M, K, dtype, flags), wo = plan_operand(w, ldw, N, K, dtype, flags);
-    const ProductPlan p = plan_product(M, N, K, dtype, flags);
+    const ProductPlan p = plan_forward(M, N, K, act, pre, dtype, flags);
     const bool decode = decodes(M, dtype, flags);
     const size_t need = forward_bytes(xo, wo, p, decode);
     if (need > 0 && (!ws || ws_bytes < need)) return LCE_ERR_WS_TOO_SMALL;
