@@ -108,6 +108,13 @@ def _rows_readable(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _heads_like(x: torch.Tensor) -> torch.Tensor:
+    """An output of ``x``'s shape whose last dimension is contiguous, as the kernels write it: in ``x``'s layout where that
+    is dense. Of an overlapping view (``unfold``) ``empty_like`` may order the dimensions otherwise."""
+    out = torch.empty_like(x)
+    return out if out.stride(-1) == 1 or x.shape[-1] == 1 else x.new_empty(x.shape)
+
+
 # ----------------------------------------------------------------------------------------------
 # what crosses the C ABI
 # ----------------------------------------------------------------------------------------------
@@ -144,7 +151,7 @@ def _place(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor):
 # ----------------------------------------------------------------------------------------------
 def _rope(x, positions, frequencies, interleaved, scale, inverse):
     x = _rows_readable(x)
-    out = torch.empty_like(x)
+    out = _heads_like(x)
     rows = array("q", _row_fields(x, out))
     _launch("lce_rope", x.device, rows.buffer_info()[0], *_place(x, positions, frequencies), interleaved, scale, inverse,
             _DTYPE_CODE[x.dtype])
@@ -187,7 +194,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
 # qk_norm_rope
 # ----------------------------------------------------------------------------------------------
 def _qk_forward(q, k, q_weight, k_weight, positions, frequencies, eps, interleaved, scale):
-    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    q_out, k_out = _heads_like(q), _heads_like(k)
     rows = array("q", _row_fields(q, q_out, None, q_weight) + _row_fields(k, k_out, None, k_weight))
     at = rows.buffer_info()[0]
     _launch("lce_qk_norm_rope_forward", q.device, at, at + _ROW_BYTES, *_place(q, positions, frequencies), interleaved, scale,
@@ -213,7 +220,7 @@ class _QKNormRope(torch.autograd.Function):
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
         eps, interleaved, scale = ctx.how
         gq, gk = (_rows_readable(g) for g in grad_outputs)
-        dq, dk = torch.empty_like(q), torch.empty_like(k)
+        dq, dk = _heads_like(q), _heads_like(k)
         dqw = torch.empty_like(q_weight) if ctx.needs_input_grad[2] else None
         dkw = torch.empty_like(k_weight) if ctx.needs_input_grad[3] else None
         ws = _workspace(_backward_bytes(q.shape[-1]), q.device)
