@@ -14,7 +14,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from .ops import (FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _check_reduction, _need_cuda, _need_dtype, _on_device,
+from .ops import (FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _check_reduction, _differentiated, _need_cuda, _need_dtype, _on_device,
                   _stream, _workspace)
 
 _OP = "for tritium.cross_entropy"
@@ -125,7 +125,7 @@ def cross_entropy(logits: torch.Tensor, target: torch.Tensor, *, reduction: str 
                   ignore_index: int = -100) -> torch.Tensor:
     """Cross-entropy of 2-D ``logits[N, V]`` against ``target[N]`` without a materialised softmax
     (reference :708-713): 0-dim float32 mean by default."""
-    if not (torch.is_grad_enabled() and logits.requires_grad):
+    if not _differentiated(logits):
         loss, _ = _forward(logits, target, reduction, ignore_index)
         return loss
     return _CrossEntropy.apply(logits, target, reduction, ignore_index)

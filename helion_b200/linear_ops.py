@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import FLOAT_DTYPES, _DTYPE_CODE, _launch_scratch, _need_cuda, _need_dtype, _path_flags, _ptr
+from .ops import FLOAT_DTYPES, _DTYPE_CODE, _differentiated, _launch_scratch, _need_cuda, _need_dtype, _path_flags, _ptr
 
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -145,7 +145,6 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     pitch; inputs whose elements are not contiguous are copied first. fp32 is computed in fp32 throughout. Differentiable
     in ``x``, ``weight``, ``bias`` and ``residual``; sums are formed in a fixed order."""
     act = _check(x, weight, bias, activation, residual)
-    if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
-            (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
+    if _differentiated(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, act)
     return _forward(x, weight, bias, residual, act, False)[0]

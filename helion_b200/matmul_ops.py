@@ -13,7 +13,8 @@ from typing import Any
 import torch
 
 from . import _lib
-from .ops import FLOAT_DTYPES, _DTYPE_CODE, _need_cuda, _need_dtype, _on_device, _path_flags, _stream, _workspace
+from .ops import FLOAT_DTYPES, _DTYPE_CODE, _differentiated, _need_cuda, _need_dtype, _on_device, _path_flags, _stream, \
+    _workspace
 
 
 def _check_matmul_inputs(a: torch.Tensor, b: torch.Tensor) -> tuple[int, int, int]:
@@ -88,7 +89,7 @@ class _MatMul(torch.autograd.Function):
 
 def matmul(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """Return the matrix product ``a @ b`` with autograd support (reference :336-340)."""
-    if not (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad)):
+    if not _differentiated(a, b):
         return _product(a, b)
     return _MatMul.apply(a, b)
 

@@ -16,7 +16,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from .ops import FLOAT_DTYPES, _DTYPE_CODE, _need_cuda, _need_dtype, _on_device, _stream, _workspace
+from .ops import FLOAT_DTYPES, _DTYPE_CODE, _differentiated, _need_cuda, _need_dtype, _on_device, _stream, _workspace
 
 MAX_RMSNORM_HIDDEN_NEXT_POW2 = 65536
 
@@ -154,14 +154,10 @@ class _ResidualRMSNorm(torch.autograd.Function):
         return (dz if ctx.needs_input_grad[0] else None), (dz if ctx.needs_input_grad[1] else None), dweight, None
 
 
-def _autograd(*tensors: torch.Tensor) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
-
-
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
     """``x * rsqrt(mean(x**2) + eps) * weight`` over the last dimension (reference :737-746)."""
     check_inputs(x, weight)
-    if not _autograd(x, weight):
+    if not _differentiated(x, weight):
         return _forward(x, None, weight, eps, False)[0]
     return _RMSNorm.apply(x, weight, eps)
 
@@ -182,7 +178,7 @@ def residual_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
     """``(rmsnorm(x + residual), x + residual)`` in one pass (reference :749-778)."""
     check_inputs(x, weight)
     _check_residual(x, residual)
-    if not _autograd(x, residual, weight):
+    if not _differentiated(x, residual, weight):
         out, res_out, _ = _forward(x, residual, weight, eps, False)
         return out, res_out
     return _ResidualRMSNorm.apply(x, residual, weight, eps)

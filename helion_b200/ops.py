@@ -22,6 +22,7 @@ from threading import get_ident
 from typing import Any, Callable
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, grad_norm, parallel
 
@@ -117,6 +118,18 @@ def _check_reduction(reduction: str) -> int:
     if reduction not in _lib.REDUCTIONS:
         raise ValueError(f"reduction must be one of 'none', 'mean', 'sum'; got {reduction!r}.")
     return _lib.REDUCTIONS[reduction]
+
+
+def _differentiated(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call has to go through its autograd function: a gradient is asked for, or an input carries a forward-mode
+    tangent, which a launch on raw pointers would drop without a word and the function refuses."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level < 0:  # no level is open, torch.func.jvp's included
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 # ----------------------------------------------------------------------------------------------
@@ -521,7 +534,7 @@ def linear_cross_entropy(
     this rank's contiguous vocabulary shard (rows ``vocab_start ..``, default ``rank * V_local``) and every
     rank returns the same loss.
     """
-    if not (torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)):
+    if not _differentiated(hidden, weight):
         loss, _ = _forward(hidden, weight, target, reduction, ignore_index, process_group, vocab_start)
         return loss
     return _LinearCrossEntropy.apply(hidden, weight, target, reduction, ignore_index, process_group, vocab_start)

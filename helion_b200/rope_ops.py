@@ -24,7 +24,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _launch, _need_cuda, _need_dtype, _workspace
+from .ops import FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _differentiated, _launch, _need_cuda, _need_dtype, _workspace
 
 MAX_HEAD_DIM = 1024
 _SCALINGS = (None, "linear", "ntk", "yarn")
@@ -185,7 +185,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, *,
     Differentiable in ``x``; the backward pass is the same kernel turning the other way."""
     _check_heads("x", x)
     _check_positions(x.shape, x.device, positions, frequencies)
-    if x.requires_grad and torch.is_grad_enabled():
+    if _differentiated(x):
         return _Rope.apply(x, positions, frequencies, bool(interleaved), float(scale), False)
     return _rope(x, positions, frequencies, bool(interleaved), float(scale), False)
 
@@ -263,6 +263,6 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     if not eps >= 0:
         raise ValueError("eps must not be negative.")
     q, k = _rows_readable(q), _rows_readable(k)
-    if (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad) and torch.is_grad_enabled():
+    if _differentiated(q, k, q_weight, k_weight):
         return _QKNormRope.apply(q, k, q_weight, k_weight, positions, frequencies, float(eps), bool(interleaved), float(scale))
     return _qk_forward(q, k, q_weight, k_weight, positions, frequencies, float(eps), bool(interleaved), float(scale))
