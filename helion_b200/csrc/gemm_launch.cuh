@@ -22,6 +22,15 @@ inline PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 // The current device with everything that the GEMM cores need (status word, completion counters, tensor-map encoder).
 int device_info(DeviceInfo** out);
 
+// Sets the wait limit and the announcement hook (ptx.cuh) of the including source file, whose own they are.
+static int set_debug_waits(unsigned long long limit_ns, unsigned announce_extra_bytes) {
+    if (cuda_failed(cudaMemcpyToSymbol(ptx::g_wait_limit_ns, &limit_ns, sizeof(limit_ns))) ||
+        cuda_failed(cudaMemcpyToSymbol(ptx::g_debug_announce_extra, &announce_extra_bytes, sizeof(announce_extra_bytes))))
+        return LCE_ERR_CUDA;
+    return LCE_OK;
+}
+int linear_debug_waits(unsigned long long limit_ns, unsigned announce_extra_bytes);  // linear_api.cu's
+
 // 2-D tensor map over a row-major 16-bit matrix: `inner` contiguous elements per row, `outer`
 // rows, `pitch_bytes` between rows; 128-byte swizzle; out-of-range elements read as zero.
 // Encoding is host-only work (no driver state is touched), but it costs about a microsecond per map and

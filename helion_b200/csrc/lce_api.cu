@@ -893,10 +893,8 @@ int lce_debug_wait_test(unsigned long long limit_ns, unsigned announce_extra_byt
     if (rc) return rc;
     const unsigned long long limit = limit_ns ? limit_ns : LCE_WAIT_LIMIT_NS;
     if (cudaDeviceSynchronize() != cudaSuccess) return LCE_ERR_CUDA;
-    if (cudaMemcpyToSymbol(ptx::g_wait_limit_ns, &limit, sizeof(limit)) != cudaSuccess) return LCE_ERR_CUDA;
-    if (cudaMemcpyToSymbol(ptx::g_debug_announce_extra, &announce_extra_bytes, sizeof(unsigned)) != cudaSuccess)
-        return LCE_ERR_CUDA;
-    return LCE_OK;
+    if ((rc = set_debug_waits(limit, announce_extra_bytes))) return rc;
+    return linear_debug_waits(limit, announce_extra_bytes);
 }
 
 int lce_debug_gemm(const void* a, const void* b, float* out, int64_t M, int64_t N, int64_t K,

@@ -10,6 +10,8 @@ namespace {
 // The row pitch of what a forward saves for its backward: whole 16-byte vectors whatever the type.
 inline long long pre_pitch(long long N) { return cdiv(N, 8) * 8; }
 
+std::atomic<unsigned> g_decode_announce_extra{0};  // the decode kernel's test hook
+
 constexpr long long kDzCtas = 592;  // CTAs that the column sums of the backward aim for (4 per SM on 148 SMs, one wave)
 
 // Scratch of one product C[M, N] = A[M, K] B[N, K]^T: slabs of a split contraction.
@@ -206,7 +208,8 @@ int launch_decode(const DeviceInfo& d, const Operand& x, const Operand& w, long 
     }
     cfg.attrs = attr;
     cfg.numAttrs = n_attr;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, tm_w, tm_x, static_cast<int>(k_blocks), splits, tail, d.status_ptr);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kern, tm_w, tm_x, static_cast<int>(k_blocks), splits, tail, d.status_ptr,
+                                               g_decode_announce_extra.load(std::memory_order_relaxed));
     LCE_COUNT_LAUNCH();
     return cuda_failed(err) ? LCE_ERR_CUDA : LCE_OK;
 }
@@ -316,6 +319,12 @@ int linear_backward_impl(const DeviceInfo& d, BackwardPlan& b, const void* dy, l
 }
 
 }  // namespace
+
+int linear_debug_waits(unsigned long long limit_ns, unsigned announce_extra_bytes) {
+    g_decode_announce_extra.store(announce_extra_bytes, std::memory_order_relaxed);
+    return set_debug_waits(limit_ns, announce_extra_bytes);
+}
+
 }  // namespace lce
 
 using namespace lce;

@@ -529,6 +529,7 @@ linear_reduce_kernel(const float* scratch, int slices, long long slab_floats, in
 // tile in shared memory, and after one cluster barrier every CTA adds BN / S columns of it over the cluster in rank order
 // and runs the epilogue on them. A ring of about 100 KB lets two CTAs share an SM, so a whole wave of W is in flight.
 // Warp roles: 0 TMA producer, 1 MMA issuer and tensor-memory owner, 2-5 read the accumulator (warp w lanes 32*(w%4)..).
+// announce_extra: the test hook of ptx.cuh, as an argument: reading the variable delayed the first copy by 0.5 us.
 // ---------------------------------------------------------------------------------------------
 template <int BN>
 struct DecodeSmem {
@@ -548,7 +549,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 template <class T, int BN>
 __global__ void __launch_bounds__(kGemmThreads, 2)
 linear_decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, int k_blocks, int splits,
-                     const LinearTail<T> t, int* __restrict__ status) {
+                     const LinearTail<T> t, int* __restrict__ status, unsigned announce_extra) {
     using S = DecodeSmem<BN>;
     constexpr int kStages = S::kStages;
     constexpr uint32_t kTmemCols = BN < 32 ? 32 : BN;
@@ -593,28 +594,20 @@ linear_decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     ptx::grid_dep_launch();
     ptx::grid_dep_wait();  // nothing above touched global memory
 
+    int issued = 0;  // by the producer's lane
     if (warp == 0) {
         if (ptx::elect_one()) {
             const uint64_t keep = ptx::make_l2_policy(ptx::kL2EvictLast), stream = ptx::make_l2_policy(ptx::kL2EvictFirst);
-            int issued = 0;
-            bool ok = true;
             for (int kb = kb0; kb < kb1; ++kb, ++issued) {
                 const int s = issued % kStages;
                 if (!ptx::mbar_wait(empty(s), ((issued / kStages) & 1u) ^ 1u, abort_flag)) {
-                    ok = false;
+                    atomicCAS(status, 0, kDevErrProducerTimeout);
                     break;
                 }
                 const uint32_t sa = base + s * S::kStageBytes;
-                ptx::mbar_arrive_expect_tx(full(s), S::kStageBytes);
+                ptx::mbar_arrive_expect_tx(full(s), S::kStageBytes + (issued == 0 ? announce_extra : 0u));
                 ptx::tma_load_2d_hint(sa, &tm_w, full(s), kb * kBK, tile * kBM, stream);   // W: read once
                 ptx::tma_load_2d_hint(sa + S::kABytes, &tm_x, full(s), kb * kBK, 0, keep);  // x: every CTA reads it
-            }
-            if (!ok) {  // let the copies in flight land before the CTA retires
-                atomicCAS(status, 0, kDevErrProducerTimeout);
-                const int back = issued < kStages ? issued : kStages;
-                for (int j = 1; j <= back; ++j)
-                    for (int spin = 0; spin < (1 << 16); ++spin)
-                        if (ptx::mbar_try_wait(full((issued - j) % kStages), ((issued - j) / kStages) & 1u)) break;
             }
         }
         __syncwarp();
@@ -656,6 +649,15 @@ linear_decode_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         for (int c = 0; c < static_cast<int>(kTmemCols); c += 32) ptx::tmem_ld_32x32(taddr + c, *reinterpret_cast<float(*)[32]>(acc + c));
         ptx::tmem_ld_wait();
         ptx::tc_fence_before_sync();
+    }
+    __syncthreads();  // every wait on the ring has ended, so the flag holds still
+    if (*abort_flag) {
+        // a wait ran out: the copies in flight land (or are given the time to) before their space is used and the CTA retires
+        const int back = issued < kStages ? issued : kStages;
+        for (int j = 1; j <= back; ++j)
+            for (int spin = 0; spin < (1 << 16); ++spin)
+                if (ptx::mbar_try_wait(full((issued - j) % kStages), ((issued - j) / kStages) & 1u)) break;
+        __syncthreads();
     }
     const int n = tile * kBM + feature;
     // G tokens of feature n from token m0 on (those below m1): everything is read before anything is written.

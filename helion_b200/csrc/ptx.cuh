@@ -119,7 +119,8 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
 #endif
 
 // The limit every bounded wait uses, in nanoseconds of %globaltimer. A variable rather than a constant so
-// that a test can shorten it to a few milliseconds and watch a wait run out (read only on the slow path).
+// that a test can shorten it to a few milliseconds and watch a wait run out (read only on the slow path). Each source
+// file of the library has its own copy, as of the hook below; lce_debug_wait_test sets them all.
 __device__ unsigned long long g_wait_limit_ns = LCE_WAIT_LIMIT_NS;
 
 // Test hook, 0 in normal operation: a producer announces this many bytes MORE on its first full-barrier
