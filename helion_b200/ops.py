@@ -198,7 +198,7 @@ def _launch(what: str, device: torch.device, *args) -> None:
 def _launch_scratch(what: str, size: Callable[[], int], device: torch.device, *args, flags: int) -> None:
     """``what(*args, ws, ws_bytes, flags, stream)`` with the scratch that is there already; ``size()`` bytes are asked for
     only where the call finds it too small, which it does before it launches anything."""
-    ws = None if torch.cuda.is_current_stream_capturing() else _ws_cache.get(_ws_key(device))
+    ws = None if _capturing(device) else _ws_cache.get(_ws_key(device))
     code = _call(what, device, *args, _ptr(ws), 0 if ws is None else ws.numel(), flags)
     if code == _lib.ERR_WS_TOO_SMALL:
         ws = _workspace(size(), device)
@@ -219,6 +219,15 @@ def _ws_key(device: torch.device) -> tuple[int, int, int]:
     return (device.index if device.index is not None else torch.cuda.current_device(), _stream(device), get_ident())
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the stream that a call for ``device`` launches on is being captured; torch answers for the current device."""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """Scratch for one C-ABI call. Small requests (latency-bound problems, where an allocation is a visible
     share of the call) reuse one buffer per (device, stream, thread): the calls that a thread makes on one stream run
@@ -228,7 +237,7 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     graph keeps using its scratch whenever it is replayed, possibly beside other work of any stream, so its
     scratch has to come from the graph's own pool."""
     nbytes = max(int(nbytes), 256)
-    if nbytes > _WS_CACHE_MAX or torch.cuda.is_current_stream_capturing():
+    if nbytes > _WS_CACHE_MAX or _capturing(device):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = _ws_key(device)
     buf = _ws_cache.get(key)
