@@ -329,6 +329,6 @@ def sample_logits(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: 
         code = _DTYPE_CODE[logits.dtype]
         u = uniforms.contiguous()
         _launch("lce_sample_logits", dev, flat.data_ptr(), flat.stride(0) if rows > 1 else vocab, rows, vocab, code,
-                u.data_ptr(), _ptr(t), t_all, _ptr(k), k is not None and k.dtype is torch.int64, int(k_all),
+                u.data_ptr(), _ptr(t), t_all, _ptr(k), k is not None and k.dtype is torch.int64, int(min(k_all, vocab)),
                 _ptr(p), p_all, _ptr(m), m_all, token.data_ptr(), _ptr(logprob), None, 0)  # no scratch
     return (token, logprob) if return_logprob else token
