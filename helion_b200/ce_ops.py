@@ -14,8 +14,8 @@ from typing import Any
 import torch
 
 from . import _lib
-from .ops import (FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _check_reduction, _differentiated, _need_cuda, _need_dtype, _on_device,
-                  _stream, _workspace)
+from .ops import (FLOAT_DTYPES, INDEX_DTYPES, _DTYPE_CODE, _check_reduction, _differentiated, _launch, _need_cuda, _need_dtype,
+                  _workspace)
 
 _OP = "for tritium.cross_entropy"
 
@@ -54,13 +54,8 @@ def _forward(logits: torch.Tensor, target: torch.Tensor, reduction: str, ignore_
     L = _lib.lib()
     loss = torch.empty((n_rows,) if red == _lib.REDUCTION_NONE else (), dtype=torch.float32, device=dev)
     ws = _workspace(L.lce_ce_workspace_bytes(n_rows, vocab_size, _DTYPE_CODE[logits.dtype]), dev)
-    with _on_device(dev):
-        _lib.check(
-            L.lce_ce_forward(logits.data_ptr(), target.data_ptr(), int(target.dtype == torch.int64), n_rows, vocab_size,
-                             _DTYPE_CODE[logits.dtype], ignore_index, red, lse.data_ptr(), loss.data_ptr(), None,
-                             ws.data_ptr(), ws.numel(), _stream(dev)),
-            "lce_ce_forward",
-        )
+    _launch("lce_ce_forward", dev, logits.data_ptr(), target.data_ptr(), int(target.dtype == torch.int64), n_rows, vocab_size,
+            _DTYPE_CODE[logits.dtype], ignore_index, red, lse.data_ptr(), loss.data_ptr(), None, ws.data_ptr(), ws.numel())
     return loss, lse
 
 
@@ -93,13 +88,9 @@ def cross_entropy_backward(grad_out: torch.Tensor, logits: torch.Tensor, target:
     go = grad_out if grad_out.dtype == torch.float32 else grad_out.float()
     go = go.contiguous()
     ws = _workspace(L.lce_ce_workspace_bytes(n_rows, vocab_size, _DTYPE_CODE[logits.dtype]), dev)
-    with _on_device(dev):
-        _lib.check(
-            L.lce_ce_backward(logits.data_ptr(), target.data_ptr(), int(target.dtype == torch.int64), logsumexp.data_ptr(),
-                              go.data_ptr(), n_rows, vocab_size, _DTYPE_CODE[logits.dtype], ignore_index, red,
-                              dlogits.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dev)),
-            "lce_ce_backward",
-        )
+    _launch("lce_ce_backward", dev, logits.data_ptr(), target.data_ptr(), int(target.dtype == torch.int64), logsumexp.data_ptr(),
+            go.data_ptr(), n_rows, vocab_size, _DTYPE_CODE[logits.dtype], ignore_index, red, dlogits.data_ptr(), ws.data_ptr(),
+            ws.numel())
     return dlogits
 
 

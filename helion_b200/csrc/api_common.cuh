@@ -16,8 +16,8 @@ namespace lce {
 constexpr int kMaxDevices = 64;
 
 struct DeviceInfo {
-    bool known = false;  // sm_count and cc_major hold
-    bool ready = false;  // status_ptr and done_counters hold
+    std::atomic<bool> known{false};  // sm_count and cc_major hold
+    std::atomic<bool> ready{false};  // status_ptr and done_counters hold, and the tensor-map encoder
     int index = 0;
     int sm_count = 0;
     int cc_major = 0;
@@ -44,13 +44,13 @@ inline int device_basics(DeviceInfo** out) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return LCE_ERR_CUDA;
     if (dev < 0 || dev >= kMaxDevices) return LCE_ERR_ARG;
-    std::lock_guard<std::mutex> lock(g_mutex);
     DeviceInfo& d = g_dev[dev];
-    if (!d.known) {
+    if (!d.known.load(std::memory_order_acquire)) {
+        std::lock_guard<std::mutex> lock(g_mutex);
         d.index = dev;
         if (cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return LCE_ERR_CUDA;
         if (cudaDeviceGetAttribute(&d.cc_major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess) return LCE_ERR_CUDA;
-        d.known = true;
+        d.known.store(true, std::memory_order_release);
     }
     *out = &d;
     return d.cc_major == 10 ? LCE_OK : LCE_ERR_ARCH;

@@ -30,25 +30,26 @@ int device_info(DeviceInfo** out) {
     DeviceInfo* basics;
     const int rc = device_basics(&basics);
     if (rc) return rc;
-    std::lock_guard<std::mutex> lock(g_mutex);
     DeviceInfo& d = *basics;
-    if (!d.ready) {
+    *out = &d;
+    if (d.ready.load(std::memory_order_acquire)) return LCE_OK;
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (!d.ready.load(std::memory_order_relaxed)) {
         void* p = nullptr;
         if (cudaGetSymbolAddress(&p, g_device_status) != cudaSuccess) return LCE_ERR_CUDA;
         d.status_ptr = static_cast<int*>(p);
         if (cudaGetSymbolAddress(&p, g_done_counters) != cudaSuccess) return LCE_ERR_CUDA;
         d.done_counters = static_cast<unsigned*>(p);
-        d.ready = true;
+        if (g_encode == nullptr) {
+            void* fn = nullptr;
+            cudaDriverEntryPointQueryResult qres;
+            if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres) != cudaSuccess ||
+                qres != cudaDriverEntryPointSuccess || fn == nullptr)
+                return LCE_ERR_CUDA;
+            g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+        }
+        d.ready.store(true, std::memory_order_release);
     }
-    if (g_encode == nullptr) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult qres;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres) != cudaSuccess ||
-            qres != cudaDriverEntryPointSuccess || fn == nullptr)
-            return LCE_ERR_CUDA;
-        g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    *out = &d;
     return LCE_OK;
 }
 

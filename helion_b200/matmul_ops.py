@@ -13,8 +13,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from .ops import FLOAT_DTYPES, _DTYPE_CODE, _differentiated, _need_cuda, _need_dtype, _on_device, _path_flags, _stream, \
-    _workspace
+from .ops import FLOAT_DTYPES, _DTYPE_CODE, _differentiated, _launch, _need_cuda, _need_dtype, _path_flags, _workspace
 
 
 def _check_matmul_inputs(a: torch.Tensor, b: torch.Tensor) -> tuple[int, int, int]:
@@ -63,12 +62,8 @@ def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     dtype = _DTYPE_CODE[a.dtype]
     flags = _path_flags() & ~_lib.FLAG_FORCE_TC  # "tc" stays a preference here: fp32 has no tensor-core path
     ws = _workspace(L.lce_matmul_workspace_bytes(m, n, k, dtype, flags), dev)
-    with _on_device(dev):
-        _lib.check(
-            L.lce_matmul(a.data_ptr(), b.data_ptr(), c.data_ptr(), m, n, k, int(a_t), lda, int(not b_t), ldb, n, dtype,
-                         ws.data_ptr(), ws.numel(), flags, _stream(dev)),
-            "lce_matmul",
-        )
+    _launch("lce_matmul", dev, a.data_ptr(), b.data_ptr(), c.data_ptr(), m, n, k, int(a_t), lda, int(not b_t), ldb, n, dtype,
+            ws.data_ptr(), ws.numel(), flags)
     return c
 
 

@@ -123,10 +123,11 @@ def _check_reduction(reduction: str) -> int:
 def _differentiated(*tensors: torch.Tensor | None) -> bool:
     """Whether a call has to go through its autograd function: a gradient is asked for, or an input carries a forward-mode
     tangent, which a launch on raw pointers would drop without a word and the function refuses."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            if torch.is_grad_enabled():
                 return True
+            break
     if forward_ad._current_level < 0:  # no level is open, torch.func.jvp's included
         return False
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
@@ -150,13 +151,19 @@ def _block_bytes() -> int:
     return int(os.environ.get("HELION_B200_BLOCK_BYTES", "0"))
 
 
+# torch.cuda's queries without their Python wrappers: every call holds CUDA tensors, so that CUDA is initialised, and the
+# wrappers are a visible share of the smallest calls.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_stream_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream(device: torch.device) -> int:
     """Raw handle of torch's current stream on ``device`` (the stream every launch is enqueued on)."""
-    try:
-        return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else
-                                                  torch.cuda.current_device())
-    except AttributeError:  # older / newer torch without the private fast path
-        return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return _raw_stream(_current_device() if index is None else index)
 
 
 class _on_device:
@@ -166,7 +173,7 @@ class _on_device:
 
     def __init__(self, device: torch.device):
         self.guard = None
-        if device.index is not None and device.index != torch.cuda.current_device():
+        if device.index is not None and device.index != _current_device():
             self.guard = torch.cuda.device(device)
 
     def __enter__(self):
@@ -183,7 +190,7 @@ def _call(what: str, device: torch.device, *args) -> int:
     current for it; the lean form of ``with _on_device(...)`` for calls that take a few microseconds in all."""
     fn = getattr(_lib.lib(), what)
     index = device.index
-    if index is None or index == torch.cuda.current_device():
+    if index is None or index == _current_device():
         return fn(*args, _stream(device))
     with torch.cuda.device(device):
         return fn(*args, _stream(device))
@@ -216,16 +223,17 @@ _ws_cache: dict[tuple[int, int, int], torch.Tensor] = {}
 
 
 def _ws_key(device: torch.device) -> tuple[int, int, int]:
-    return (device.index if device.index is not None else torch.cuda.current_device(), _stream(device), get_ident())
+    index = device.index
+    return (_current_device() if index is None else index, _stream(device), get_ident())
 
 
 def _capturing(device: torch.device) -> bool:
     """Whether the stream that a call for ``device`` launches on is being captured; torch answers for the current device."""
     index = device.index
-    if index is None or index == torch.cuda.current_device():
-        return torch.cuda.is_current_stream_capturing()
+    if index is None or index == _current_device():
+        return _stream_capturing()
     with torch.cuda.device(device):
-        return torch.cuda.is_current_stream_capturing()
+        return _stream_capturing()
 
 
 def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
@@ -237,9 +245,12 @@ def _workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     graph keeps using its scratch whenever it is replayed, possibly beside other work of any stream, so its
     scratch has to come from the graph's own pool."""
     nbytes = max(int(nbytes), 256)
-    if nbytes > _WS_CACHE_MAX or _capturing(device):
+    index, current = device.index, _current_device()
+    if index is None:
+        index = current
+    if nbytes > _WS_CACHE_MAX or (_stream_capturing() if index == current else _capturing(device)):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = _ws_key(device)
+    key = (index, _raw_stream(index), get_ident())  # _ws_key
     buf = _ws_cache.get(key)
     if buf is None or buf.numel() < nbytes:
         if len(_ws_cache) >= 64:  # streams come and go: do not let the cache grow without bound
@@ -313,13 +324,9 @@ def _forward_single(hidden2d: torch.Tensor, weight: torch.Tensor, target1d: torc
     lse = torch.empty((n_rows,), dtype=torch.float32, device=dev)
     loss = torch.empty(tuple(target_shape) if red == _lib.REDUCTION_NONE else (), dtype=torch.float32, device=dev)
     ws = _workspace(L.lce_forward_loss_workspace_bytes(n_rows, hidden_size, v, dtype, flags), dev)
-    with _on_device(dev):
-        _lib.check(
-            L.lce_forward_loss(hidden2d.data_ptr(), weight.data_ptr(), target1d.data_ptr(),
-                               int(target1d.dtype == torch.int64), n_rows, hidden_size, v, dtype, ignore_index, red,
-                               lse.data_ptr(), loss.data_ptr(), None, ws.data_ptr(), ws.numel(), flags, _stream(dev)),
-            "lce_forward_loss",
-        )
+    _launch("lce_forward_loss", dev, hidden2d.data_ptr(), weight.data_ptr(), target1d.data_ptr(),
+            int(target1d.dtype == torch.int64), n_rows, hidden_size, v, dtype, ignore_index, red, lse.data_ptr(),
+            loss.data_ptr(), None, ws.data_ptr(), ws.numel(), flags)
     return loss, lse
 
 
@@ -416,15 +423,10 @@ def _backward(grad_out: torch.Tensor, hidden2d: torch.Tensor, weight: torch.Tens
 
     # the head's share of the gradient norm, summed up by the dW epilogue while it stores (no second read of dW)
     dw_sumsq = torch.empty((), dtype=torch.float32, device=dev) if (dw is not None and grad_norm.enabled()) else None
-    with _on_device(dev):
-        _lib.check(
-            L.lce_backward(hidden2d.data_ptr(), weight.data_ptr(), target1d.data_ptr(),
-                           int(target1d.dtype == torch.int64), logsumexp.data_ptr(), grad_out.data_ptr(), n_rows,
-                           hidden_size, v_local, vstart, dtype, ignore_index, red, _ptr(dx), _ptr(dw), ws.data_ptr(),
-                           ws.numel(), flags, block, event_array, ctypes.byref(scatter) if scatter is not None else None,
-                           _ptr(dw_sumsq), _stream(dev)),
-            "lce_backward",
-        )
+    _launch("lce_backward", dev, hidden2d.data_ptr(), weight.data_ptr(), target1d.data_ptr(),
+            int(target1d.dtype == torch.int64), logsumexp.data_ptr(), grad_out.data_ptr(), n_rows, hidden_size, v_local,
+            vstart, dtype, ignore_index, red, _ptr(dx), _ptr(dw), ws.data_ptr(), ws.numel(), flags, block, event_array,
+            ctypes.byref(scatter) if scatter is not None else None, _ptr(dw_sumsq))
     if dw_sumsq is not None:
         grad_norm.remember(dw, dw_sumsq)
     if peers is not None:

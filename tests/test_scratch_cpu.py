@@ -24,10 +24,10 @@ def two_devices(monkeypatch):
         finally:
             state["current"] = previous
 
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+    monkeypatch.setattr(ops, "_current_device", lambda: state["current"])
     monkeypatch.setattr(torch.cuda, "device", device)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["current"] == state["captured"])
-    monkeypatch.setattr(ops, "_stream", lambda device: 7)
+    monkeypatch.setattr(ops, "_stream_capturing", lambda: state["current"] == state["captured"])
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 7)
     monkeypatch.setattr(ops, "_ws_cache", {})
     empty = torch.empty
     monkeypatch.setattr(torch, "empty", lambda n, dtype=None, device=None: empty(n, dtype=dtype))
