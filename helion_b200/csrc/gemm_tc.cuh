@@ -458,7 +458,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         // ------------------------------------------------------------------ epilogue warps
         const int quarter = warp & 3;
         constexpr int kCols = BN / (kEpiWarps / 4);  // columns this warp handles, from col_begin
-        const int col_begin = (warp - 2) / 4 * kCols;
+        const int col_begin = kEpiWarps == 4 ? 0 : (warp - 2) / 4 * kCols;
         uint32_t local_tile = 0;
         bool ok = true;
         typename Epi::State st;
