@@ -214,13 +214,14 @@ int heads_call(const lce_head_rows* q, const lce_head_rows* k, int64_t batch, in
 constexpr long long kSampleSliceBytes = 64 << 10;       // a CTA's share of a row: two CTAs and more fit an SM
 constexpr long long kSampleMaxSliceBytes = 160 << 10;   // beyond it a CTA re-reads its share from L2
 
-// CTAs per row: enough that a share fits shared memory well and, for few rows, that the GPU is busy - as long as a share
-// is worth the cluster's barriers.
 // bf16 batches that take sample_values_kernel, a CTA per row. top_p 0.95, sample_kernel against it, us, at 128256 logits:
 // 24 rows 52 / 72, 48 rows 84 / 72, 148 rows 160 / 74, 256 rows 250 / 94; at 50257: 24 rows 37 / 49, 48 rows 61 / 49; at
 // 8003: 148 rows 27 / 32, 256 rows 47 / 35, 16384 rows 1323 / 1186; below that a row's bins cost as much as they save (4000:
-// 1055 / 1110). Rows without filters, of which sample_kernel only needs the maximum and the weights: 48 rows of 128256
-// 43 / 63, 256 rows 125 / 88, 256 rows of 50257 64 / 53, 1024 rows of 8000 57 / 84.
+// 1055 / 1110). A top_k of 50: 40 rows of 128256 37 / 41, 64 rows 47 / 41, 256 rows 98 / 53, 256 rows of 8003 36 / 25; of
+// 5000: 64 rows of 128256 67 / 59, 256 rows 171 / 80. Parameters of each row, of every kind, count as filters: 40 rows of
+// 128256 56 / 72, 64 rows 64 / 72, 148 rows 98 / 71, 256 rows 157 / 93. Rows without filters, of which sample_kernel only
+// needs the maximum and the weights: 48 rows of 128256 43 / 63, 256 rows 125 / 88, 256 rows of 50257 64 / 53, 1024 rows of
+// 8000 57 / 84.
 inline bool takes_values(long long rows, long long vocab, bool filtered) {
     return filtered ? rows >= 40 && vocab >= 8000 && rows * vocab >= 2000000 : rows >= 128 && vocab >= 32768;
 }
@@ -250,6 +251,8 @@ int launch_sample(const DeviceInfo& d, const void* logits, long long ld, long lo
         if (takes_values(rows, vocab, filtered) && groups * kSampleWarps <= kValueMaxChunks)
             return launch_sample_values(d, static_cast<const T*>(logits), ld, rows, vocab, static_cast<int>(groups), p, s);
     }
+    // CTAs per row: enough that a share fits shared memory well and, for few rows, that the GPU is busy - as long as a share
+    // is worth the cluster's barriers.
     int ctas = 1;
     while (ctas < kSampleMaxCluster &&
            (cdiv(n_vec, ctas) * 16 > kSampleSliceBytes || (rows * ctas < 2 * d.sm_count && vocab / (2 * ctas) >= 2048)))

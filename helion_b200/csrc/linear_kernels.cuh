@@ -28,7 +28,7 @@ constexpr float kGeluA = 0.044715f;
 // exponential itself would flush to zero.
 //
 // For 16-bit results (FAST) the exponential and the reciprocal are the hardware's, 1e-6 relative, and two elements share
-// an instruction where the hardware has it (fma, mul and add of fp32 pairs): at a contraction of 1024 a tile's epilogue
+// an instruction where the hardware has it (fma and mul of fp32 pairs): at a contraction of 1024 a tile's epilogue
 // has to be done in 8000 cycles of its four schedulers. The normal distribution is
 //   F(-a) = exp(-a^2 / 2) g(a),  g a polynomial in 1 / (1 + 0.26 a)
 // fitted here by reweighted least squares to 3.4e-7 of g for a up to 14 (with the exponential 2e-6 up to a = 6).

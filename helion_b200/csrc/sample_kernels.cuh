@@ -94,7 +94,7 @@ struct SampleSlot {
 
 struct SampleShared {
     uint32_t hist[2][kSampleBins];
-    double table[kSampleTable];  // 2^(i / 128)
+    double table[kSampleTable];  // 2^(i / 512)
     SampleSlot slots[2][kSampleMaxCluster];
     double wd[3][kSampleWarps];
     long long wn[1][kSampleWarps];
@@ -975,11 +975,11 @@ sample_kernel(const T* __restrict__ logits, long long ld, int vocab, int n_ctas,
 // Batches of bf16 rows, a CTA per row: a histogram with one bin per VALUE. A bin's weights are then known from its count,
 // so thresholds cost an exponential per value that occurs, nothing has to be narrowed, and the weights of the kept logits
 // are looked up. Two passes over the row: counts, then the kept weights by chunks of 1024 logits, of which one holds the
-// token. Values of a magnitude of 2^-32 and more below 1020 have bins, and zero. Masks of -1020 and below, finite or not,
-// have none: such a value weighs nothing in 64 bits where the maximum lies 700 temperatures above it. A row in which one might weigh
-// something, or with a value closer to zero or larger (one in 100000 of rounded normal values), is drawn by sample_row:
-// 64 x 128256 with a fifth of the logits at -1e4 took 308 us that way, 82 in this one (at -inf 78). 256 x 128256 with top_p 0.95: 94 us where a cluster a
-// row takes 250; 1024 rows 303 against 880. What bounds it is shared memory: one atomic per logit, and one 8-byte lookup
+// token. Values of a magnitude of 2^-32 and more below 1020 have bins, and zero. What is -1020 or less, a mask mostly, has
+// none: it weighs nothing in 64 bits where the maximum lies 700 temperatures above it. A row in which it might weigh
+// something, or with any other value (one in 100000 of rounded normal ones), is drawn by sample_row: 64 x 128256 with a
+// fifth of the logits at -1e4 took 308 us that way and takes 82 now, 78 with -inf in their place. 256 x 128256 with top_p
+// 0.95: 94 us where a cluster a row takes 250; 1024 rows 303 against 880. What bounds it is shared memory: one atomic per logit, and one 8-byte lookup
 // per kept logit; a lone CTA on an SM (up to 148 rows: 74 us) also waits for its own loads and 64-bit chains. Four vectors of
 // a lane in flight: two took 98, eight spilled and took 109. A cluster of 2 for a row, each adding up both's counts,
 // took 66 us against 74 at 64 rows and lost from 100 rows on.

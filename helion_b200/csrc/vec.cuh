@@ -103,7 +103,7 @@ __device__ __forceinline__ void rms_store(T* __restrict__ row, int c, int H, con
     }
 }
 
-// Two fp32 values that share an instruction where the hardware has one (multiply, add and fused multiply-add).
+// Two fp32 values that share an instruction where the hardware has one (multiply and fused multiply-add).
 struct Pair {
     unsigned long long v;
 };
@@ -117,11 +117,6 @@ __device__ __forceinline__ void split(Pair p, float& lo, float& hi) { asm("mov.b
 __device__ __forceinline__ Pair operator*(Pair a, Pair b) {
     Pair d;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-    Pair d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
     return d;
 }
 __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {

@@ -143,7 +143,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     ``residual`` shaped like the result; all of one type (bf16, fp16, fp32) and device. ``activation`` is ``None``,
     ``"relu"``, ``"gelu"`` (with the normal distribution function), ``"gelu_tanh"`` or ``"silu"``. Rows may have any
     pitch; inputs whose elements are not contiguous are copied first. fp32 is computed in fp32 throughout. Differentiable
-    in ``x``, ``weight``, ``bias`` and ``residual``; sums are formed in a fixed order."""
+    in ``x``, ``weight``, ``bias`` and ``residual``, not in forward mode; sums are formed in a fixed order. In fp32 relu's
+    slopes, which are stored when a gradient is asked for, do not depend on the batch that a row is in."""
     act = _check(x, weight, bias, activation, residual)
     if _differentiated(x, weight, bias, residual):
         return _Linear.apply(x, weight, bias, residual, act)

@@ -301,7 +301,8 @@ int lce_rmsnorm_backward(const void* dy, const void* x, const void* weight, cons
  * out[M, N] = act(x[M, K] w[N, K]^T + bias[N]) + residual[M, N], one rounding at the end; bias and residual may be NULL.
  * Rows have their pitches (ldx, ldw >= K; ldr, ldo >= N, in elements) and contiguous elements. `pre` (M rows of
  * N rounded up to a multiple of 8 elements, 16-byte aligned; may be NULL, ignored for LCE_ACT_NONE) receives what the
- * backward pass derives act' from: pass it on unread.
+ * backward pass derives act' from: pass it on unread. An fp32 forward with relu and `pre` does not split its
+ * contraction: the slope, the sign of z, is then that of one chain of fused multiply-adds in every batch.
  * The backward takes dy = dLoss/dout and writes dx[M, K], dw[N, K], dbias[N] (each contiguous, each may be NULL); the
  * residual's gradient is dy itself. dbias is summed in a fixed order from the unrounded dy * act', which is rounded to
  * the element type as the operand of the two products. M = 0 is a sum of nothing: dw and dbias are zeroed.
