@@ -46,13 +46,12 @@ struct SimtOperand {
                           // other operand has zeros there)
 };
 
-// How a thread fetches its share (4 elements) of a 128 x 8 operand tile:
-//   kSimtGeneric  four scalar loads with run-time strides and per-element bounds tests: any dtype,
+// How a thread fetches its share (kLoads elements) of a TS x kDepth operand tile:
+//   kSimtGeneric  scalar loads with run-time strides and per-element bounds tests: any dtype,
 //                 any alignment, any majorness (consecutive threads walk the contiguous direction);
-//   kSimtVecK     fp32, k contiguous: one 16-byte load of 4 consecutive k of one row (thread t: row t/2,
-//                 k 4*(t%2)), deposited as four conflict-free scalar stores (the tile is [k][mn]);
-//   kSimtVecMN    fp32, m/n contiguous: one 16-byte load of 4 consecutive m/n at one k (thread t: k t/32,
-//                 m/n 4*(t%32)), deposited as one 16-byte store.
+//   kSimtVecK     fp32, k contiguous: 16-byte loads of 4 consecutive k of one row, each deposited as four
+//                 scalar stores (the tile is [k][mn]);
+//   kSimtVecMN    fp32, m/n contiguous: 16-byte copies of 4 consecutive m/n at one k, which land as they are.
 // The vector modes need a 16-byte aligned base, strides and the vectorised extent in multiples of 4;
 // the host picks them (launch_simt). Row validity is settled once per tile, and the pointer just advances.
 enum SimtMode { kSimtGeneric = 0, kSimtVecK = 1, kSimtVecMN = 2 };
